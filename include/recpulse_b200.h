@@ -197,6 +197,42 @@ int rp_conv2d_backward_ex(void* grad_input, int accumulate_input, void* grad_wei
                           const void* weight, const void* col_all, void* dcol_ws, const RpbConv2d* c, DType dtype, int device_id,
                           void* stream);
 
+/* ---- additive: short causal convolution along a sequence ---------------------
+ * One filter of 1 to 8 taps per channel, as it stands in front of a recurrent scan.  RecPulse has conv2d only (ops/ops.c:
+ * 4735-4770).  x, y: [batch, len, channels] with element strides between sequences and rows and unit channel stride, so the
+ * column blocks of a projection's output are read in place:
+ *   y[b,t,d] = act(bias[d] + sum over j < width of w[d,j] * xp[b, t + j, d]),  act = identity or v / (1 + exp(-v)),
+ * xp = the width-1 rows of state_in in front of x (zeros when state_in is NULL).  w: [channels, width] packed; bias: channels
+ * elements or NULL.  state_in / state_out: [batch, width-1, channels] packed, oldest row first; state_out (or NULL) receives
+ * the last width-1 rows of xp and may be state_in.  One token per call (len = 1) with the state in place is the form for
+ * generation.  lengths: NULL, or `batch` ints in device memory; rows at and behind lengths[b] (clamped to 0 .. len) are not
+ * part of sequence b: they are not read, their y (and dx) is 0, and the state is the one after the last row in front of them.
+ * y must not overlap x (refused).  Everything is of `dtype`; sums are float32 (float64 for float64), one rounding.
+ * Asynchronous on `stream`; 0 / -1. */
+typedef struct {
+    int batch, len, channels, width;
+    int activation;                     /* 0: none, 1: SiLU */
+    long long x_batch, x_row;
+    long long y_batch, y_row;           /* of y, and of dy in the backward call */
+    long long dx_batch, dx_row;         /* backward call only */
+} RpbCausalConv;
+/* Fills `c` for packed operands. */
+void rpb_causal_conv_packed(RpbCausalConv* c, int batch, int len, int channels, int width, int activation);
+int rp_causal_conv_ex(void* y, void* state_out, const void* x, const void* w, const void* bias, const void* state_in,
+                      const int* lengths, const RpbCausalConv* c, DType dtype, int device_id, void* stream);
+/* Bytes of the workspace that the filter's gradients need; -1 for an invalid geometry. */
+long long rp_causal_conv_ws_bytes(const RpbCausalConv* c, DType dtype);
+/* The gradients, each NULL when it is not wanted: dx (strides dx_*), dw [channels, width], dbias [channels], and dstate_in.
+ * dy, and the gradient of state_out (dstate_out, NULL: zero), are given; x, w, bias, state_in and lengths as in the forward
+ * call.  `accumulate`: RPB_CONV_ACC_* bits of the outputs that are added to.  ws: rp_causal_conv_ws_bytes bytes, for this call
+ * alone (needed for dw and dbias).  The sums over rows have a fixed order. */
+#define RPB_CONV_ACC_DX 1
+#define RPB_CONV_ACC_DW 2
+#define RPB_CONV_ACC_DBIAS 4
+int rp_causal_conv_grad_ex(void* dx, void* dw, void* dbias, void* dstate_in, int accumulate, const void* dy,
+                           const void* dstate_out, const void* x, const void* w, const void* bias, const void* state_in,
+                           const int* lengths, void* ws, const RpbCausalConv* c, DType dtype, int device_id, void* stream);
+
 /* ---- additive: strided / batched GEMM on raw pointers ----------------------*/
 
 typedef struct {

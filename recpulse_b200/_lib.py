@@ -45,6 +45,11 @@ class RpbConv2d(C.Structure):
                                        "dilation_h", "dilation_w")]
 
 
+class RpbCausalConv(C.Structure):
+    _fields_ = [(f, C.c_int) for f in ("batch", "len", "channels", "width", "activation")] + \
+               [(f, C.c_longlong) for f in ("x_batch", "x_row", "y_batch", "y_row", "dx_batch", "dx_row")]
+
+
 class RpbGemm(C.Structure):
     _fields_ = [("m", C.c_int), ("n", C.c_int), ("k", C.c_int), ("batch", C.c_int), ("reduce", C.c_int),
                 ("a_row", C.c_longlong), ("a_col", C.c_longlong), ("a_batch", C.c_longlong), ("a_reduce", C.c_longlong),
@@ -80,6 +85,11 @@ SYMBOLS = {
                                        C.c_void_p]),
     "rp_conv2d_backward_ex": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                         C.POINTER(RpbConv2d), C.c_int, C.c_int, C.c_void_p]),
+    "rpb_causal_conv_packed": (None, [C.POINTER(RpbCausalConv)] + [C.c_int] * 5),
+    "rp_causal_conv_ex": (C.c_int, [C.c_void_p] * 7 + [C.POINTER(RpbCausalConv), C.c_int, C.c_int, C.c_void_p]),
+    "rp_causal_conv_ws_bytes": (C.c_longlong, [C.POINTER(RpbCausalConv), C.c_int]),
+    "rp_causal_conv_grad_ex": (C.c_int, [C.c_void_p] * 4 + [C.c_int] + [C.c_void_p] * 8 +
+                               [C.POINTER(RpbCausalConv), C.c_int, C.c_int, C.c_void_p]),
     "rp_colsum_ex": (C.c_int, [C.c_void_p, C.c_void_p, C.c_longlong, C.c_int, C.c_longlong, C.c_int, C.c_int, C.c_int,
                                C.c_void_p]),
     "rpb_gemm_packed": (None, [C.POINTER(RpbGemm), C.c_int, C.c_int, C.c_int]),

@@ -1,0 +1,194 @@
+/* Shared by the operators along a sequence (causal_conv.cu, selective_scan.cu, block_norm.cu): element types and
+ * their accumulators, vectors of channels, device selection. */
+#ifndef RPB_SEQ_COMMON_CUH
+#define RPB_SEQ_COMMON_CUH
+
+#include <cstdio>
+#include <cstring>
+#include <type_traits>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "rpb_common.h"
+
+extern "C" void rpb_count_launches(int n);      /* gemm_dispatch.cu */
+
+namespace rpb_seq {
+
+#define SEQ_CUDA(call)                                                                          \
+    do {                                                                                        \
+        cudaError_t e_ = (call);                                                                \
+        if (e_ != cudaSuccess) {                                                                \
+            fprintf(stderr, "recpulse_b200: %s failed: %s\n", #call, cudaGetErrorString(e_));   \
+            return -1;                                                                          \
+        }                                                                                       \
+    } while (0)
+
+/* Sums, states and statistics are held in float, in double for float64. */
+template <typename T> struct AccOf { typedef float type; };
+template <> struct AccOf<double> { typedef double type; };
+
+template <typename T> __device__ __forceinline__ typename AccOf<T>::type up(T v) { return (typename AccOf<T>::type)v; }
+template <> __device__ __forceinline__ float up<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float up<__half>(__half v) { return __half2float(v); }
+template <typename T, typename A> __device__ __forceinline__ T down(A v) { return (T)v; }
+template <> __device__ __forceinline__ __nv_bfloat16 down<__nv_bfloat16, float>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half down<__half, float>(float v) { return __float2half_rn(v); }
+
+/* V consecutive channels of one row, as they lie in memory. */
+template <typename T, int V> struct alignas((sizeof(T) * V) < 16 ? sizeof(T) * V : 16) Pack {
+    T v[V];
+};
+
+template <typename T, int V> __device__ __forceinline__ Pack<T, V> zero_pack() {
+    Pack<T, V> p;
+#pragma unroll
+    for (int i = 0; i < V; ++i) p.v[i] = down<T>(typename AccOf<T>::type(0));
+    return p;
+}
+
+/* Reads `valid` (<= V, may be <= 0) channels at p, zeros behind them; `vec`: p is aligned for the whole pack. */
+template <typename T, int V> __device__ __forceinline__ Pack<T, V> load_pack(const T* p, int valid, bool vec) {
+    if (vec && valid >= V) return *reinterpret_cast<const Pack<T, V>*>(p);
+    Pack<T, V> r = zero_pack<T, V>();
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (i < valid) r.v[i] = p[i];
+    return r;
+}
+template <typename T, int V> __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& r, int valid, bool vec) {
+    if (vec && valid >= V) { *reinterpret_cast<Pack<T, V>*>(p) = r; return; }
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (i < valid) p[i] = r.v[i];
+}
+
+__device__ __forceinline__ float ex2_fast(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float exp_of(float v) { return __expf(v); }
+__device__ __forceinline__ double exp_of(double v) { return exp(v); }
+
+/* 1 / (1 + exp(-v)); the quotient of a finite numerator by +inf is 0, so both ends are exact */
+__device__ __forceinline__ float logistic(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
+__device__ __forceinline__ double logistic(double v) { return 1.0 / (1.0 + exp(-v)); }
+
+/* log(1 + exp(v)) without overflow */
+__device__ __forceinline__ float softplus_of(float v) { return fmaxf(v, 0.0f) + log1pf(__expf(-fabsf(v))); }
+__device__ __forceinline__ double softplus_of(double v) { return fmax(v, 0.0) + log1p(exp(-fabs(v))); }
+
+/* Runs a call on the tensors' device and gives the caller's current device back. */
+struct DeviceScope {
+    int prev = -1; bool moved = false;
+    int enter(int device) {
+        if (cudaGetDevice(&prev) != cudaSuccess) return -1;
+        if (prev != device) { if (cudaSetDevice(device) != cudaSuccess) return -1; moved = true; }
+        return 0;
+    }
+    ~DeviceScope() { if (moved) cudaSetDevice(prev); }
+};
+
+inline int refuse(const char* what, const char* why) {
+    fprintf(stderr, "recpulse_b200: %s: %s\n", what, why);
+    return -1;
+}
+
+/* A strided [batch, len, channels] operand with unit channel stride, for the host's checks. */
+struct Rows { const void* p; long long batch, row, channels; };
+
+/* Strides of such an operand that is READ: rows of at least `channels` elements; a batch stride of 0 (one sequence for
+ * all) is allowed.  Strides that no index uses (one row, one sequence) may be anything. */
+inline bool readable(const Rows& r, int batch, int len) {
+    return (len == 1 || r.row >= r.channels) && (batch == 1 || r.batch >= 0);
+}
+/* ... and of one that is WRITTEN: no two elements at one address, sequences one after the other or row by row in turn. */
+inline bool writable(const Rows& r, int batch, int len) {
+    if (len > 1 && r.row < r.channels) return false;
+    if (batch == 1) return true;
+    if (len == 1) return r.batch >= r.channels;
+    return r.batch >= (len - 1) * r.row + r.channels || (r.batch >= r.channels && r.row >= (batch - 1) * r.batch + r.channels);
+}
+/* Whether packs of `bytes` bytes can be moved at every row of the operand. */
+inline bool aligned_rows(const Rows& r, int batch, int len, size_t es, size_t bytes) {
+    const long long size = (long long)es, step = (long long)bytes;
+    return (reinterpret_cast<uintptr_t>(r.p) % bytes) == 0 && (batch == 1 || r.batch * size % step == 0) && (len == 1 || r.row * size % step == 0);
+}
+
+/* Whether two such operands share an element.  Column blocks of one buffer (the halves of a projection's output) do not;
+ * where that cannot be seen from the strides, operands whose extents meet count as sharing. */
+inline bool overlaps(const Rows& a, const Rows& b, int batch, int len, size_t es) {
+    if (!a.p || !b.p) return false;
+    const char *a0 = reinterpret_cast<const char*>(a.p), *b0 = reinterpret_cast<const char*>(b.p);
+    const long long size = (long long)es;
+    const char* a1 = a0 + ((batch - 1) * a.batch + (len - 1) * a.row + a.channels) * size;
+    const char* b1 = b0 + ((batch - 1) * b.batch + (len - 1) * b.row + b.channels) * size;
+    if (a1 <= b0 || b1 <= a0) return false;
+    const long long unit = len > 1 ? a.row : a.batch;       /* every row of both begins a multiple of `unit` from its base */
+    if (unit <= 0 || (len > 1 && a.row != b.row)) return true;
+    if (batch > 1 && (a.batch % unit != 0 || b.batch % unit != 0)) return true;
+    const long long apart = (b0 - a0) % (unit * size);
+    const long long shift = apart < 0 ? apart + unit * size : apart;
+    return !(shift >= a.channels * size && shift + b.channels * size <= unit * size);
+}
+
+constexpr int SM_COUNT = 148;       /* of the one chip this library is written for; sizes of splits follow it */
+
+/* Sums of partial results, parts x columns, into up to three outputs: out[c] (+)= sum over parts, in a fixed order
+ * (each of 8 threads every eighth part, then the eight sums in turn), so equal inputs give equal bits. */
+struct PartSums {
+    void* out[3];                   /* NULL: not wanted */
+    long long first[3], cols[3];    /* the output's columns within a part */
+    int accumulate[3];
+    int blocks[3];
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) sum_parts_kernel(PartSums d, const typename AccOf<T>::type* __restrict__ parts, int n_parts,
+                                                        long long part_stride) {
+    typedef typename AccOf<T>::type A;
+    __shared__ A sums[8][33];
+    rpb_pdl_trigger();
+    rpb_pdl_wait();
+    int k = 0;
+    long long block = blockIdx.x;
+    while (k < 2 && block >= d.blocks[k]) block -= d.blocks[k++];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const long long col = block * 32 + tx;
+    A s = 0;
+    if (col < d.cols[k]) {
+        const A* p = parts + d.first[k] + col;
+        for (int i = ty; i < n_parts; i += 8) s += p[i * part_stride];
+    }
+    sums[ty][tx] = s;
+    __syncthreads();
+    if (ty == 0 && col < d.cols[k]) {
+#pragma unroll
+        for (int i = 1; i < 8; ++i) s += sums[i][tx];
+        T* o = reinterpret_cast<T*>(d.out[k]) + col;
+        if (d.accumulate[k]) s += up(*o);
+        *o = down<T>(s);
+    }
+}
+
+template <typename T>
+int sum_parts(PartSums d, const void* parts, int n_parts, long long part_stride, cudaStream_t s) {
+    typedef typename AccOf<T>::type A;
+    long long blocks = 0;
+    for (int k = 0; k < 3; ++k) {
+        d.blocks[k] = d.out[k] ? (int)((d.cols[k] + 31) / 32) : 0;
+        blocks += d.blocks[k];
+    }
+    if (blocks == 0) return 0;
+    SEQ_CUDA(rpb_launch(sum_parts_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, 1, d, reinterpret_cast<const A*>(parts), n_parts,
+                        part_stride));
+    rpb_count_launches(1);
+    return 0;
+}
+
+}  // namespace rpb_seq
+
+#endif

@@ -1,0 +1,242 @@
+"""rp_causal_conv_ex / rp_causal_conv_grad_ex against the definition in float64: types, widths, odd sizes, strided column
+blocks, states, lengths, accumulation, streams and graphs."""
+import ctypes as C
+
+import pytest
+import torch
+
+import recpulse_b200 as rpb
+from seq_helpers import CODE, TYPES, close, ptr, stream, unit
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def lib():
+    lib = rpb.load()
+    yield lib
+    assert lib.rpb_device_status(0) == 0
+
+
+def reference(x, w, bias, state, lengths, silu, dy=None, dstate_out=None, dtype="float32"):
+    """y, final state and gradients in float64, each with the slack its float32 (float64) arithmetic may cost."""
+    u = unit(dtype)
+    x, w = x.double().cpu(), w.double().cpu()
+    batch, length, d = x.shape
+    width = w.shape[1]
+    bias = bias.double().cpu() if bias is not None else torch.zeros(d, dtype=torch.float64)
+    ends = [min(max(int(n), 0), length) for n in lengths] if lengths is not None else [length] * batch
+    out = {k: torch.zeros_like(x) for k in ("y", "y_slack", "dx", "dx_slack")}
+    out["state"] = torch.zeros(batch, width - 1, d, dtype=torch.float64)
+    out["dstate"], out["dstate_slack"] = torch.zeros_like(out["state"]), torch.zeros_like(out["state"])
+    for k in ("dw", "dw_slack"):
+        out[k] = torch.zeros_like(w)
+    for k in ("dbias", "dbias_slack"):
+        out[k] = torch.zeros_like(bias)
+    for b, end in enumerate(ends):
+        first = state[b].double().cpu() if state is not None else torch.zeros(width - 1, d, dtype=torch.float64)
+        line = torch.cat([first, x[b, :end]])
+        out["state"][b] = line[end:]
+        taps = torch.stack([line[j:j + end] for j in range(width)], dim=-1)
+        pre = (taps * w).sum(-1) + bias
+        # width products and sums, each rounded once
+        pre_slack = (width + 1) * u * ((taps * w).abs().sum(-1) + bias.abs())
+        sig = 1 / (1 + torch.exp(-pre))
+        # exp within (4 + |v|) steps, a sum, a quotient: |d silu| <= 1.1 |d pre| + |v| s (1 - s) (4 + |v|) 2u + 4u |silu|
+        own = (pre.abs() * sig * (1 - sig) * (4 + pre.abs()) * 2 + 6 * (pre * sig).abs()) * u if silu else 0 * pre
+        out["y"][b, :end] = pre * sig if silu else pre
+        out["y_slack"][b, :end] = 1.1 * pre_slack + own
+        if dy is None:
+            continue
+        g = dy[b, :end].double().cpu()
+        slope = sig * (1 + pre * (1 - sig)) if silu else torch.ones_like(pre)
+        # |d slope / d pre| <= 0.5; its own arithmetic: a few steps of values below 2 + |v|
+        slope_slack = 0.5 * pre_slack + 16 * u * (1 + pre.abs()) * (sig * (1 - sig) * (1 + pre.abs()) + sig) if silu else 0 * pre
+        dpre, dpre_slack = g * slope, g.abs() * (slope_slack + u * slope.abs())
+        back, back_slack = torch.zeros_like(line), torch.zeros_like(line)
+        for j in range(width):
+            back[j:j + end] += w[:, j] * dpre
+            back_slack[j:j + end] += w[:, j].abs() * (dpre_slack + (width + 2) * u * dpre.abs())
+            out["dw"][:, j] += (dpre * line[j:j + end]).sum(0)
+            # a run of at most 64 rows in sequence, four runs, an eighth of the parts, eight sums: below 96 + rows / 64 steps
+            out["dw_slack"][:, j] += (line[j:j + end].abs() * (dpre_slack + (96 + batch * length / 64) * u * dpre.abs())).sum(0)
+        out["dbias"] += dpre.sum(0)
+        out["dbias_slack"] += (dpre_slack + (96 + batch * length / 64) * u * dpre.abs()).sum(0)
+        if dstate_out is not None:
+            back[end:] += dstate_out[b].double().cpu()
+            back_slack[end:] += u * dstate_out[b].double().cpu().abs()
+        out["dx"][b, :end], out["dx_slack"][b, :end] = back[width - 1:], back_slack[width - 1:]
+        out["dstate"][b], out["dstate_slack"][b] = back[:width - 1], back_slack[:width - 1]
+    return out
+
+
+def make(batch, length, d, width, dtype, seed, state=False, cols=2):
+    gen = torch.Generator().manual_seed(seed)
+    t = TYPES[dtype]
+    rand = lambda *s: torch.randn(*s, generator=gen).to(t).cuda()          # noqa: E731
+    x = rand(batch, length, cols * d)[:, :, (cols - 1) * d:]
+    return x, rand(d, width), rand(d), rand(batch, width - 1, d) if state else None, rand(batch, length, d)
+
+
+def geometry(x, width, silu, dx=None):
+    batch, length, d = x.shape
+    c = rpb.RpbCausalConv()
+    rpb.load().rpb_causal_conv_packed(C.byref(c), batch, length, d, width, silu)
+    c.x_batch, c.x_row = x.stride(0), x.stride(1)
+    if dx is not None:
+        c.dx_batch, c.dx_row = dx.stride(0), dx.stride(1)
+    return c
+
+
+def forward(lib, x, w, bias, state, lengths, c, dtype, state_out=None):
+    y = torch.full((c.batch, c.len, c.channels), float("nan"), dtype=x.dtype, device="cuda")
+    assert lib.rp_causal_conv_ex(ptr(y), ptr(state_out), ptr(x), ptr(w), ptr(bias), ptr(state), ptr(lengths), C.byref(c), CODE[dtype],
+                                 0, stream()) == 0
+    return y
+
+
+def backward(lib, dy, x, w, bias, state, lengths, c, dtype, dx, dw, dbias, dstate=None, dstate_out=None, accumulate=0):
+    ws = torch.empty(lib.rp_causal_conv_ws_bytes(C.byref(c), CODE[dtype]), dtype=torch.uint8, device="cuda")
+    assert lib.rp_causal_conv_grad_ex(ptr(dx), ptr(dw), ptr(dbias), ptr(dstate), accumulate, ptr(dy), ptr(dstate_out), ptr(x), ptr(w),
+                                      ptr(bias), ptr(state), ptr(lengths), ptr(ws), C.byref(c), CODE[dtype], 0, stream()) == 0
+
+
+SIZES = [(1, 1, 1), (2, 1, 64), (1, 2, 7), (3, 5, 33), (2, 9, 40), (1, 67, 129), (2, 130, 264), (5, 33, 8)]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("width", [1, 2, 3, 4, 5, 6, 7, 8])
+def test_forward_and_backward(lib, dtype, width):
+    for k, (batch, length, d) in enumerate(SIZES):
+        silu, with_state = (k + width) % 2, k % 3 != 0
+        x, w, bias, state, dy = make(batch, length, d, width, dtype, 100 * width + k, state=with_state, cols=1 + k % 2)
+        if k % 4 == 3:
+            bias = None
+        dstate_out = torch.randn(batch, width - 1, d, generator=torch.Generator().manual_seed(k)).to(x.dtype).cuda() if with_state else None
+        ref = reference(x, w, bias, state, None, silu, dy, dstate_out, dtype)
+        dx = torch.full((batch, length, d + 3), float("nan"), dtype=x.dtype, device="cuda")[:, :, :d]
+        c = geometry(x, width, silu, dx)
+        last = torch.full((batch, width - 1, d), float("nan"), dtype=x.dtype, device="cuda")
+        what = f"{dtype} width {width} {batch}x{length}x{d}"
+        y = forward(lib, x, w, bias, state, None, c, dtype, last)
+        close(y, ref["y"], ref["y_slack"], what + " y")
+        assert torch.equal(last.double().cpu(), ref["state"]), what
+        dw, db = torch.full_like(w, float("nan")), torch.full((d,), float("nan"), dtype=x.dtype, device="cuda")
+        ds = torch.full_like(last, float("nan"))
+        backward(lib, dy, x, w, bias, state, None, c, dtype, dx, dw, db, ds, dstate_out)
+        close(dx, ref["dx"], ref["dx_slack"], what + " dx")
+        close(dw, ref["dw"], ref["dw_slack"], what + " dw")
+        close(db, ref["dbias"], ref["dbias_slack"], what + " dbias")
+        close(ds, ref["dstate"], ref["dstate_slack"], what + " dstate")
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_lengths_of_a_padded_batch(lib, dtype):
+    """Rows behind a sequence hold infinities and NaN: nothing of them reaches an output; lengths out of range are clamped."""
+    batch, length, d, width = 7, 21, 24, 4
+    x, w, bias, state, dy = make(batch, length, d, width, dtype, 5, state=True)
+    ends = [0, 1, 2, 3, 20, 21, 21]
+    given = torch.tensor([-4, 1, 2, 3, 20, 21, 999], dtype=torch.int32, device="cuda")
+    ref = reference(x, w, bias, state, ends, 1, dy, state, dtype)
+    x, dy = x.clone(), dy.clone()
+    for b, end in enumerate(ends):
+        x[b, end:] = float("nan")
+        dy[b, end:] = float("inf")
+    c = geometry(x, width, 1)
+    last = torch.full_like(state, float("nan"))
+    close(forward(lib, x, w, bias, state, given, c, dtype, last), ref["y"], ref["y_slack"], "y")
+    assert torch.equal(last.double().cpu(), ref["state"])
+    dx, dw, db, ds = torch.full_like(x, float("nan")), torch.empty_like(w), torch.empty_like(bias), torch.empty_like(state)
+    backward(lib, dy, x, w, bias, state, given, c, dtype, dx, dw, db, ds, state)
+    for name, got in (("dx", dx), ("dw", dw), ("dbias", db), ("dstate", ds)):
+        close(got, ref[name], ref[name + "_slack"], name)
+
+
+def test_prompt_then_tokens_equals_the_whole(lib):
+    """A prompt, then single tokens with the state in place, give the bits of one call over the whole sequence."""
+    batch, length, d, width, dtype = 3, 45, 70, 4, "bfloat16"
+    x, w, bias, _, _ = make(batch, length, d, width, dtype, 8)
+    whole = forward(lib, x, w, bias, None, None, geometry(x, width, 1), dtype)
+    state = torch.empty(batch, width - 1, d, dtype=x.dtype, device="cuda")
+    got = [forward(lib, x[:, :40], w, bias, None, None, geometry(x[:, :40], width, 1), dtype, state)]
+    for t in range(40, length):
+        part = x[:, t:t + 1]
+        got.append(forward(lib, part, w, bias, state, None, geometry(part, width, 1), dtype, state))
+    assert torch.equal(torch.cat(got, dim=1), whole)
+
+
+def test_long_state_in_place_over_many_runs(lib):
+    """state_out == state_in on a sequence that many threads share: only the first run reads the old state."""
+    batch, length, d, width, dtype = 2, 700, 16, 8, "float32"
+    x, w, bias, state, _ = make(batch, length, d, width, dtype, 9, state=True)
+    ref = reference(x, w, bias, state, None, 0, dtype=dtype)
+    for _ in range(3):
+        s = state.clone()
+        close(forward(lib, x, w, bias, s, None, geometry(x, width, 0), dtype, s), ref["y"], ref["y_slack"], "y")
+        assert torch.equal(s.double().cpu(), ref["state"])
+
+
+@pytest.mark.parametrize("dtype", ["float16", "float32"])
+def test_accumulates_into_existing_gradients(lib, dtype):
+    batch, length, d, width = 2, 50, 35, 3
+    x, w, bias, _, dy = make(batch, length, d, width, dtype, 11)
+    ref = reference(x, w, bias, None, None, 1, dy, None, dtype)
+    c = geometry(x, width, 1)
+    first = {"dx": torch.randn(batch, length, d).to(x.dtype).cuda(), "dw": torch.randn(d, width).to(x.dtype).cuda(), "dbias": torch.randn(d).to(x.dtype).cuda()}
+    have = {k: v.clone() for k, v in first.items()}
+    backward(lib, dy, x, w, bias, None, None, c, dtype, have["dx"], have["dw"], have["dbias"], accumulate=7)
+    for name, got in have.items():
+        want = ref[name] + first[name].double().cpu()
+        close(got, want, ref[name + "_slack"] + unit(dtype) * want.abs(), name)
+    # one output alone, and equal inputs give equal bits
+    dx, dw = torch.empty(batch, length, d, dtype=x.dtype, device="cuda"), torch.empty_like(w)
+    backward(lib, dy, x, w, bias, None, None, c, dtype, dx, None, None)
+    backward(lib, dy, x, w, bias, None, None, c, dtype, None, dw, None)
+    close(dx, ref["dx"], ref["dx_slack"], "dx alone")
+    again = torch.empty_like(dw)
+    backward(lib, dy, x, w, bias, None, None, c, dtype, None, again, None)
+    assert torch.equal(dw, again)
+
+
+def test_gradients_against_differences(lib):
+    batch, length, d, width, dtype = 2, 6, 5, 4, "float64"
+    x, w, bias, state, dy = make(batch, length, d, width, dtype, 13, state=True, cols=1)
+    c = geometry(x, width, 1)
+    grads = [torch.empty_like(v) for v in (x, w, bias, state)]
+    backward(lib, dy, x, w, bias, state, None, c, dtype, *grads)
+    total = lambda: float((forward(lib, x, w, bias, state, None, c, dtype) * dy).sum())            # noqa: E731
+    step = 1e-5
+    for leaf, grad in zip((x, w, bias, state), grads):
+        flat, g = leaf.view(-1), grad.view(-1)
+        for i in range(0, flat.numel(), 7):
+            keep = float(flat[i])
+            flat[i] = keep + step; hi = total()
+            flat[i] = keep - step; lo = total()
+            flat[i] = keep
+            # central differences: step^2 times a third derivative of order 1, and rounding of the sums over 2 step
+            assert abs((hi - lo) / (2 * step) - float(g[i])) < 1e-8
+
+
+def test_replayed_from_a_graph_on_another_stream(lib):
+    batch, length, d, width, dtype = 2, 90, 72, 4, "bfloat16"
+    x, w, bias, _, dy = make(batch, length, d, width, dtype, 17)
+    c = geometry(x, width, 1)
+    y, dx, dw, db = torch.empty_like(dy), torch.empty_like(dy), torch.empty_like(w), torch.empty_like(bias)
+    ws = torch.empty(lib.rp_causal_conv_ws_bytes(C.byref(c), CODE[dtype]), dtype=torch.uint8, device="cuda")
+
+    def step():
+        assert lib.rp_causal_conv_ex(ptr(y), None, ptr(x), ptr(w), ptr(bias), None, None, C.byref(c), CODE[dtype], 0, stream()) == 0
+        assert lib.rp_causal_conv_grad_ex(ptr(dx), ptr(dw), ptr(db), None, 0, ptr(dy), None, ptr(x), ptr(w), ptr(bias), None, None, ptr(ws),
+                                          C.byref(c), CODE[dtype], 0, stream()) == 0
+
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        step()
+    for seed in range(2):
+        x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(seed)))
+        graph.replay()
+        torch.cuda.synchronize()
+        ref = reference(x, w, bias, None, None, 1, dy, None, dtype)
+        for name, got in (("y", y), ("dx", dx), ("dw", dw), ("dbias", db)):
+            close(got, ref[name], ref[name + "_slack"], name)
