@@ -233,6 +233,52 @@ int rp_causal_conv_grad_ex(void* dx, void* dw, void* dbias, void* dstate_in, int
                            const void* dstate_out, const void* x, const void* w, const void* bias, const void* state_in,
                            const int* lengths, void* ws, const RpbCausalConv* c, DType dtype, int device_id, void* stream);
 
+/* ---- additive: selective state space scan -------------------------------------
+ * The recurrent cell of a selective state space layer over whole sequences (RecPulse's recurrent cells, recpulse/module.py:
+ * 256-348, are stepped one token at a time).  Per sequence b and channel d a state h of `states` (1 to 64) values:
+ *   delta = dt + dt_bias, or log(1 + exp(dt + dt_bias)) when `softplus` is 1
+ *   h_t = exp(delta_t A) h_{t-1} + delta_t x_t B_t       y_t = C_t . h_t + D x_t       out_t = y_t, or y_t z_t / (1 + exp(-z_t))
+ * x, dt, z (or NULL), y: [batch, len, channels]; B, C: [batch, len, groups * states], each group shared by channels / groups
+ * neighbouring channels; all of `dtype`, with element strides between sequences and rows and unit stride within a row, so that
+ * column blocks of a projection's output are read in place.  A [channels, states], D, dt_bias [channels] (or NULL) and the
+ * states h_in, h_out [batch, channels, states] (or NULL: zeros / not wanted; h_out may be h_in) are packed float32 (float64
+ * when `dtype` is float64), and so are all sums.  One token per call (len = 1) with the state in place is the form for
+ * generation.  lengths: as in rp_causal_conv_ex; h_out is the state behind the last row in front of lengths[b].
+ * y must not overlap an operand (refused).  Asynchronous on `stream`; 0 / -1. */
+typedef struct {
+    int batch, len, channels, states, groups;
+    int softplus;
+    long long x_batch, x_row, dt_batch, dt_row, b_batch, b_row, c_batch, c_row, z_batch, z_row;
+    long long y_batch, y_row;           /* of y, and of dy in the backward call */
+    long long dx_batch, dx_row, ddt_batch, ddt_row, db_batch, db_row, dc_batch, dc_row, dz_batch, dz_row;    /* backward call only */
+} RpbScan;
+/* Fills `c` for packed operands. */
+void rpb_scan_packed(RpbScan* c, int batch, int len, int channels, int states, int groups, int softplus);
+/* float32 (float64) elements of `saved`; bytes of the workspace of the forward (grad = 0: may be 0) or backward call (grad = 1).
+ * -1 for an invalid geometry. */
+long long rp_selective_scan_saved_elems(const RpbScan* c, DType dtype);
+long long rp_selective_scan_ws_bytes(const RpbScan* c, DType dtype, int grad);
+/* saved: NULL, or where the states that the backward call starts from are kept.  ws: a workspace for this call alone. */
+int rp_selective_scan_ex(void* y, void* h_out, void* saved, const void* x, const void* dt, const void* A, const void* B,
+                         const void* C, const void* D, const void* dt_bias, const void* z, const void* h_in, const int* lengths,
+                         void* ws, const RpbScan* c, DType dtype, int device_id, void* stream);
+/* The gradients, each NULL when it is not wanted: dx, ddt, dz [batch, len, channels] and dB, dC [batch, len, groups * states]
+ * of `dtype` with strides of their own; dA, dD, ddt_bias, dh_in packed float32 (float64).  dy, and the gradient of h_out
+ * (dh_out, NULL: zero), are given; the other operands as in the forward call, `saved` as that call left it.  `accumulate`:
+ * RPB_SCAN_ACC_* bits of the outputs that are added to.  All sums have a fixed order. */
+#define RPB_SCAN_ACC_DX 1
+#define RPB_SCAN_ACC_DDT 2
+#define RPB_SCAN_ACC_DA 4
+#define RPB_SCAN_ACC_DB 8
+#define RPB_SCAN_ACC_DC 16
+#define RPB_SCAN_ACC_DD 32
+#define RPB_SCAN_ACC_DDT_BIAS 64
+#define RPB_SCAN_ACC_DZ 128
+int rp_selective_scan_grad_ex(void* dx, void* ddt, void* dA, void* dB, void* dC, void* dD, void* ddt_bias, void* dz, void* dh_in,
+                              int accumulate, const void* dy, const void* dh_out, const void* x, const void* dt, const void* A,
+                              const void* B, const void* C, const void* D, const void* dt_bias, const void* z, const int* lengths,
+                              const void* saved, void* ws, const RpbScan* c, DType dtype, int device_id, void* stream);
+
 /* ---- additive: strided / batched GEMM on raw pointers ----------------------*/
 
 typedef struct {

@@ -50,6 +50,11 @@ class RpbCausalConv(C.Structure):
                [(f, C.c_longlong) for f in ("x_batch", "x_row", "y_batch", "y_row", "dx_batch", "dx_row")]
 
 
+class RpbScan(C.Structure):
+    _fields_ = [(f, C.c_int) for f in ("batch", "len", "channels", "states", "groups", "softplus")] + \
+               [(f + end, C.c_longlong) for f in ("x", "dt", "b", "c", "z", "y", "dx", "ddt", "db", "dc", "dz") for end in ("_batch", "_row")]
+
+
 class RpbGemm(C.Structure):
     _fields_ = [("m", C.c_int), ("n", C.c_int), ("k", C.c_int), ("batch", C.c_int), ("reduce", C.c_int),
                 ("a_row", C.c_longlong), ("a_col", C.c_longlong), ("a_batch", C.c_longlong), ("a_reduce", C.c_longlong),
@@ -90,6 +95,12 @@ SYMBOLS = {
     "rp_causal_conv_ws_bytes": (C.c_longlong, [C.POINTER(RpbCausalConv), C.c_int]),
     "rp_causal_conv_grad_ex": (C.c_int, [C.c_void_p] * 4 + [C.c_int] + [C.c_void_p] * 8 +
                                [C.POINTER(RpbCausalConv), C.c_int, C.c_int, C.c_void_p]),
+    "rpb_scan_packed": (None, [C.POINTER(RpbScan)] + [C.c_int] * 6),
+    "rp_selective_scan_saved_elems": (C.c_longlong, [C.POINTER(RpbScan), C.c_int]),
+    "rp_selective_scan_ws_bytes": (C.c_longlong, [C.POINTER(RpbScan), C.c_int, C.c_int]),
+    "rp_selective_scan_ex": (C.c_int, [C.c_void_p] * 14 + [C.POINTER(RpbScan), C.c_int, C.c_int, C.c_void_p]),
+    "rp_selective_scan_grad_ex": (C.c_int, [C.c_void_p] * 9 + [C.c_int] + [C.c_void_p] * 13 +
+                                  [C.POINTER(RpbScan), C.c_int, C.c_int, C.c_void_p]),
     "rp_colsum_ex": (C.c_int, [C.c_void_p, C.c_void_p, C.c_longlong, C.c_int, C.c_longlong, C.c_int, C.c_int, C.c_int,
                                C.c_void_p]),
     "rpb_gemm_packed": (None, [C.POINTER(RpbGemm), C.c_int, C.c_int, C.c_int]),

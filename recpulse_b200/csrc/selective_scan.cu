@@ -1,0 +1,944 @@
+/*
+ * Selective state space scan: per sequence and channel a vector h of `states` values with
+ *   delta = dt + dt_bias (behind a softplus when asked for),   h_t = exp(delta A) h_{t-1} + delta x_t B_t,
+ *   y_t = C_t . h_t + D x_t,   out = y (or y z / (1 + exp(-z))).
+ * B and C are shared by the channels of a group.  Backward, with dy the gradient of y:
+ *   dh_t = C_t dy_t + a_{t+1} dh_{t+1},  a = exp(delta A);   da_t = dh_t h_{t-1} a_t (by the exponent)
+ *   dA = sum of da delta,  ddelta = sum_n (da A + dh B x),  dx = delta sum_n dh B + D dy,
+ *   dB = sum over channels of dh delta x,  dC = sum over channels of dy h,  dD = sum of dy x.
+ */
+#include "seq_common.cuh"
+
+namespace rpb_scan {
+
+using namespace rpb_seq;
+
+constexpr int NT = 128;             /* threads per block */
+constexpr int S = 4;                /* states per thread */
+constexpr int SEG = 8;              /* rows between two saved states: one backward segment, whose history is in registers */
+constexpr int MAX_STATES = 64;
+
+struct Args {
+    int batch, len, channels, states, groups, softplus;
+    long long x_batch, x_row, dt_batch, dt_row, b_batch, b_row, c_batch, c_row, z_batch, z_row, y_batch, y_row;
+    long long dx_batch, dx_row, ddt_batch, ddt_row, dz_batch, dz_row;
+    int per_group;                  /* channels of a group */
+    int blocks;                     /* channel blocks of a group */
+    int chunk, chunks;              /* rows per chunk (a multiple of the tile), and chunks per sequence */
+    bool vec_x, vec_dt, vec_z, vec_y, vec_dx, vec_ddt, vec_dz, vec_n;
+};
+
+/* P lanes per channel (4 states each), CH channels per block, tiles of TT rows: each thread loads V channels of one row of a
+ * tile, and afterwards walks the whole tile for its channel's four states. */
+template <int P> struct Shape {
+    static constexpr int CH = NT / P, TT = P <= 4 ? 8 * P : 32, V = CH * TT / NT, NP = S * P;
+    static constexpr int PAD = 32 / P;          /* rows of a [TT][CH] result are this much longer: P rows of a warp in 32 banks */
+};
+
+template <typename A> struct Pair { A delta, dx; };
+
+__device__ __forceinline__ float decay(float delta, float a) { return ex2_fast(delta * a); }
+__device__ __forceinline__ double decay(double delta, double a) { return exp(delta * a); }
+/* A as the decay wants it: in float times log2(e), for the base-2 exponential */
+__device__ __forceinline__ float decay_rate(float a) { return a * 1.44269504088896341f; }
+__device__ __forceinline__ double decay_rate(double a) { return a; }
+
+__device__ __forceinline__ int row_end(const int* lengths, int b, int len) {
+    if (!lengths) return len;
+    const int n = lengths[b];
+    return n < 0 ? 0 : n > len ? len : n;
+}
+
+/* four states from (to) a packed [.., states] row, 0 behind the last one */
+template <typename A> __device__ __forceinline__ void load_states(A (&v)[S], const A* p, int n0, int states, bool vec) {
+    const Pack<A, S> r = load_pack<A, S>(p + n0, states - n0, vec);
+#pragma unroll
+    for (int i = 0; i < S; ++i) v[i] = r.v[i];
+}
+template <typename A> __device__ __forceinline__ void store_states(A* p, const A (&v)[S], int n0, int states, bool vec) {
+    Pack<A, S> r;
+#pragma unroll
+    for (int i = 0; i < S; ++i) r.v[i] = v[i];
+    store_pack<A, S>(p + n0, r, states - n0, vec);
+}
+
+/* Sums v[0 .. G-1] over the M lanes whose numbers differ in the bits of M * UNIT - UNIT; lane m of them keeps the sums of
+ * the G / M entries from m * (G / M) on (at least one: for G < M neighbouring lanes hold the same), in v[0 ..]. */
+template <int G, int M, int UNIT, typename A> __device__ __forceinline__ void sum_lanes(A (&v)[G], int lane) {
+    int left = G;
+#pragma unroll
+    for (int m = M / 2; m >= 1; m /= 2) {
+        if (left > 1) {
+            const int half = left / 2;
+            const bool upper = lane & (m * UNIT);
+#pragma unroll
+            for (int i = 0; i < G / 2; ++i) {
+                if (i >= half) continue;
+                const A give = upper ? v[i] : v[i + half], keep = upper ? v[i + half] : v[i];
+                v[i] = keep + __shfl_xor_sync(0xffffffffu, give, m * UNIT);
+            }
+            left = half;
+        } else {
+            v[0] += __shfl_xor_sync(0xffffffffu, v[0], m * UNIT);
+        }
+    }
+}
+
+/* Where a block works: sequence, group, first channel, channels left in the group, chunk of rows. */
+struct Place { int b, g, d0, valid, c; };
+template <int CH> __device__ __forceinline__ Place place_of(const Args& a) {
+    Place p;
+    long long i = blockIdx.x;
+    const int per_seq = a.groups * a.blocks;
+    const long long sc = i / per_seq;
+    const int gb = (int)(i - sc * per_seq);
+    p.b = (int)(sc / a.chunks); p.c = (int)(sc - (long long)p.b * a.chunks);
+    p.g = gb / a.blocks;
+    const int first = (gb - p.g * a.blocks) * CH;
+    p.d0 = p.g * a.per_group + first;
+    p.valid = a.per_group - first;
+    return p;
+}
+
+template <typename T, typename A>
+__device__ __forceinline__ A delta_of(T raw, A bias, int softplus) {
+    const A v = up(raw) + bias;
+    return softplus ? softplus_of(v) : v;
+}
+
+/* ------------------------------------------------------------------------------------------------ forward
+ * AGG: the first of two passes over a long sequence that is split into chunks.  It leaves, per chunk, the state that the
+ * chunk would end with from zero and the sum of its deltas; exp(A sum) is the whole chunk's decay, so the state in front of
+ * a chunk is folded from these, and the second pass (AGG = false) runs every chunk from its own. */
+template <typename T, int P, bool AGG>
+__global__ void __launch_bounds__(NT) forward_kernel(T* __restrict__ y, typename AccOf<T>::type* h_out, typename AccOf<T>::type* __restrict__ saved,
+                                                     typename AccOf<T>::type* __restrict__ chunk_h, typename AccOf<T>::type* __restrict__ chunk_s,
+                                                     const T* __restrict__ x, const T* __restrict__ dt, const typename AccOf<T>::type* __restrict__ Am,
+                                                     const T* __restrict__ Bm, const T* __restrict__ Cm, const typename AccOf<T>::type* __restrict__ Dv,
+                                                     const typename AccOf<T>::type* __restrict__ dt_bias, const T* __restrict__ z,
+                                                     const typename AccOf<T>::type* h_in, const int* __restrict__ lengths, Args a) {
+    typedef typename AccOf<T>::type A;
+    typedef Shape<P> Sh;
+    constexpr int CH = Sh::CH, TT = Sh::TT, V = Sh::V, NP = Sh::NP, YROW = CH + Sh::PAD;
+    __shared__ __align__(16) Pair<A> pairs[TT][CH];
+    __shared__ __align__(16) A Bs[TT][NP], Cs[AGG ? 1 : TT][NP], ys[AGG ? 1 : TT][YROW];
+    rpb_pdl_trigger();
+    rpb_pdl_wait();
+    const Place pl = place_of<CH>(a);
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int end = row_end(lengths, pl.b, a.len);
+    const int first = pl.c * a.chunk, last = first + a.chunk < a.len ? first + a.chunk : a.len;
+    /* as a loader */
+    const int lr = tid / (CH / V), lc = (tid % (CH / V)) * V, lvalid = pl.valid - lc;
+    const T* xp = x + pl.b * a.x_batch + pl.d0 + lc;
+    const T* dp = dt + pl.b * a.dt_batch + pl.d0 + lc;
+    const T* zp = z ? z + pl.b * a.z_batch + pl.d0 + lc : nullptr;
+    const T* bp = Bm + pl.b * a.b_batch + pl.g * a.states;
+    const T* cp = Cm + pl.b * a.c_batch + pl.g * a.states;
+    A bias[V], skip[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        bias[i] = dt_bias && i < lvalid ? dt_bias[pl.d0 + lc + i] : A(0);
+        skip[i] = !AGG && Dv && i < lvalid ? Dv[pl.d0 + lc + i] : A(0);
+    }
+    /* as a walker */
+    const int p = tid % P, ch = tid / P, n0 = p * S;
+    const bool on = ch < pl.valid;
+    const long long d = pl.d0 + ch;
+    A rate[S], h[S], sum = 0;
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+        rate[i] = on && n0 + i < a.states ? decay_rate(Am[d * a.states + n0 + i]) : A(0);
+        h[i] = 0;
+    }
+    /* the last chunk's slot holds a copy of h_in, which h_out may overwrite while other chunks have yet to begin */
+    if (on && (a.chunks == 1 || (AGG && pl.c == a.chunks - 1))) {
+        if (h_in) load_states(h, h_in + (pl.b * (long long)a.channels + d) * a.states, n0, a.states, a.vec_n);
+        if (AGG) store_states(chunk_h + ((pl.b * (long long)a.chunks + pl.c) * a.channels + d) * a.states, h, n0, a.states, a.vec_n);
+    }
+    if (AGG && pl.c == a.chunks - 1) return;
+    if (!AGG && on && a.chunks > 1) {
+        load_states(h, chunk_h + ((pl.b * (long long)a.chunks + a.chunks - 1) * a.channels + d) * a.states, n0, a.states, a.vec_n);
+        for (int c = 0; c < pl.c; ++c) {
+            const long long at = (pl.b * (long long)a.chunks + c) * a.channels + d;
+            A part[S];
+            load_states(part, chunk_h + at * a.states, n0, a.states, a.vec_n);
+            const A s = chunk_s[at];
+#pragma unroll
+            for (int i = 0; i < S; ++i) h[i] = decay(s, rate[i]) * h[i] + part[i];
+        }
+    }
+    constexpr int BC = (TT * NP + NT - 1) / NT;
+    Pack<T, V> xr, dr, zr, xn, dn, zn;
+    T bn[BC], cn[BC];
+    auto fetch = [&](int t0) {
+        const int t = t0 + lr;
+        const bool row = t < last && t < end;
+        xn = row ? load_pack<T, V>(xp + t * a.x_row, lvalid, a.vec_x) : zero_pack<T, V>();
+        dn = row ? load_pack<T, V>(dp + t * a.dt_row, lvalid, a.vec_dt) : zero_pack<T, V>();
+        if (!AGG) zn = row && zp ? load_pack<T, V>(zp + t * a.z_row, lvalid, a.vec_z) : zero_pack<T, V>();
+#pragma unroll
+        for (int k = 0; k < BC; ++k) {
+            const int e = tid + k * NT, r = e / NP, n = e - r * NP;
+            const bool in = e < TT * NP && t0 + r < last && t0 + r < end && n < a.states;
+            bn[k] = in ? bp[(t0 + r) * a.b_row + n] : down<T>(A(0));
+            if (!AGG) cn[k] = in ? cp[(t0 + r) * a.c_row + n] : down<T>(A(0));
+        }
+    };
+    fetch(first);
+    for (int t0 = first; t0 < last; t0 += TT) {
+        xr = xn; dr = dn;
+        if (!AGG) zr = zn;
+        const bool row = t0 + lr < last && t0 + lr < end;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const A dl = row && i < lvalid ? delta_of<T, A>(dr.v[i], bias[i], a.softplus) : A(0);
+            pairs[lr][lc + i] = Pair<A>{dl, dl * up(xr.v[i])};
+        }
+#pragma unroll
+        for (int k = 0; k < BC; ++k) {
+            const int e = tid + k * NT, r = e / NP, n = e - r * NP;
+            if (e < TT * NP) {
+                Bs[r][n] = up(bn[k]);
+                if (!AGG) Cs[r][n] = up(cn[k]);
+            }
+        }
+        if (t0 + TT < last) fetch(t0 + TT);
+        __syncthreads();
+#pragma unroll(P >= 4 ? 1 : 4 / P)
+        for (int t = 0; t < TT; t += P) {
+            A v[P];
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+                if (!AGG && saved && (t + k) % SEG == 0 && on && t0 + t + k < last)
+                    store_states(saved + ((pl.b * (long long)((a.len + SEG - 1) / SEG) + (t0 + t + k) / SEG) * a.channels + d) * a.states, h, n0,
+                                 a.states, a.vec_n);
+                const Pair<A> pr = pairs[t + k][ch];
+                const Pack<A, S> bv = *reinterpret_cast<const Pack<A, S>*>(&Bs[t + k][n0]);
+                A o = 0;
+#pragma unroll
+                for (int i = 0; i < S; ++i) h[i] = decay(pr.delta, rate[i]) * h[i] + pr.dx * bv.v[i];
+                if (AGG) {
+                    sum += pr.delta;
+                } else {
+                    const Pack<A, S> cv = *reinterpret_cast<const Pack<A, S>*>(&Cs[t + k][n0]);
+#pragma unroll
+                    for (int i = 0; i < S; ++i) o += h[i] * cv.v[i];
+                }
+                v[k] = o;
+            }
+            if (!AGG) {
+                sum_lanes<P, P, 1>(v, lane);
+                ys[t + p][ch] = v[0];
+            }
+        }
+        __syncthreads();
+        if (!AGG && t0 + lr < last && lvalid > 0) {
+            Pack<T, V> o;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                A r = ys[lr][lc + i] + skip[i] * up(xr.v[i]);
+                if (zp) { const A g = up(zr.v[i]); r *= g * logistic(g); }
+                o.v[i] = down<T>(row ? r : A(0));
+            }
+            store_pack<T, V>(y + pl.b * a.y_batch + (t0 + lr) * a.y_row + pl.d0 + lc, o, lvalid, a.vec_y);
+        }
+    }
+    if (!on) return;
+    if (AGG) {
+        const long long at = (pl.b * (long long)a.chunks + pl.c) * a.channels + d;
+        store_states(chunk_h + at * a.states, h, n0, a.states, a.vec_n);
+        if (p == 0) chunk_s[at] = sum;
+    } else if (h_out && pl.c == a.chunks - 1) {
+        store_states(h_out + (pl.b * (long long)a.channels + d) * a.states, h, n0, a.states, a.vec_n);
+    }
+}
+
+/* One token per sequence: what moves is the state, once in and once out.  P lanes per channel as above; each thread takes
+ * the same channel of R sequences, so that A is read once for them and R states are on their way together. */
+template <typename T, int P, int R>
+__global__ void __launch_bounds__(256) token_kernel(T* __restrict__ y, typename AccOf<T>::type* h_out, const T* __restrict__ x, const T* __restrict__ dt,
+                                                    const typename AccOf<T>::type* __restrict__ Am, const T* __restrict__ Bm, const T* __restrict__ Cm,
+                                                    const typename AccOf<T>::type* __restrict__ Dv, const typename AccOf<T>::type* __restrict__ dt_bias,
+                                                    const T* __restrict__ z, const typename AccOf<T>::type* h_in, const int* __restrict__ lengths, Args a,
+                                                    int channel_blocks) {
+    typedef typename AccOf<T>::type A;
+    rpb_pdl_trigger();
+    rpb_pdl_wait();
+    const int group = blockIdx.x / channel_blocks;
+    const int ch = ((int)(blockIdx.x - group * channel_blocks) * (int)blockDim.x + (int)threadIdx.x) / P;
+    const int p = threadIdx.x % P, n0 = p * S, b0 = group * R;
+    const bool on = ch < a.channels;
+    const long long d = on ? ch : 0;
+    const int g = (int)(d / a.per_group);
+    A rate[S], h[R][S], xv[R], dl[R], zv[R], bv[R][S], cv[R][S];
+    bool live[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int b = b0 + r;
+        const bool in = on && b < a.batch;
+        live[r] = in && row_end(lengths, b, 1) > 0;
+#pragma unroll
+        for (int i = 0; i < S; ++i) h[r][i] = 0;
+        if (in && h_in) load_states(h[r], h_in + (b * (long long)a.channels + d) * a.states, n0, a.states, a.vec_n);
+        xv[r] = live[r] ? up(x[b * a.x_batch + d]) : A(0);
+        dl[r] = live[r] ? up(dt[b * a.dt_batch + d]) : A(0);
+        zv[r] = live[r] && z ? up(z[b * a.z_batch + d]) : A(0);
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            const bool s = live[r] && n0 + i < a.states;
+            bv[r][i] = s ? up(Bm[b * a.b_batch + g * a.states + n0 + i]) : A(0);
+            cv[r][i] = s ? up(Cm[b * a.c_batch + g * a.states + n0 + i]) : A(0);
+        }
+    }
+    load_states(rate, Am + d * a.states, n0, a.states, a.vec_n);
+    const A bias = dt_bias ? dt_bias[d] : A(0), skip = Dv ? Dv[d] : A(0);
+#pragma unroll
+    for (int i = 0; i < S; ++i) rate[i] = decay_rate(rate[i]);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int b = b0 + r;
+        A o[1] = {0};
+        if (live[r]) {
+            const A v = dl[r] + bias, delta = a.softplus ? softplus_of(v) : v, dx = delta * xv[r];
+#pragma unroll
+            for (int i = 0; i < S; ++i) {
+                h[r][i] = decay(delta, rate[i]) * h[r][i] + dx * bv[r][i];
+                o[0] += h[r][i] * cv[r][i];
+            }
+        }
+        if (on && b < a.batch && h_out) store_states(h_out + (b * (long long)a.channels + d) * a.states, h[r], n0, a.states, a.vec_n);
+        sum_lanes<1, P, 1>(o, threadIdx.x & 31);
+        if (p == 0 && on && b < a.batch) {
+            A out = o[0] + skip * xv[r];
+            if (z) out *= zv[r] * logistic(zv[r]);
+            y[b * a.y_batch + d] = down<T>(live[r] ? out : A(0));
+        }
+    }
+}
+
+/* ------------------------------------------------------------------------------------------------ backward
+ * A block walks its chunk's tiles from the last to the first.  Within a tile each thread takes segments of SEG rows: from
+ * the saved state in front of the segment it runs the rows forward once more, with the states and decays of all rows in
+ * registers, and then backward.  Sums over the states of a channel and over the channels of a warp are taken by exchanging
+ * halves between lanes, so that every lane ends with a sum of its own.
+ * AGG: as in the forward call, from the chunk's end: the gradient that leaves the chunk's first row when none enters at its
+ * end, and the sum of the deltas. */
+template <typename T, int P> struct BackwardShared {
+    typedef typename AccOf<T>::type A;
+    typedef Shape<P> Sh;
+    Pair<A> pairs[Sh::TT][Sh::CH];
+    A dys[Sh::TT][Sh::CH];
+    A Bs[Sh::TT][Sh::NP], Cs[Sh::TT][Sh::NP];
+    A q[Sh::TT][Sh::CH + Sh::PAD], r[Sh::TT][Sh::CH + Sh::PAD], yc[Sh::TT][Sh::CH + Sh::PAD];
+    A dB[NT / 32][Sh::TT][Sh::NP], dC[NT / 32][Sh::TT][Sh::NP];
+    A dD[NT][Sh::V], dbias[NT][Sh::V];
+};
+
+template <typename T> struct Grads {
+    typedef typename AccOf<T>::type A;
+    T *dx, *ddt, *dz;
+    A *dh_in, *parts, *part_b, *part_c;     /* parts: per (sequence, chunk) dA [channels, states], dD, ddt_bias [channels] */
+    int acc_dx, acc_ddt, acc_dz;
+};
+
+template <typename T, int P, bool AGG>
+__global__ void __launch_bounds__(NT) backward_kernel(Grads<T> out, typename AccOf<T>::type* __restrict__ chunk_g, typename AccOf<T>::type* __restrict__ chunk_s,
+                                                      const T* __restrict__ dy, const typename AccOf<T>::type* __restrict__ dh_out,
+                                                      const T* __restrict__ x, const T* __restrict__ dt, const typename AccOf<T>::type* __restrict__ Am,
+                                                      const T* __restrict__ Bm, const T* __restrict__ Cm, const typename AccOf<T>::type* __restrict__ Dv,
+                                                      const typename AccOf<T>::type* __restrict__ dt_bias, const T* __restrict__ z,
+                                                      const int* __restrict__ lengths, const typename AccOf<T>::type* __restrict__ saved, Args a) {
+    typedef typename AccOf<T>::type A;
+    typedef Shape<P> Sh;
+    constexpr int CH = Sh::CH, TT = Sh::TT, V = Sh::V, NP = Sh::NP;
+    extern __shared__ __align__(16) unsigned char raw_shared[];
+    BackwardShared<T, P>& sh = *reinterpret_cast<BackwardShared<T, P>*>(raw_shared);
+    rpb_pdl_trigger();
+    rpb_pdl_wait();
+    const Place pl = place_of<CH>(a);
+    if (AGG && pl.c == 0) return;       /* nothing is in front of it */
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int end = row_end(lengths, pl.b, a.len);
+    const int first = pl.c * a.chunk, last = first + a.chunk < a.len ? first + a.chunk : a.len;
+    const int lr = tid / (CH / V), lc = (tid % (CH / V)) * V, lvalid = pl.valid - lc;
+    const T* xp = x + pl.b * a.x_batch + pl.d0 + lc;
+    const T* dp = dt + pl.b * a.dt_batch + pl.d0 + lc;
+    const T* zp = z ? z + pl.b * a.z_batch + pl.d0 + lc : nullptr;
+    const T* gp = dy + pl.b * a.y_batch + pl.d0 + lc;
+    const T* bp = Bm + pl.b * a.b_batch + pl.g * a.states;
+    const T* cp = Cm + pl.b * a.c_batch + pl.g * a.states;
+    const long long segs = (a.len + SEG - 1) / SEG;
+
+    const int p = tid % P, ch = tid / P, n0 = p * S;
+    const bool on = ch < pl.valid;
+    const long long d = pl.d0 + ch;
+    A rate[S], Av[S], g[S], dA[S], sum = 0;
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+        Av[i] = on && n0 + i < a.states ? Am[d * a.states + n0 + i] : A(0);
+        rate[i] = decay_rate(Av[i]);
+        g[i] = dA[i] = 0;
+    }
+    if (!AGG && on) {
+        if (dh_out) load_states(g, dh_out + (pl.b * (long long)a.channels + d) * a.states, n0, a.states, a.vec_n);
+        for (int c = a.chunks - 1; c > pl.c; --c) {
+            const long long at = (pl.b * (long long)a.chunks + c) * a.channels + d;
+            A part[S];
+            load_states(part, chunk_g + at * a.states, n0, a.states, a.vec_n);
+            const A s = chunk_s[at];
+#pragma unroll
+            for (int i = 0; i < S; ++i) g[i] = decay(s, rate[i]) * g[i] + part[i];
+        }
+    }
+    if (!AGG) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) sh.dD[tid][i] = sh.dbias[tid][i] = 0;
+    }
+    const int tiles = (last - first + TT - 1) / TT;
+    for (int tile = tiles - 1; tile >= 0; --tile) {
+        const int t0 = first + tile * TT, t = t0 + lr;
+        const bool row = t < last && t < end;
+        {
+            const Pack<T, V> xr = row ? load_pack<T, V>(xp + t * a.x_row, lvalid, a.vec_x) : zero_pack<T, V>();
+            const Pack<T, V> dr = row ? load_pack<T, V>(dp + t * a.dt_row, lvalid, a.vec_dt) : zero_pack<T, V>();
+            const Pack<T, V> zr = row && zp ? load_pack<T, V>(zp + t * a.z_row, lvalid, a.vec_z) : zero_pack<T, V>();
+            const Pack<T, V> gr = row ? load_pack<T, V>(gp + t * a.y_row, lvalid, a.vec_y) : zero_pack<T, V>();
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const bool in = row && i < lvalid;
+                const A bias = dt_bias && in ? dt_bias[pl.d0 + lc + i] : A(0);
+                const A dl = in ? delta_of<T, A>(dr.v[i], bias, a.softplus) : A(0);
+                A gy = up(gr.v[i]);
+                if (zp) { const A zv = up(zr.v[i]); gy *= zv * logistic(zv); }
+                sh.pairs[lr][lc + i] = Pair<A>{dl, dl * up(xr.v[i])};
+                sh.dys[lr][lc + i] = in ? gy : A(0);
+            }
+            for (int e = tid; e < TT * NP; e += NT) {
+                const int r = e / NP, n = e - r * NP;
+                const bool in = t0 + r < last && t0 + r < end && n < a.states;
+                if (!AGG) sh.Bs[r][n] = in ? up(bp[(t0 + r) * a.b_row + n]) : A(0);
+                sh.Cs[r][n] = in ? up(cp[(t0 + r) * a.c_row + n]) : A(0);
+            }
+        }
+        __syncthreads();
+        if constexpr (AGG) {
+#pragma unroll 4
+            for (int k = TT - 1; k >= 0; --k) {
+                const A dl = sh.pairs[k][ch].delta, gy = sh.dys[k][ch];
+                const Pack<A, S> cv = *reinterpret_cast<const Pack<A, S>*>(&sh.Cs[k][n0]);
+                sum += dl;
+#pragma unroll
+                for (int i = 0; i < S; ++i) g[i] = (g[i] + cv.v[i] * gy) * decay(dl, rate[i]);
+            }
+        } else {
+        /* One segment; PARTIAL: rows from `live` on are not part of the sequence (or the chunk).  Their decay is 1 and nothing
+         * enters, so the state and its gradient pass through them, and their results are 0 whatever the state holds. */
+        auto segment = [&](int r0, int live, auto partial) {
+            constexpr bool PARTIAL = decltype(partial)::value;
+            A h0[S] = {0, 0, 0, 0}, av[SEG][S], h[SEG][S];
+            if (on && t0 + r0 < last) load_states(h0, saved + ((pl.b * segs + (t0 + r0) / SEG) * a.channels + d) * a.states, n0, a.states, a.vec_n);
+            A yv[SEG], qv[SEG], rv[SEG];
+#pragma unroll
+            for (int k = 0; k < SEG; ++k) {
+                const Pair<A> pr = sh.pairs[r0 + k][ch];
+                const Pack<A, S> bv = *reinterpret_cast<const Pack<A, S>*>(&sh.Bs[r0 + k][n0]);
+                const Pack<A, S> cv = *reinterpret_cast<const Pack<A, S>*>(&sh.Cs[r0 + k][n0]);
+                yv[k] = 0;
+#pragma unroll
+                for (int i = 0; i < S; ++i) {
+                    av[k][i] = decay(pr.delta, rate[i]);
+                    h[k][i] = av[k][i] * (k ? h[k - 1][i] : h0[i]) + pr.dx * bv.v[i];
+                    yv[k] += h[k][i] * cv.v[i];
+                }
+            }
+            /* M lanes of a warp hold the same states of M channels; MS rows give one sum (or more) per lane */
+            constexpr int M = 32 / P, MS = M / S < 1 ? 1 : M / S;
+            static_assert(SEG % MS == 0, "");
+            A bsum[MS * S], csum[MS * S];
+#pragma unroll
+            for (int k = SEG - 1; k >= 0; --k) {
+                const Pair<A> pr = sh.pairs[r0 + k][ch];
+                const A gy = sh.dys[r0 + k][ch];
+                const Pack<A, S> bv = *reinterpret_cast<const Pack<A, S>*>(&sh.Bs[r0 + k][n0]);
+                const Pack<A, S> cv = *reinterpret_cast<const Pack<A, S>*>(&sh.Cs[r0 + k][n0]);
+                qv[k] = rv[k] = 0;
+                if (PARTIAL && k >= live) {
+#pragma unroll
+                    for (int i = 0; i < S; ++i) bsum[(k % MS) * S + i] = csum[(k % MS) * S + i] = 0;
+                } else {
+#pragma unroll
+                for (int i = 0; i < S; ++i) {
+                    const A dh = g[i] + cv.v[i] * gy;
+                    g[i] = dh * av[k][i];
+                    const A da = g[i] * (k ? h[k - 1][i] : h0[i]);
+                    qv[k] += dh * bv.v[i];
+                    rv[k] += da * Av[i];
+                    dA[i] += da * pr.delta;
+                    bsum[(k % MS) * S + i] = dh * pr.dx;
+                    csum[(k % MS) * S + i] = gy * h[k][i];
+                }
+                }
+                if (k % MS == 0) {
+                    sum_lanes<MS * S, M, P>(bsum, lane);
+                    sum_lanes<MS * S, M, P>(csum, lane);
+                    constexpr int LEFT = MS * S / M;
+                    const int m = lane / P;
+#pragma unroll
+                    for (int e = 0; e < LEFT; ++e) {
+                        const int at = m * LEFT + e;
+                        sh.dB[warp][r0 + k + at / S][n0 + at % S] = bsum[e];
+                        sh.dC[warp][r0 + k + at / S][n0 + at % S] = csum[e];
+                    }
+                }
+            }
+            /* over the P lanes of a channel: G rows at a time, each lane left with one */
+            constexpr int G = P < SEG ? P : SEG;
+#pragma unroll
+            for (int k = 0; k < SEG; k += G) {
+                A v0[G], v1[G], v2[G];
+#pragma unroll
+                for (int i = 0; i < G; ++i) { v0[i] = qv[k + i]; v1[i] = rv[k + i]; v2[i] = yv[k + i]; }
+                sum_lanes<G, P, 1>(v0, lane);
+                sum_lanes<G, P, 1>(v1, lane);
+                if (zp) sum_lanes<G, P, 1>(v2, lane);
+                const int mine = r0 + k + p / (P / G);
+                if (p % (P / G) == 0) { sh.q[mine][ch] = v0[0]; sh.r[mine][ch] = v1[0]; if (zp) sh.yc[mine][ch] = v2[0]; }
+            }
+        };
+        const int stop = (end < last ? end : last) - t0;
+        for (int r0 = TT - SEG; r0 >= 0; r0 -= SEG) {
+            if (r0 + SEG <= stop) segment(r0, SEG, std::false_type());
+            else segment(r0, stop - r0, std::true_type());
+        }
+        __syncthreads();
+        if (t < last && lvalid > 0) {
+            const Pack<T, V> xr = row ? load_pack<T, V>(xp + t * a.x_row, lvalid, a.vec_x) : zero_pack<T, V>();
+            const Pack<T, V> dr = row ? load_pack<T, V>(dp + t * a.dt_row, lvalid, a.vec_dt) : zero_pack<T, V>();
+            const Pack<T, V> zr = row && zp ? load_pack<T, V>(zp + t * a.z_row, lvalid, a.vec_z) : zero_pack<T, V>();
+            const Pack<T, V> gr = row && zp ? load_pack<T, V>(gp + t * a.y_row, lvalid, a.vec_y) : zero_pack<T, V>();
+            T* dxp = out.dx ? out.dx + pl.b * a.dx_batch + t * a.dx_row + pl.d0 + lc : nullptr;
+            T* ddtp = out.ddt ? out.ddt + pl.b * a.ddt_batch + t * a.ddt_row + pl.d0 + lc : nullptr;
+            T* dzp = out.dz ? out.dz + pl.b * a.dz_batch + t * a.dz_row + pl.d0 + lc : nullptr;
+            Pack<T, V> o0 = zero_pack<T, V>(), o1 = o0, o2 = o0;
+            if (dxp && out.acc_dx) o0 = load_pack<T, V>(dxp, lvalid, a.vec_dx);
+            if (ddtp && out.acc_ddt) o1 = load_pack<T, V>(ddtp, lvalid, a.vec_ddt);
+            if (dzp && out.acc_dz) o2 = load_pack<T, V>(dzp, lvalid, a.vec_dz);
+            if (row) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    if (i >= lvalid) continue;
+                    const A xv = up(xr.v[i]), gy = sh.dys[lr][lc + i], q = sh.q[lr][lc + i];
+                    const A skip = Dv ? Dv[pl.d0 + lc + i] : A(0);
+                    A dd = sh.r[lr][lc + i] + xv * q;
+                    if (a.softplus) dd *= logistic(up(dr.v[i]) + (dt_bias ? dt_bias[pl.d0 + lc + i] : A(0)));
+                    o0.v[i] = down<T>(up(o0.v[i]) + sh.pairs[lr][lc + i].delta * q + skip * gy);
+                    o1.v[i] = down<T>(up(o1.v[i]) + dd);
+                    if (zp) {
+                        const A zv = up(zr.v[i]), s = logistic(zv);
+                        o2.v[i] = down<T>(up(o2.v[i]) + up(gr.v[i]) * (sh.yc[lr][lc + i] + skip * xv) * s * (A(1) + zv * (A(1) - s)));
+                    }
+                    sh.dD[tid][i] += gy * xv;
+                    sh.dbias[tid][i] += dd;
+                }
+            }
+            if (dxp) store_pack<T, V>(dxp, o0, lvalid, a.vec_dx);
+            if (ddtp) store_pack<T, V>(ddtp, o1, lvalid, a.vec_ddt);
+            if (dzp) store_pack<T, V>(dzp, o2, lvalid, a.vec_dz);
+        }
+        /* the block's part of dB and dC: the warps' sums in turn */
+        const long long rows = (long long)a.batch * a.len;
+        const int blk = (pl.d0 - pl.g * a.per_group) / CH;
+        for (int e = tid; e < TT * NP; e += NT) {
+            const int r = e / NP, n = e - r * NP;
+            if (t0 + r >= last || n >= a.states) continue;
+            const long long at = ((blk * rows + (long long)pl.b * a.len + t0 + r) * a.groups + pl.g) * a.states + n;
+            A sb = sh.dB[0][r][n], sc = sh.dC[0][r][n];
+#pragma unroll
+            for (int w = 1; w < NT / 32; ++w) { sb += sh.dB[w][r][n]; sc += sh.dC[w][r][n]; }
+            if (out.part_b) out.part_b[at] = sb;
+            if (out.part_c) out.part_c[at] = sc;
+        }
+        }
+        __syncthreads();
+    }
+    if (AGG) {
+        if (on) {
+            const long long at = (pl.b * (long long)a.chunks + pl.c) * a.channels + d;
+            store_states(chunk_g + at * a.states, g, n0, a.states, a.vec_n);
+            if (p == 0) chunk_s[at] = sum;
+        }
+        return;
+    }
+    if (on && out.dh_in && pl.c == 0) store_states(out.dh_in + (pl.b * (long long)a.channels + d) * a.states, g, n0, a.states, a.vec_n);
+    if (!out.parts) return;
+    const long long D = a.channels;
+    A* part = out.parts + (pl.b * (long long)a.chunks + pl.c) * D * (a.states + 2);
+    if (on) store_states(part + d * a.states, dA, n0, a.states, false);
+    /* the loaders' sums of one channel: one per row of a tile, in turn */
+    for (int c = tid; c < CH && c < pl.valid; c += NT) {
+        A s0 = 0, s1 = 0;
+        for (int r = 0; r < TT; ++r) {
+            const int th = r * (CH / V) + c / V;
+            s0 += sh.dD[th][c % V]; s1 += sh.dbias[th][c % V];
+        }
+        part[D * a.states + pl.d0 + c] = s0;
+        part[D * (a.states + 1) + pl.d0 + c] = s1;
+    }
+}
+
+/* dB and dC (+)= the channel blocks' parts, [parts][rows][cols] -> rows of `cols` with the output's own strides */
+template <typename T>
+__global__ void __launch_bounds__(256) sum_blocks_kernel(T* __restrict__ out0, T* __restrict__ out1, const typename AccOf<T>::type* __restrict__ part0,
+                                                         const typename AccOf<T>::type* __restrict__ part1, int n_parts, long long rows, int len, int cols,
+                                                         long long batch0, long long row0, long long batch1, long long row1, int acc0, int acc1) {
+    typedef typename AccOf<T>::type A;
+    __shared__ A sums[8][33];
+    rpb_pdl_trigger();
+    rpb_pdl_wait();
+    const bool second = blockIdx.y != 0;
+    T* out = second ? out1 : out0;
+    if (!out) return;
+    const A* part = second ? part1 : part0;
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const long long e = (long long)blockIdx.x * 32 + tx, total = rows * cols;
+    A s = 0;
+    if (e < total)
+        for (int i = ty; i < n_parts; i += 8) s += part[i * total + e];
+    sums[ty][tx] = s;
+    __syncthreads();
+    if (ty != 0 || e >= total) return;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) s += sums[i][tx];
+    const long long r = e / cols, b = r / len, t = r - b * len;
+    T* o = out + b * (second ? batch1 : batch0) + t * (second ? row1 : row0) + (e - r * cols);
+    if (second ? acc1 : acc0) s += up(*o);
+    *o = down<T>(s);
+}
+
+/* ------------------------------------------------------------------------------------------------ host */
+
+int lanes_for(int states) {
+    int p = 1;
+    while (p * S < states) p *= 2;
+    return p;
+}
+
+/* Rows per chunk.  Splitting a sequence costs a second pass over it (all of its exponentials again), so it pays only where
+ * the channels alone leave most of the chip idle. */
+int pick_chunk(const RpbScan* c) {
+    const int p = lanes_for(c->states), ch = NT / p, tt = p <= 4 ? 8 * p : 32;
+    const long long per_group = c->channels / c->groups;
+    const long long warps = (long long)c->batch * c->groups * ((per_group + ch - 1) / ch) * (NT / 32);
+    const int whole = (c->len + tt - 1) / tt * tt;
+    if (warps >= SM_COUNT * 3 || c->len < 4 * tt) return whole;
+    long long chunks = (SM_COUNT * 16 + warps - 1) / warps;
+    if (chunks > 64) chunks = 64;
+    long long chunk = (c->len + chunks - 1) / chunks;
+    if (chunk < 2 * tt) chunk = 2 * tt;
+    chunk = (chunk + tt - 1) / tt * tt;
+    return chunk >= whole ? whole : (int)chunk;
+}
+
+const char* bad_geometry(const RpbScan* c, DType dtype) {
+    if (!c) return "no geometry";
+    if (!rpb_dtype_size((int)dtype)) return "unknown element type";
+    if (c->batch <= 0 || c->len <= 0 || c->channels <= 0) return "batch, len and channels must be positive";
+    if (c->states < 1 || c->states > MAX_STATES) return "states must be 1 to 64";
+    if (c->groups < 1 || c->channels % c->groups != 0) return "groups must divide the channels";
+    if (c->softplus != 0 && c->softplus != 1) return "softplus must be 0 or 1";
+    return nullptr;
+}
+
+Args make_args(const RpbScan* c) {
+    Args a;
+    a.batch = c->batch; a.len = c->len; a.channels = c->channels; a.states = c->states; a.groups = c->groups; a.softplus = c->softplus;
+    a.x_batch = c->x_batch; a.x_row = c->x_row; a.dt_batch = c->dt_batch; a.dt_row = c->dt_row;
+    a.b_batch = c->b_batch; a.b_row = c->b_row; a.c_batch = c->c_batch; a.c_row = c->c_row;
+    a.z_batch = c->z_batch; a.z_row = c->z_row; a.y_batch = c->y_batch; a.y_row = c->y_row;
+    a.dx_batch = c->dx_batch; a.dx_row = c->dx_row; a.ddt_batch = c->ddt_batch; a.ddt_row = c->ddt_row;
+    a.dz_batch = c->dz_batch; a.dz_row = c->dz_row;
+    a.per_group = c->channels / c->groups;
+    const int ch = NT / lanes_for(c->states);
+    a.blocks = (a.per_group + ch - 1) / ch;
+    a.chunk = pick_chunk(c);
+    a.chunks = (c->len + a.chunk - 1) / a.chunk;
+    a.vec_x = a.vec_dt = a.vec_z = a.vec_y = a.vec_dx = a.vec_ddt = a.vec_dz = a.vec_n = false;
+    return a;
+}
+
+struct Rowset { Rows x, dt, B, C, z, y; };
+Rowset rows_of(const RpbScan* c, const void* x, const void* dt, const void* B, const void* C, const void* z, const void* y) {
+    const long long gn = (long long)c->groups * c->states;
+    return {{x, c->x_batch, c->x_row, c->channels}, {dt, c->dt_batch, c->dt_row, c->channels}, {B, c->b_batch, c->b_row, gn},
+            {C, c->c_batch, c->c_row, gn}, {z, c->z_batch, c->z_row, c->channels}, {y, c->y_batch, c->y_row, c->channels}};
+}
+
+/* whole packs of V channels: the rows are aligned, and so is the first channel of every block */
+template <typename T, int V> bool packs_ok(const RpbScan* c, const Rows& r) {
+    const size_t bytes = sizeof(T) * V < 16 ? sizeof(T) * V : 16;
+    return r.p && aligned_rows(r, c->batch, c->len, sizeof(T), bytes) && (c->groups == 1 || (c->channels / c->groups) % V == 0);
+}
+template <typename A> bool states_ok(const RpbScan* c, const void* p) {
+    return !p || (c->states % S == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0);
+}
+
+template <typename T>
+long long chunk_bytes(const RpbScan* c) {
+    const int chunk = pick_chunk(c);
+    const long long chunks = (c->len + chunk - 1) / chunk;
+    if (chunks == 1) return 0;
+    return ((long long)c->batch * chunks * c->channels * (c->states + 1) + 3) / 4 * 4 * (long long)sizeof(typename AccOf<T>::type);
+}
+
+template <typename T>
+long long grad_bytes(const RpbScan* c) {
+    const long long es = sizeof(typename AccOf<T>::type), chunk = pick_chunk(c), chunks = (c->len + chunk - 1) / chunk;
+    const int ch = NT / lanes_for(c->states);
+    const long long blocks = (c->channels / c->groups + ch - 1) / ch;
+    return chunk_bytes<T>(c) + es * ((long long)c->batch * chunks * c->channels * (c->states + 2) +
+                                     2 * blocks * c->batch * c->len * c->groups * c->states);
+}
+
+struct Operands {
+    const void *x, *dt, *A, *B, *C, *D, *dt_bias, *z;
+    const int* lengths;
+};
+
+template <typename T, int P>
+int forward_p(void* y, void* h_out, void* saved, const Operands& o, const void* h_in, void* ws, const RpbScan* c, cudaStream_t s) {
+    typedef typename AccOf<T>::type A;
+    typedef Shape<P> Sh;
+    Args a = make_args(c);
+    const Rowset r = rows_of(c, o.x, o.dt, o.B, o.C, o.z, y);
+    const A *Am = reinterpret_cast<const A*>(o.A), *Dv = reinterpret_cast<const A*>(o.D), *bias = reinterpret_cast<const A*>(o.dt_bias);
+    const T *x = reinterpret_cast<const T*>(o.x), *dt = reinterpret_cast<const T*>(o.dt), *B = reinterpret_cast<const T*>(o.B);
+    const T *C = reinterpret_cast<const T*>(o.C), *z = reinterpret_cast<const T*>(o.z);
+    const A* hi = reinterpret_cast<const A*>(h_in);
+    A* ho = reinterpret_cast<A*>(h_out);
+    a.vec_n = states_ok<A>(c, h_in) && states_ok<A>(c, h_out);
+    if (c->len == 1 && !saved) {
+        a.vec_n = a.vec_n && states_ok<A>(c, o.A);
+        constexpr int R = 2, BLOCK = 128;
+        const int channel_blocks = (c->channels * P + BLOCK - 1) / BLOCK;
+        const long long blocks = (long long)((c->batch + R - 1) / R) * channel_blocks;
+        if (blocks > 0x7fffffffLL) return refuse("rp_selective_scan_ex", "too many sequences for one launch");
+        SEQ_CUDA(rpb_launch(token_kernel<T, P, R>, dim3((unsigned)blocks), dim3(BLOCK), 0, s, 1, reinterpret_cast<T*>(y), ho, x, dt, Am, B, C, Dv, bias, z,
+                            hi, o.lengths, a, channel_blocks));
+        rpb_count_launches(1);
+        return 0;
+    }
+    a.vec_x = packs_ok<T, Sh::V>(c, r.x); a.vec_dt = packs_ok<T, Sh::V>(c, r.dt);
+    a.vec_z = packs_ok<T, Sh::V>(c, r.z); a.vec_y = packs_ok<T, Sh::V>(c, r.y);
+    a.vec_n = a.vec_n && states_ok<A>(c, saved) && states_ok<A>(c, ws);
+    const long long blocks = (long long)c->batch * a.chunks * c->groups * a.blocks;
+    if (blocks > 0x7fffffffLL) return refuse("rp_selective_scan_ex", "too many sequences for one launch");
+    A* chunk_h = reinterpret_cast<A*>(ws);
+    A* chunk_s = chunk_h ? chunk_h + (long long)c->batch * a.chunks * c->channels * c->states : nullptr;
+    if (a.chunks > 1) {
+        SEQ_CUDA(rpb_launch(forward_kernel<T, P, true>, dim3((unsigned)blocks), dim3(NT), 0, s, 1, reinterpret_cast<T*>(y), ho, reinterpret_cast<A*>(saved),
+                            chunk_h, chunk_s, x, dt, Am, B, C, Dv, bias, z, hi, o.lengths, a));
+        rpb_count_launches(1);
+    }
+    SEQ_CUDA(rpb_launch(forward_kernel<T, P, false>, dim3((unsigned)blocks), dim3(NT), 0, s, 1, reinterpret_cast<T*>(y), ho, reinterpret_cast<A*>(saved),
+                        chunk_h, chunk_s, x, dt, Am, B, C, Dv, bias, z, hi, o.lengths, a));
+    rpb_count_launches(1);
+    return 0;
+}
+
+struct Wanted {
+    void *dx, *ddt, *dA, *dB, *dC, *dD, *ddt_bias, *dz, *dh_in;
+    int accumulate;
+};
+
+template <typename T, int P>
+int backward_p(const Wanted& w, const void* dy, const void* dh_out, const Operands& o, const void* saved, void* ws, const RpbScan* c,
+               cudaStream_t s) {
+    typedef typename AccOf<T>::type A;
+    typedef Shape<P> Sh;
+    Args a = make_args(c);
+    const Rowset r = rows_of(c, o.x, o.dt, o.B, o.C, o.z, dy);
+    const A *Am = reinterpret_cast<const A*>(o.A), *Dv = reinterpret_cast<const A*>(o.D), *bias = reinterpret_cast<const A*>(o.dt_bias);
+    const T *x = reinterpret_cast<const T*>(o.x), *dt = reinterpret_cast<const T*>(o.dt), *B = reinterpret_cast<const T*>(o.B);
+    const T *C = reinterpret_cast<const T*>(o.C), *z = reinterpret_cast<const T*>(o.z), *g = reinterpret_cast<const T*>(dy);
+    a.vec_x = packs_ok<T, Sh::V>(c, r.x); a.vec_dt = packs_ok<T, Sh::V>(c, r.dt);
+    a.vec_z = packs_ok<T, Sh::V>(c, r.z); a.vec_y = packs_ok<T, Sh::V>(c, r.y);
+    a.vec_dx = packs_ok<T, Sh::V>(c, {w.dx, c->dx_batch, c->dx_row, c->channels});
+    a.vec_ddt = packs_ok<T, Sh::V>(c, {w.ddt, c->ddt_batch, c->ddt_row, c->channels});
+    a.vec_dz = packs_ok<T, Sh::V>(c, {w.dz, c->dz_batch, c->dz_row, c->channels});
+    a.vec_n = states_ok<A>(c, saved) && states_ok<A>(c, ws) && states_ok<A>(c, dh_out) && states_ok<A>(c, w.dh_in);
+    const long long blocks = (long long)c->batch * a.chunks * c->groups * a.blocks;
+    if (blocks > 0x7fffffffLL) return refuse("rp_selective_scan_grad_ex", "too many sequences for one launch");
+    const long long rows = (long long)c->batch * c->len, cols = (long long)c->groups * c->states;
+    A* chunk_g = reinterpret_cast<A*>(ws);
+    A* chunk_s = chunk_g + (long long)c->batch * a.chunks * c->channels * c->states;
+    A* parts = reinterpret_cast<A*>(reinterpret_cast<char*>(ws) + chunk_bytes<T>(c));
+    A* part_b = parts + (long long)c->batch * a.chunks * c->channels * (c->states + 2);
+    A* part_c = part_b + a.blocks * rows * cols;
+    Grads<T> out;
+    out.dx = reinterpret_cast<T*>(w.dx); out.ddt = reinterpret_cast<T*>(w.ddt); out.dz = reinterpret_cast<T*>(w.dz);
+    out.dh_in = reinterpret_cast<A*>(w.dh_in);
+    out.parts = w.dA || w.dD || w.ddt_bias ? parts : nullptr;
+    out.part_b = w.dB ? part_b : nullptr; out.part_c = w.dC ? part_c : nullptr;
+    out.acc_dx = (w.accumulate & RPB_SCAN_ACC_DX) != 0; out.acc_ddt = (w.accumulate & RPB_SCAN_ACC_DDT) != 0;
+    out.acc_dz = (w.accumulate & RPB_SCAN_ACC_DZ) != 0;
+    const size_t smem = sizeof(BackwardShared<T, P>);
+    if (smem > 48 * 1024) {
+        SEQ_CUDA(cudaFuncSetAttribute(backward_kernel<T, P, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        SEQ_CUDA(cudaFuncSetAttribute(backward_kernel<T, P, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    }
+    const A* dho = reinterpret_cast<const A*>(dh_out);
+    const A* sv = reinterpret_cast<const A*>(saved);
+    if (a.chunks > 1) {
+        SEQ_CUDA(rpb_launch(backward_kernel<T, P, true>, dim3((unsigned)blocks), dim3(NT), smem, s, 1, out, chunk_g, chunk_s, g, dho, x, dt, Am, B, C, Dv, bias,
+                            z, o.lengths, sv, a));
+        rpb_count_launches(1);
+    }
+    SEQ_CUDA(rpb_launch(backward_kernel<T, P, false>, dim3((unsigned)blocks), dim3(NT), smem, s, 1, out, chunk_g, chunk_s, g, dho, x, dt, Am, B, C, Dv, bias, z,
+                        o.lengths, sv, a));
+    rpb_count_launches(1);
+    if (w.dB || w.dC) {
+        const long long sum_blocks = (rows * cols + 31) / 32;
+        if (sum_blocks > 0x7fffffffLL) return refuse("rp_selective_scan_grad_ex", "too many rows for one launch");
+        SEQ_CUDA(rpb_launch(sum_blocks_kernel<T>, dim3((unsigned)sum_blocks, 2), dim3(256), 0, s, 1, reinterpret_cast<T*>(w.dB), reinterpret_cast<T*>(w.dC),
+                            (const A*)part_b, (const A*)part_c, a.blocks, rows, c->len, (int)cols, c->db_batch, c->db_row, c->dc_batch, c->dc_row,
+                            (w.accumulate & RPB_SCAN_ACC_DB) != 0, (w.accumulate & RPB_SCAN_ACC_DC) != 0));
+        rpb_count_launches(1);
+    }
+    if (!out.parts) return 0;
+    const long long D = c->channels, N = c->states;
+    PartSums d = {};
+    d.out[0] = w.dA; d.first[0] = 0; d.cols[0] = D * N; d.accumulate[0] = (w.accumulate & RPB_SCAN_ACC_DA) != 0;
+    d.out[1] = w.dD; d.first[1] = D * N; d.cols[1] = D; d.accumulate[1] = (w.accumulate & RPB_SCAN_ACC_DD) != 0;
+    d.out[2] = w.ddt_bias; d.first[2] = D * (N + 1); d.cols[2] = D; d.accumulate[2] = (w.accumulate & RPB_SCAN_ACC_DDT_BIAS) != 0;
+    return sum_parts<A>(d, parts, c->batch * a.chunks, D * (N + 2), s);
+}
+
+template <typename F> int by_lanes(int states, F f) {
+    switch (lanes_for(states)) {
+        case 1: return f(std::integral_constant<int, 1>());
+        case 2: return f(std::integral_constant<int, 2>());
+        case 4: return f(std::integral_constant<int, 4>());
+        case 8: return f(std::integral_constant<int, 8>());
+        case 16: return f(std::integral_constant<int, 16>());
+    }
+    return -1;
+}
+
+template <typename F> int by_type(DType dtype, F f) {
+    switch ((int)dtype) {
+        case DTYPE_FLOAT32: return f(float());
+        case DTYPE_FLOAT64: return f(double());
+        case DTYPE_FLOAT16: return f(__half());
+        case DTYPE_BFLOAT16: return f(__nv_bfloat16());
+    }
+    return -1;
+}
+
+/* what both directions check about the operands that they read */
+const char* bad_operands(const RpbScan* c, const Rowset& r, const Operands& o, bool z_given) {
+    if (!o.x || !o.dt || !o.A || !o.B || !o.C) return "x, dt, A, B and C are needed";
+    if (!readable(r.x, c->batch, c->len)) return "strides of x";
+    if (!readable(r.dt, c->batch, c->len)) return "strides of dt";
+    if (!readable(r.B, c->batch, c->len)) return "strides of B";
+    if (!readable(r.C, c->batch, c->len)) return "strides of C";
+    if (z_given && !readable(r.z, c->batch, c->len)) return "strides of z";
+    return nullptr;
+}
+
+bool meets_any(const RpbScan* c, const Rows& w, const Rowset& r, size_t es, bool with_y) {
+    return overlaps(w, r.x, c->batch, c->len, es) || overlaps(w, r.dt, c->batch, c->len, es) || overlaps(w, r.B, c->batch, c->len, es) ||
+           overlaps(w, r.C, c->batch, c->len, es) || overlaps(w, r.z, c->batch, c->len, es) || (with_y && overlaps(w, r.y, c->batch, c->len, es));
+}
+
+}  // namespace rpb_scan
+
+using namespace rpb_seq;
+using namespace rpb_scan;
+
+extern "C" {
+
+void rpb_scan_packed(RpbScan* c, int batch, int len, int channels, int states, int groups, int softplus) {
+    memset(c, 0, sizeof(*c));
+    c->batch = batch; c->len = len; c->channels = channels; c->states = states; c->groups = groups; c->softplus = softplus;
+    c->x_row = c->dt_row = c->z_row = c->y_row = c->dx_row = c->ddt_row = c->dz_row = channels;
+    c->x_batch = c->dt_batch = c->z_batch = c->y_batch = c->dx_batch = c->ddt_batch = c->dz_batch = (long long)len * channels;
+    c->b_row = c->c_row = c->db_row = c->dc_row = (long long)groups * states;
+    c->b_batch = c->c_batch = c->db_batch = c->dc_batch = (long long)len * groups * states;
+}
+
+long long rp_selective_scan_saved_elems(const RpbScan* c, DType dtype) {
+    const char* why = bad_geometry(c, dtype);
+    if (why) return refuse("rp_selective_scan_saved_elems", why);
+    return (long long)c->batch * ((c->len + SEG - 1) / SEG) * c->channels * c->states;
+}
+
+long long rp_selective_scan_ws_bytes(const RpbScan* c, DType dtype, int grad) {
+    const char* why = bad_geometry(c, dtype);
+    if (why) return refuse("rp_selective_scan_ws_bytes", why);
+    if ((int)dtype == DTYPE_FLOAT64) return grad ? grad_bytes<double>(c) : chunk_bytes<double>(c);
+    return grad ? grad_bytes<float>(c) : chunk_bytes<float>(c);
+}
+
+int rp_selective_scan_ex(void* y, void* h_out, void* saved, const void* x, const void* dt, const void* A, const void* B, const void* C, const void* D,
+                         const void* dt_bias, const void* z, const void* h_in, const int* lengths, void* ws, const RpbScan* c, DType dtype,
+                         int device_id, void* stream) {
+    const char* name = "rp_selective_scan_ex";
+    const char* why = bad_geometry(c, dtype);
+    if (why) return refuse(name, why);
+    if (!y) return refuse(name, "y is needed");
+    if (device_id < 0) return refuse(name, "needs a CUDA device (no CPU path in this library)");
+    const Operands o = {x, dt, A, B, C, D, dt_bias, z, lengths};
+    const Rowset r = rows_of(c, x, dt, B, C, z, y);
+    why = bad_operands(c, r, o, z != nullptr);
+    if (why) return refuse(name, why);
+    if (!writable(r.y, c->batch, c->len)) return refuse(name, "strides of y");
+    if (meets_any(c, r.y, r, rpb_dtype_size((int)dtype), false)) return refuse(name, "y overlaps an operand");
+    if (!ws && rp_selective_scan_ws_bytes(c, dtype, 0) > 0) return refuse(name, "this size needs a workspace");
+    if (saved && (saved == h_in || saved == h_out || saved == ws)) return refuse(name, "saved overlaps another buffer");
+    DeviceScope scope;
+    if (scope.enter(device_id)) return refuse(name, "no such device");
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    return by_type(dtype, [&](auto t) {
+        return by_lanes(c->states, [&](auto p) { return forward_p<decltype(t), decltype(p)::value>(y, h_out, saved, o, h_in, ws, c, s); });
+    });
+}
+
+int rp_selective_scan_grad_ex(void* dx, void* ddt, void* dA, void* dB, void* dC, void* dD, void* ddt_bias, void* dz, void* dh_in, int accumulate,
+                              const void* dy, const void* dh_out, const void* x, const void* dt, const void* A, const void* B, const void* C,
+                              const void* D, const void* dt_bias, const void* z, const int* lengths, const void* saved, void* ws, const RpbScan* c,
+                              DType dtype, int device_id, void* stream) {
+    const char* name = "rp_selective_scan_grad_ex";
+    const char* why = bad_geometry(c, dtype);
+    if (why) return refuse(name, why);
+    if (!dx && !ddt && !dA && !dB && !dC && !dD && !ddt_bias && !dz && !dh_in) return refuse(name, "no gradient is wanted");
+    if (!dy || !saved || !ws) return refuse(name, "dy, the saved states of the forward call and a workspace are needed");
+    if (dz && !z) return refuse(name, "dz without z");
+    if (device_id < 0) return refuse(name, "needs a CUDA device (no CPU path in this library)");
+    const Operands o = {x, dt, A, B, C, D, dt_bias, z, lengths};
+    const Rowset r = rows_of(c, x, dt, B, C, z, dy);
+    why = bad_operands(c, r, o, z != nullptr);
+    if (why) return refuse(name, why);
+    if (!readable(r.y, c->batch, c->len)) return refuse(name, "strides of dy");
+    const long long gn = (long long)c->groups * c->states;
+    const Rows w[5] = {{dx, c->dx_batch, c->dx_row, c->channels}, {ddt, c->ddt_batch, c->ddt_row, c->channels}, {dz, c->dz_batch, c->dz_row, c->channels},
+                       {dB, c->db_batch, c->db_row, gn}, {dC, c->dc_batch, c->dc_row, gn}};
+    const size_t es = rpb_dtype_size((int)dtype);
+    for (int i = 0; i < 5; ++i) {
+        if (!w[i].p) continue;
+        if (!writable(w[i], c->batch, c->len)) return refuse(name, "strides of a gradient");
+        if (meets_any(c, w[i], r, es, true)) return refuse(name, "a gradient overlaps an operand");
+        for (int k = 0; k < i; ++k)
+            if (overlaps(w[i], w[k], c->batch, c->len, es)) return refuse(name, "two gradients overlap");
+    }
+    if (dh_in && dh_in == dh_out) return refuse(name, "dh_in overlaps dh_out");
+    DeviceScope scope;
+    if (scope.enter(device_id)) return refuse(name, "no such device");
+    const Wanted want = {dx, ddt, dA, dB, dC, dD, ddt_bias, dz, dh_in, accumulate};
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    return by_type(dtype, [&](auto t) {
+        return by_lanes(c->states, [&](auto p) { return backward_p<decltype(t), decltype(p)::value>(want, dy, dh_out, o, saved, ws, c, s); });
+    });
+}
+
+}  // extern "C"
