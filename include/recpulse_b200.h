@@ -279,6 +279,43 @@ int rp_selective_scan_grad_ex(void* dx, void* ddt, void* dA, void* dB, void* dC,
                               const void* B, const void* C, const void* D, const void* dt_bias, const void* z, const int* lengths,
                               const void* saved, void* ws, const RpbScan* c, DType dtype, int device_id, void* stream);
 
+/* ---- additive: the norms around a block ----------------------------------------
+ * What stands between two blocks of a residual network, one pass over each row of [rows, channels] (up to 16384 channels):
+ *   v = u z / (1 + exp(-z))   (z NULL: u)                       the block's output behind its gate
+ *   s = v / sqrt(mean v^2 + eps_after) * w_after   (NULL: v)     the norm after the block
+ *   out = r + scale * s       (scale NULL: 1, r NULL: 0)         the residual stream, scale per channel
+ *   y = out / sqrt(mean out^2 + eps_before) * w_before           the norm before the next block
+ * out or y may be NULL (not wanted); w_before is needed for y.  y is computed from the sum before its rounding.  Everything is
+ * of `dtype`; means and sums are float32 (float64), each output is rounded once.  Row strides in elements, channel stride 1;
+ * weights packed.  out and y must not overlap an operand or one another (refused).  Asynchronous on `stream`; 0 / -1. */
+typedef struct {
+    long long rows;
+    int channels;
+    float eps_after, eps_before;
+    long long u_row, z_row, r_row;
+    long long out_row, y_row;           /* of out and y, and of dout and dy in the backward call */
+    long long du_row, dz_row, dr_row;   /* backward call only */
+} RpbBlockNorm;
+/* Fills `c` for packed operands and one eps. */
+void rpb_block_norm_packed(RpbBlockNorm* c, long long rows, int channels, float eps);
+int rp_block_norm_ex(void* out, void* y, const void* u, const void* z, const void* w_after, const void* scale, const void* r,
+                     const void* w_before, const RpbBlockNorm* c, DType dtype, int device_id, void* stream);
+/* Bytes of the workspace that the weights' gradients need; -1 for an invalid geometry. */
+long long rp_block_norm_ws_bytes(const RpbBlockNorm* c, DType dtype);
+/* The gradients, each NULL when it is not wanted, from dout and / or dy (NULL: zero).  `accumulate`: RPB_NORM_ACC_* bits of the
+ * outputs that are added to.  ws: rp_block_norm_ws_bytes bytes, for this call alone (needed for the weights' gradients).  The
+ * sums over rows have a fixed order. */
+#define RPB_NORM_ACC_DU 1
+#define RPB_NORM_ACC_DZ 2
+#define RPB_NORM_ACC_DR 4
+#define RPB_NORM_ACC_DW_AFTER 8
+#define RPB_NORM_ACC_DSCALE 16
+#define RPB_NORM_ACC_DW_BEFORE 32
+int rp_block_norm_grad_ex(void* du, void* dz, void* dr, void* dw_after, void* dscale, void* dw_before, int accumulate,
+                          const void* dout, const void* dy, const void* u, const void* z, const void* w_after, const void* scale,
+                          const void* r, const void* w_before, void* ws, const RpbBlockNorm* c, DType dtype, int device_id,
+                          void* stream);
+
 /* ---- additive: strided / batched GEMM on raw pointers ----------------------*/
 
 typedef struct {

@@ -55,6 +55,11 @@ class RpbScan(C.Structure):
                [(f + end, C.c_longlong) for f in ("x", "dt", "b", "c", "z", "y", "dx", "ddt", "db", "dc", "dz") for end in ("_batch", "_row")]
 
 
+class RpbBlockNorm(C.Structure):
+    _fields_ = [("rows", C.c_longlong), ("channels", C.c_int), ("eps_after", C.c_float), ("eps_before", C.c_float)] + \
+               [(f + "_row", C.c_longlong) for f in ("u", "z", "r", "out", "y", "du", "dz", "dr")]
+
+
 class RpbGemm(C.Structure):
     _fields_ = [("m", C.c_int), ("n", C.c_int), ("k", C.c_int), ("batch", C.c_int), ("reduce", C.c_int),
                 ("a_row", C.c_longlong), ("a_col", C.c_longlong), ("a_batch", C.c_longlong), ("a_reduce", C.c_longlong),
@@ -101,6 +106,11 @@ SYMBOLS = {
     "rp_selective_scan_ex": (C.c_int, [C.c_void_p] * 14 + [C.POINTER(RpbScan), C.c_int, C.c_int, C.c_void_p]),
     "rp_selective_scan_grad_ex": (C.c_int, [C.c_void_p] * 9 + [C.c_int] + [C.c_void_p] * 13 +
                                   [C.POINTER(RpbScan), C.c_int, C.c_int, C.c_void_p]),
+    "rpb_block_norm_packed": (None, [C.POINTER(RpbBlockNorm), C.c_longlong, C.c_int, C.c_float]),
+    "rp_block_norm_ex": (C.c_int, [C.c_void_p] * 8 + [C.POINTER(RpbBlockNorm), C.c_int, C.c_int, C.c_void_p]),
+    "rp_block_norm_ws_bytes": (C.c_longlong, [C.POINTER(RpbBlockNorm), C.c_int]),
+    "rp_block_norm_grad_ex": (C.c_int, [C.c_void_p] * 6 + [C.c_int] + [C.c_void_p] * 9 +
+                              [C.POINTER(RpbBlockNorm), C.c_int, C.c_int, C.c_void_p]),
     "rp_colsum_ex": (C.c_int, [C.c_void_p, C.c_void_p, C.c_longlong, C.c_int, C.c_longlong, C.c_int, C.c_int, C.c_int,
                                C.c_void_p]),
     "rpb_gemm_packed": (None, [C.POINTER(RpbGemm), C.c_int, C.c_int, C.c_int]),

@@ -56,3 +56,100 @@ def test_convolution_refuses_bad_calls():
     assert grad(at(30000), None, at(20000), None, y, x) == -1      # dstate_in over dstate_out
     assert lib.rp_causal_conv_ws_bytes(None, 0) == -1 and lib.rp_causal_conv_ws_bytes(C.byref(c), 7) == -1
     assert lib.rp_causal_conv_ws_bytes(C.byref(c), 0) > 0
+
+
+def scan(batch=2, length=5, channels=8, states=4, groups=2, softplus=1, **over):
+    c = rpb.RpbScan()
+    rpb.load().rpb_scan_packed(C.byref(c), batch, length, channels, states, groups, softplus)
+    for k, v in over.items():
+        setattr(c, k, v)
+    return c
+
+
+def test_packed_scan_geometry_and_sizes():
+    lib, c = rpb.load(), scan()
+    assert (c.x_batch, c.x_row, c.b_batch, c.b_row, c.dz_batch, c.dz_row) == (40, 8, 40, 8, 40, 8)
+    assert lib.rp_selective_scan_saved_elems(C.byref(c), 0) == 2 * 1 * 8 * 4
+    assert lib.rp_selective_scan_saved_elems(C.byref(scan(length=9)), 0) == 2 * 2 * 8 * 4
+    assert lib.rp_selective_scan_ws_bytes(C.byref(c), 0, 0) == 0 and lib.rp_selective_scan_ws_bytes(C.byref(c), 0, 1) > 0
+    assert lib.rp_selective_scan_ws_bytes(C.byref(scan(batch=1, length=4096)), 0, 0) > 0         # few channels, long: split
+
+
+@pytest.mark.parametrize("wrong", [dict(batch=0), dict(length=0), dict(channels=0), dict(states=0), dict(states=65), dict(groups=0), dict(groups=3),
+                                   dict(softplus=2), dict(x_row=7), dict(dt_row=1), dict(b_row=7), dict(c_row=7), dict(z_row=7), dict(y_row=7),
+                                   dict(y_batch=39), dict(x_batch=-1)])
+def test_scan_refuses_bad_geometry(wrong):
+    lib, c = rpb.load(), scan(**wrong)
+    a = [at(2048 * i) for i in range(9)]
+    assert lib.rp_selective_scan_ex(a[0], None, None, a[1], a[2], a[3], a[4], a[5], None, None, a[6], None, None, None, C.byref(c), 0, 0, None) == -1
+    if not any(k.endswith(("row", "_batch")) for k in wrong):
+        assert lib.rp_selective_scan_saved_elems(C.byref(c), 0) == -1 and lib.rp_selective_scan_ws_bytes(C.byref(c), 0, 1) == -1
+
+
+def test_scan_refuses_bad_calls():
+    lib, c = rpb.load(), scan()
+    y, x, dt, A, B, Cm, z = (at(2048 * i) for i in range(7))
+
+    def call(y=y, x=x, dt=dt, A=A, B=B, Cm=Cm, z=z, c=c, saved=None, h_out=None, dtype=0, device=0):
+        return lib.rp_selective_scan_ex(y, h_out, saved, x, dt, A, B, Cm, None, None, z, None, None, None, C.byref(c) if c else None, dtype, device, None)
+
+    for missing in ("y", "x", "dt", "A", "B", "Cm", "c"):
+        assert call(**{missing: None}) == -1
+    assert call(device=-1) == -1 and call(dtype=4) == -1
+    for other in (x, dt, B, Cm, z):
+        assert call(y=other) == -1                                  # y over an operand
+    assert call(c=scan(batch=1, length=4096)) == -1                 # split, and no workspace
+    assert call(saved=A, h_out=A) == -1
+
+    def grad(dy=at(14000), saved=at(20000), ws=at(30000), z=z, dtype=0, device=0, c=c, dh_out=None, **out):
+        names = ("dx", "ddt", "dA", "dB", "dC", "dD", "ddt_bias", "dz", "dh_in")
+        return lib.rp_selective_scan_grad_ex(*(out.get(k) for k in names), 0, dy, dh_out, x, dt, A, B, Cm, None, None, z, None, saved, ws,
+                                             C.byref(c), dtype, device, None)
+
+    free = at(40000)
+    assert grad() == -1                                             # nothing wanted
+    assert grad(dx=free, dy=None) == -1 and grad(dx=free, saved=None) == -1 and grad(dx=free, ws=None) == -1
+    assert grad(dz=free, z=None) == -1
+    assert grad(dx=free, device=-1) == -1 and grad(dx=free, dtype=7) == -1
+    assert grad(dx=x) == -1 and grad(ddt=at(14000)) == -1 and grad(dB=B) == -1          # over an operand, over dy
+    assert grad(dx=free, ddt=free) == -1                            # over one another
+    assert grad(dx=free, c=scan(dx_row=5)) == -1 and grad(dB=free, c=scan(db_batch=3)) == -1
+    assert grad(dh_in=free, dh_out=free) == -1
+
+
+def norm(rows=4, channels=8, eps=1e-5, **over):
+    c = rpb.RpbBlockNorm()
+    rpb.load().rpb_block_norm_packed(C.byref(c), rows, channels, eps)
+    for k, v in over.items():
+        setattr(c, k, v)
+    return c
+
+
+@pytest.mark.parametrize("wrong", [dict(rows=0), dict(channels=0), dict(channels=16385), dict(eps=-1.0), dict(eps=float("nan")), dict(out_row=7),
+                                   dict(y_row=-8), dict(u_row=-1), dict(r_row=-1)])
+def test_norm_refuses_bad_geometry(wrong):
+    lib, c = rpb.load(), norm(**wrong)
+    a = [at(2048 * i) for i in range(6)]
+    assert lib.rp_block_norm_ex(a[0], a[1], a[2], None, None, None, a[3], a[4], C.byref(c), 0, 0, None) == -1
+    if not any(k.endswith("row") for k in wrong):
+        assert lib.rp_block_norm_ws_bytes(C.byref(c), 0) == -1
+
+
+def test_norm_refuses_bad_calls():
+    lib, c = rpb.load(), norm()
+    out, y, u, z, r, w = (at(2048 * i) for i in range(6))
+    call = lambda out=out, y=y, u=u, wb=w, dtype=0, device=0, g=c: lib.rp_block_norm_ex(out, y, u, z, None, None, r, wb, C.byref(g) if g else None,   # noqa: E731
+                                                                                      dtype, device, None)
+    assert call(u=None) == -1 and call(out=None, y=None) == -1 and call(wb=None) == -1 and call(g=None) == -1
+    assert call(device=-1) == -1 and call(dtype=-1) == -1
+    assert call(out=u) == -1 and call(y=r) == -1 and call(out=y) == -1 and call(y=z) == -1
+    names = ("du", "dz", "dr", "dw_after", "dscale", "dw_before")
+
+    def grad(dout=at(13000), dy=at(14000), z=z, wa=w, sc=w, wb=w, ws=at(20000), **outs):
+        return lib.rp_block_norm_grad_ex(*(outs.get(k) for k in names), 0, dout, dy, u, z, wa, sc, r, wb, ws, C.byref(c), 0, 0, None)
+
+    free = at(30000)
+    assert grad() == -1 and grad(du=free, dout=None, dy=None) == -1 and grad(du=free, wb=None) == -1
+    assert grad(dz=free, z=None) == -1 and grad(dw_after=free, wa=None) == -1 and grad(dscale=free, sc=None) == -1
+    assert grad(dw_before=free, dy=None) == -1 and grad(dw_before=free, ws=None) == -1
+    assert grad(du=u) == -1 and grad(dr=at(13000)) == -1 and grad(du=free, dr=free) == -1
