@@ -70,6 +70,30 @@ __device__ __forceinline__ float ex2_fast(float v) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
+/* two floats in one 64-bit register pair: one instruction for two multiplications or multiply-adds */
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float lo, float hi) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack2(f32x2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 __device__ __forceinline__ float exp_of(float v) { return __expf(v); }
 __device__ __forceinline__ double exp_of(double v) { return exp(v); }
 
@@ -77,8 +101,23 @@ __device__ __forceinline__ double exp_of(double v) { return exp(v); }
 __device__ __forceinline__ float logistic(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
 __device__ __forceinline__ double logistic(double v) { return 1.0 / (1.0 + exp(-v)); }
 
-/* log(1 + exp(v)) without overflow */
-__device__ __forceinline__ float softplus_of(float v) { return fmaxf(v, 0.0f) + log1pf(__expf(-fabsf(v))); }
+/* log(1 + exp(v)) = max(v, 0) + log(1 + e) with e = exp(-|v|) in (0, 1]; log(1 + e) / e as a polynomial of degree 9
+ * (Chebyshev interpolation on [0, 1]), within 2.2 half-steps of float32 as computed here: a third of log1pf's instructions,
+ * and no cancellation for small e */
+__device__ __forceinline__ float softplus_of(float v) {
+    const float e = __expf(-fabsf(v));
+    float p = -0.0031760570127516985f;
+    p = fmaf(p, e, 0.019542528316378593f);
+    p = fmaf(p, e, -0.05637361481785774f);
+    p = fmaf(p, e, 0.10543623566627502f);
+    p = fmaf(p, e, -0.1526966691017151f);
+    p = fmaf(p, e, 0.1966327428817749f);
+    p = fmaf(p, e, -0.24951615929603577f);
+    p = fmaf(p, e, 0.33329710364341736f);
+    p = fmaf(p, e, -0.49999892711639404f);
+    p = fmaf(p, e, 1.0f);
+    return fmaf(p, e, fmaxf(v, 0.0f));
+}
 __device__ __forceinline__ double softplus_of(double v) { return fmax(v, 0.0) + log1p(exp(-fabs(v))); }
 
 /* Runs a call on the tensors' device and gives the caller's current device back. */
