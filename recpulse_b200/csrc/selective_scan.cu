@@ -26,13 +26,19 @@ struct Args {
     int blocks;                     /* channel blocks of a group */
     int chunk, chunks;              /* rows per chunk (a multiple of the tile), and chunks per sequence */
     bool vec_x, vec_dt, vec_z, vec_y, vec_dx, vec_ddt, vec_dz, vec_n;
+    bool fast;                      /* all operands that the call has, B and C among them, in whole packs */
 };
 
 /* P lanes per channel (4 states each), CH channels per block, tiles of TT rows: each thread loads V channels of one row of a
  * tile, and afterwards walks the whole tile for its channel's four states. */
-template <int P> struct Shape {
-    static constexpr int CH = NT / P, TT = P <= 4 ? 8 * P : 32, V = CH * TT / NT, NP = S * P;
+template <typename T, int P> struct Shape {
+    static constexpr int CH = NT / P, TT = P <= 4 ? 8 * P : sizeof(T) == 8 && P == 16 ? 16 : 32, V = CH * TT / NT, NP = S * P;
     static constexpr int PAD = 32 / P;          /* rows of a [TT][CH] result are this much longer: P rows of a warp in 32 banks */
+    static constexpr int ROW = CH + 2;          /* pairs of a row: 16 bytes more, so that two rows written at once share no bank */
+    /* the walkers' parts of y: a row holds the P parts of V channels, then 4 words of padding (the loaders that read 16 bytes
+     * of eight such groups at once meet no bank twice), and so on */
+    static constexpr int YG = V * P + 4, YROW = CH / V * YG;
+    static constexpr int UNITS = (TT * P + NT - 1) / NT;    /* groups of four values of B (C) that a loader brings */
 };
 
 template <typename A> struct Pair { A delta, dx; };
@@ -84,6 +90,26 @@ template <int G, int M, int UNIT, typename A> __device__ __forceinline__ void su
     }
 }
 
+/* V values at p when `on`, else zeros, into shared memory; FAST: all of them exist and p is aligned, asynchronously */
+template <int BYTES> __device__ __forceinline__ void async_copy(void* to, const void* from, bool on) {
+    const unsigned dst = (unsigned)__cvta_generic_to_shared(to);
+    const int size = on ? BYTES : 0;            /* the rest of the BYTES is filled with zeros; nothing is read for 0 */
+    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(from), "r"(size) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(from), "n"(BYTES), "r"(size) : "memory");
+}
+__device__ __forceinline__ void async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <typename T, int V, bool FAST> __device__ __forceinline__ void bring(Pack<T, V>* to, const T* p, bool on, int valid, bool vec) {
+    if (FAST) {
+        constexpr int BYTES = sizeof(T) * V, STEP = BYTES < 16 ? BYTES : 16;
+#pragma unroll
+        for (int i = 0; i < BYTES; i += STEP) async_copy<STEP>(reinterpret_cast<char*>(to) + i, reinterpret_cast<const char*>(p) + i, on);
+    } else {
+        *to = on ? load_pack<T, V>(p, valid, vec) : zero_pack<T, V>();
+    }
+}
+
 /* Where a block works: sequence, group, first channel, channels left in the group, chunk of rows. */
 struct Place { int b, g, d0, valid, c; };
 template <int CH> __device__ __forceinline__ Place place_of(const Args& a) {
@@ -109,39 +135,48 @@ __device__ __forceinline__ A delta_of(T raw, A bias, int softplus) {
 /* Four states of one channel and their step: h = exp(delta A) h + dx b, and c . h.  In float the four are two register pairs
  * (mul / fma.f32x2: 13 instructions instead of 20 beside the four exponentials, which bound the scan). */
 template <typename A> struct Walk {
+    typedef Pack<A, S> Four;
     A h[S], rate[S];
     __device__ __forceinline__ void set_rate(const A (&r)[S]) { for (int i = 0; i < S; ++i) rate[i] = r[i]; }
     __device__ __forceinline__ void set(const A (&v)[S]) { for (int i = 0; i < S; ++i) h[i] = v[i]; }
     __device__ __forceinline__ void get(A (&v)[S]) const { for (int i = 0; i < S; ++i) v[i] = h[i]; }
-    __device__ __forceinline__ void step(const Pair<A>& p, const A* b) {
+    __device__ __forceinline__ void decays(Four& e, A delta) const {
 #pragma unroll
-        for (int i = 0; i < S; ++i) h[i] = decay(p.delta, rate[i]) * h[i] + p.dx * b[i];
+        for (int i = 0; i < S; ++i) e.v[i] = decay(delta, rate[i]);
     }
-    __device__ __forceinline__ A dot(const A* c) const {
-        A o = h[0] * c[0];
+    __device__ __forceinline__ void step(const Four& e, A dx, const Four& b) {
 #pragma unroll
-        for (int i = 1; i < S; ++i) o += h[i] * c[i];
+        for (int i = 0; i < S; ++i) h[i] = e.v[i] * h[i] + dx * b.v[i];
+    }
+    __device__ __forceinline__ A dot(const Four& c) const {
+        A o = h[0] * c.v[0];
+#pragma unroll
+        for (int i = 1; i < S; ++i) o += h[i] * c.v[i];
         return o;
     }
 };
 template <> struct Walk<float> {
+    typedef ulonglong2 Four;
     f32x2 h0, h1, r0, r1;
     __device__ __forceinline__ void set_rate(const float (&r)[S]) { r0 = pack2(r[0], r[1]); r1 = pack2(r[2], r[3]); }
     __device__ __forceinline__ void set(const float (&v)[S]) { h0 = pack2(v[0], v[1]); h1 = pack2(v[2], v[3]); }
     __device__ __forceinline__ void get(float (&v)[S]) const { unpack2(h0, v[0], v[1]); unpack2(h1, v[2], v[3]); }
-    __device__ __forceinline__ void step(const Pair<float>& p, const float* b) {
-        const ulonglong2 bv = *reinterpret_cast<const ulonglong2*>(b);
-        const f32x2 dl = pack2(p.delta, p.delta), dx = pack2(p.dx, p.dx);
+    __device__ __forceinline__ void decays(Four& e, float delta) const {
+        const f32x2 dl = pack2(delta, delta);
         float e0, e1, e2, e3;
         unpack2(mul2(dl, r0), e0, e1);
         unpack2(mul2(dl, r1), e2, e3);
-        h0 = fma2(pack2(ex2_fast(e0), ex2_fast(e1)), h0, mul2(dx, bv.x));
-        h1 = fma2(pack2(ex2_fast(e2), ex2_fast(e3)), h1, mul2(dx, bv.y));
+        e.x = pack2(ex2_fast(e0), ex2_fast(e1));
+        e.y = pack2(ex2_fast(e2), ex2_fast(e3));
     }
-    __device__ __forceinline__ float dot(const float* c) const {
-        const ulonglong2 cv = *reinterpret_cast<const ulonglong2*>(c);
+    __device__ __forceinline__ void step(const Four& e, float dx, const Four& b) {
+        const f32x2 d2 = pack2(dx, dx);
+        h0 = fma2(e.x, h0, mul2(d2, b.x));
+        h1 = fma2(e.y, h1, mul2(d2, b.y));
+    }
+    __device__ __forceinline__ float dot(const Four& c) const {
         float lo, hi;
-        unpack2(fma2(h0, cv.x, mul2(h1, cv.y)), lo, hi);
+        unpack2(fma2(h0, c.x, mul2(h1, c.y)), lo, hi);
         return lo + hi;
     }
 };
@@ -155,6 +190,18 @@ template <> struct Walk<float> {
  * a chunk is folded from these, and the second pass (AGG = false) runs every chunk from its own. */
 template <typename T> struct Resident { static constexpr int value = sizeof(T) <= 4 ? 2 : 1; };
 
+template <typename T> struct Ring { static constexpr int DEPTH = sizeof(T) == 2 ? 3 : sizeof(T) == 4 ? 2 : 1, SLOTS = DEPTH + 2; };
+
+template <typename T, int P, bool AGG> struct ForwardShared {
+    typedef typename AccOf<T>::type A;
+    typedef Shape<T, P> Sh;
+    static constexpr int SLOTS = Ring<T>::SLOTS, ONE = AGG ? 1 : Sh::TT;
+    Pack<T, Sh::V> raw_x[SLOTS][NT], raw_dt[SLOTS][NT], raw_z[AGG ? 1 : SLOTS][AGG ? 1 : NT];
+    Pack<T, S> raw_b[SLOTS][Sh::UNITS * NT], raw_c[AGG ? 1 : SLOTS][AGG ? 1 : Sh::UNITS * NT];
+    alignas(16) Pair<A> pairs[2][Sh::TT][Sh::ROW];
+    alignas(16) A Bs[2][Sh::TT][Sh::NP], Cs[2][ONE][Sh::NP], ys[2][ONE][Sh::YROW];
+};
+
 template <typename T, int P, bool AGG>
 __global__ void __launch_bounds__(2 * NT, Resident<T>::value)
 forward_kernel(T* __restrict__ y, typename AccOf<T>::type* h_out, typename AccOf<T>::type* __restrict__ saved, typename AccOf<T>::type* __restrict__ chunk_h,
@@ -163,14 +210,10 @@ forward_kernel(T* __restrict__ y, typename AccOf<T>::type* h_out, typename AccOf
                const typename AccOf<T>::type* __restrict__ dt_bias, const T* __restrict__ z, const typename AccOf<T>::type* h_in,
                const int* __restrict__ lengths, Args a) {
     typedef typename AccOf<T>::type A;
-    typedef Shape<P> Sh;
-    constexpr int CH = Sh::CH, TT = Sh::TT, V = Sh::V, NP = Sh::NP, YROW = CH + Sh::PAD;
+    typedef Shape<T, P> Sh;
+    constexpr int CH = Sh::CH, TT = Sh::TT, V = Sh::V, NP = Sh::NP, YROW = Sh::YROW;
     extern __shared__ __align__(16) unsigned char raw_shared[];
-    struct Shared {
-        Pair<A> pairs[2][TT][CH];
-        A Bs[2][TT][NP], Cs[2][AGG ? 1 : TT][NP], ys[2][AGG ? 1 : TT][YROW];
-    };
-    Shared& sh = *reinterpret_cast<Shared*>(raw_shared);
+    ForwardShared<T, P, AGG>& sh = *reinterpret_cast<ForwardShared<T, P, AGG>*>(raw_shared);
     rpb_pdl_trigger();
     rpb_pdl_wait();
     const Place pl = place_of<CH>(a);
@@ -179,8 +222,7 @@ forward_kernel(T* __restrict__ y, typename AccOf<T>::type* h_out, typename AccOf
     const int tiles = (last - first + TT - 1) / TT;
 
     if (threadIdx.x < NT) {
-        const int tid = threadIdx.x, lane = tid & 31;
-        const int p = tid % P, ch = tid / P, n0 = p * S;
+        const int tid = threadIdx.x, p = tid % P, ch = tid / P, n0 = p * S;
         const bool on = ch < pl.valid;
         const long long d = pl.d0 + ch;
         A rate[S], h[S], sum = 0;
@@ -217,24 +259,47 @@ forward_kernel(T* __restrict__ y, typename AccOf<T>::type* h_out, typename AccOf
             const int buf = tile & 1, left = last - first - tile * TT;
             const Pair<A>* pairs = &sh.pairs[buf][0][ch];
             const A *bs = &sh.Bs[buf][0][n0], *cs = &sh.Cs[buf][0][n0];
-            A* ys = &sh.ys[buf][AGG ? 0 : p][ch];
-#pragma unroll(P >= 8 ? 1 : 8 / P)
-            for (int t = 0; t < TT; t += P) {
-                A v[P];
+            A* ys = &sh.ys[buf][0][AGG ? 0 : ch / V * Sh::YG + (ch % V) * P + p];
+            /* Four rows at a time, as a pipeline: while h takes the steps of four rows, the decays of the next four are
+             * computed, and the deltas of the four behind those are on their way from shared memory. */
+            typedef typename Walk<A>::Four Four;
+            Four e[4], f[4];
+            Pair<A> p0[4], p1[4];
 #pragma unroll
-                for (int k = 0; k < P; ++k) {
-                    if (!AGG && (t + k) % SEG == 0) {
-                        if (keep && t + k < left) { w.get(h); store_states(keep, h, n0, a.states, a.vec_n); keep += (long long)a.channels * a.states; }
-                    }
-                    const Pair<A> pr = pairs[(t + k) * CH];
-                    w.step(pr, bs + (t + k) * NP);
-                    if (AGG) sum += pr.delta;
-                    else v[k] = w.dot(cs + (t + k) * NP);
+            for (int k = 0; k < 4; ++k) { p0[k] = pairs[k * Sh::ROW]; p1[k] = pairs[(4 + k) * Sh::ROW]; }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w.decays(e[k], p0[k].delta);
+            auto four = [&](int t, Four (&now)[4], Four (&next)[4]) {
+                Four bv[4], cv[4];
+                A dx[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    bv[k] = *reinterpret_cast<const Four*>(bs + (t + k) * NP);
+                    if (!AGG) cv[k] = *reinterpret_cast<const Four*>(cs + (t + k) * NP);
+                    dx[k] = p0[k].dx;
+                    if (AGG) sum += p0[k].delta;
+                    p0[k] = p1[k];
+                    if (t + 8 < TT) p1[k] = pairs[(t + 8 + k) * Sh::ROW];
                 }
-                if (!AGG) {
-                    sum_lanes<P, P, 1>(v, lane);
-                    ys[t * YROW] = v[0];
+                if (t + 4 < TT) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) w.decays(next[k], p0[k].delta);
                 }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    w.step(now[k], dx[k], bv[k]);
+                    if (!AGG) ys[(t + k) * YROW] = w.dot(cv[k]);
+                }
+            };
+#pragma unroll 1
+            for (int t = 0; t < TT; t += SEG) {
+                if (!AGG && keep && t < left) {
+                    w.get(h);
+                    store_states(keep, h, n0, a.states, a.vec_n);
+                    keep += (long long)a.channels * a.states;
+                }
+                four(t, e, f);
+                four(t + 4, f, e);
             }
             __syncthreads();
         }
@@ -251,88 +316,120 @@ forward_kernel(T* __restrict__ y, typename AccOf<T>::type* h_out, typename AccOf
     }
 
     if (AGG && pl.c == a.chunks - 1) return;
-    const int tid = threadIdx.x - NT;
-    const int lr = tid / (CH / V), lc = (tid % (CH / V)) * V, lvalid = pl.valid - lc;
-    const T* xp = x + pl.b * a.x_batch + (long long)(first + lr) * a.x_row + pl.d0 + lc;
-    const T* dp = dt + pl.b * a.dt_batch + (long long)(first + lr) * a.dt_row + pl.d0 + lc;
-    const T* zp = z ? z + pl.b * a.z_batch + (long long)(first + lr) * a.z_row + pl.d0 + lc : nullptr;
-    const T* bp = Bm + pl.b * a.b_batch + pl.g * a.states;
-    const T* cp = Cm + pl.b * a.c_batch + pl.g * a.states;
-    T* yp = y + pl.b * a.y_batch + (long long)(first + lr) * a.y_row + pl.d0 + lc;
-    A bias[V], skip[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        bias[i] = dt_bias && i < lvalid ? dt_bias[pl.d0 + lc + i] : A(0);
-        skip[i] = !AGG && Dv && i < lvalid ? Dv[pl.d0 + lc + i] : A(0);
-    }
-    constexpr int BC = (TT * NP + NT - 1) / NT;
-    Pack<T, V> x0, x1, x2, z0, z1, z2, d2;          /* 0: of the tile to finish, 1: of the tile walked, 2: of the next one */
-    T bn[BC], cn[BC];
-    auto fetch = [&](int tile) {
-        const int t = first + tile * TT + lr;
-        const bool row = t < last && t < end;
-        x2 = row ? load_pack<T, V>(xp + (long long)tile * TT * a.x_row, lvalid, a.vec_x) : zero_pack<T, V>();
-        d2 = row ? load_pack<T, V>(dp + (long long)tile * TT * a.dt_row, lvalid, a.vec_dt) : zero_pack<T, V>();
-        if (!AGG) z2 = row && zp ? load_pack<T, V>(zp + (long long)tile * TT * a.z_row, lvalid, a.vec_z) : zero_pack<T, V>();
-#pragma unroll
-        for (int k = 0; k < BC; ++k) {
-            const int e = tid + k * NT, r = e / NP, n = e - r * NP, bt = first + tile * TT + r;
-            const bool in = e < TT * NP && bt < last && bt < end && n < a.states;
-            bn[k] = in ? bp[bt * a.b_row + n] : down<T>(A(0));
-            if (!AGG) cn[k] = in ? cp[bt * a.c_row + n] : down<T>(A(0));
-        }
-    };
-    auto stage = [&](int tile) {
-        const int t = first + tile * TT + lr, buf = tile & 1;
-        const bool row = t < last && t < end;
-        Pair<A>* to = &sh.pairs[buf][lr][lc];
+    /* The raw rows wait in a ring of shared memory, where each thread meets only what it brought itself: DEPTH tiles are on
+     * their way while one is staged.  FAST: whole packs everywhere, a full block of channels, states in whole groups of four:
+     * asynchronous copies; else plain loads. */
+    auto load = [&](auto fast) {
+        constexpr bool FAST = decltype(fast)::value;
+        constexpr int UNITS = Sh::UNITS, DEPTH = Ring<T>::DEPTH, SLOTS = Ring<T>::SLOTS;
+        const int tid = threadIdx.x - NT;
+        const int lr = tid / (CH / V), lc = (tid % (CH / V)) * V, lvalid = FAST ? V : pl.valid - lc;
+        const T* xp = x + pl.b * a.x_batch + (long long)(first + lr) * a.x_row + pl.d0 + lc;
+        const T* dp = dt + pl.b * a.dt_batch + (long long)(first + lr) * a.dt_row + pl.d0 + lc;
+        const T* zp = z ? z + pl.b * a.z_batch + (long long)(first + lr) * a.z_row + pl.d0 + lc : nullptr;
+        T* yp = y + pl.b * a.y_batch + (long long)(first + lr) * a.y_row + pl.d0 + lc;
+        const T* bp = Bm + pl.b * a.b_batch + pl.g * a.states + first * a.b_row;
+        const T* cp = Cm + pl.b * a.c_batch + pl.g * a.states + first * a.c_row;
+        A bias[V], skip[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const A dl = row && i < lvalid ? delta_of<T, A>(d2.v[i], bias[i], a.softplus) : A(0);
-            to[i] = Pair<A>{dl, dl * up(x2.v[i])};
+            bias[i] = dt_bias && i < lvalid ? dt_bias[pl.d0 + lc + i] : A(0);
+            skip[i] = !AGG && Dv && i < lvalid ? Dv[pl.d0 + lc + i] : A(0);
         }
+        const int rows = (end < last ? end : last) - first;
+        int t2 = 0, slot2 = 0;                      /* of the next fetch: row from `first`, slot of the ring */
+        auto fetch = [&]() {
+            const bool row = t2 + lr < rows;
+            bring<T, V, FAST>(&sh.raw_x[slot2][tid], xp, row, lvalid, a.vec_x);
+            bring<T, V, FAST>(&sh.raw_dt[slot2][tid], dp, row, lvalid, a.vec_dt);
+            if (!AGG && z) bring<T, V, FAST>(&sh.raw_z[slot2][AGG ? 0 : tid], zp, row, lvalid, a.vec_z);
 #pragma unroll
-        for (int k = 0; k < BC; ++k) {
-            const int e = tid + k * NT, r = e / NP, n = e - r * NP;
-            if (e < TT * NP) {
-                sh.Bs[buf][r][n] = up(bn[k]);
-                if (!AGG) sh.Cs[buf][r][n] = up(cn[k]);
+            for (int k = 0; k < UNITS; ++k) {
+                const int e = tid + k * NT, r = e / P, n = (e % P) * S;
+                const bool in = e < TT * P && t2 + r < rows;
+                bring<T, S, FAST>(&sh.raw_b[slot2][e], bp + r * a.b_row + n, in, a.states - n, false);
+                if (!AGG) bring<T, S, FAST>(&sh.raw_c[slot2][AGG ? 0 : e], cp + r * a.c_row + n, in, a.states - n, false);
             }
-        }
-        x0 = x1; x1 = x2;
-        if (!AGG) { z0 = z1; z1 = z2; }
-    };
-    auto finish = [&](int tile, const Pack<T, V>& xr, const Pack<T, V>& zr) {
-        const int t = first + tile * TT + lr;
-        if (t >= last || lvalid <= 0) return;
-        const A* from = &sh.ys[tile & 1][lr][lc];
-        Pack<T, V> o;
+            t2 += TT;
+            slot2 = slot2 + 1 == SLOTS ? 0 : slot2 + 1;
+            xp += TT * a.x_row; dp += TT * a.dt_row; bp += TT * a.b_row; cp += TT * a.c_row;
+            if (zp) zp += TT * a.z_row;
+        };
+        auto stage = [&](int tile, int slot) {
+            const bool row = tile * TT + lr < rows;
+            const Pack<T, V> xr = sh.raw_x[slot][tid], dr = sh.raw_dt[slot][tid];
+            Pack<A, 2 * V> o;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            A r = from[i] + skip[i] * up(xr.v[i]);
-            if (zp) { const A g = up(zr.v[i]); r *= g * logistic(g); }
-            o.v[i] = down<T>(t < end ? r : A(0));
+            for (int i = 0; i < V; ++i) {
+                const A dl = row && i < lvalid ? delta_of<T, A>(dr.v[i], bias[i], a.softplus) : A(0);
+                o.v[2 * i] = dl;
+                o.v[2 * i + 1] = dl * up(xr.v[i]);
+            }
+            *reinterpret_cast<Pack<A, 2 * V>*>(&sh.pairs[tile & 1][lr][lc]) = o;
+#pragma unroll
+            for (int k = 0; k < UNITS; ++k) {
+                const int e = tid + k * NT, r = e / P, n = (e % P) * S;
+                if (e < TT * P) {
+                    Pack<A, S> v;
+                    const Pack<T, S> br = sh.raw_b[slot][e];
+#pragma unroll
+                    for (int i = 0; i < S; ++i) v.v[i] = up(br.v[i]);
+                    *reinterpret_cast<Pack<A, S>*>(&sh.Bs[tile & 1][r][n]) = v;
+                    if (!AGG) {
+                        const Pack<T, S> cr = sh.raw_c[slot][AGG ? 0 : e];
+#pragma unroll
+                        for (int i = 0; i < S; ++i) v.v[i] = up(cr.v[i]);
+                        *reinterpret_cast<Pack<A, S>*>(&sh.Cs[tile & 1][AGG ? 0 : r][n]) = v;
+                    }
+                }
+            }
+        };
+        auto finish = [&](int tile, int slot) {
+            const int t = tile * TT + lr;
+            if (first + t >= last || lvalid <= 0) return;
+            const A* from = &sh.ys[tile & 1][AGG ? 0 : lr][lc / V * Sh::YG];
+            A part[V * P];
+#pragma unroll
+            for (int j = 0; j < V * P; j += 4) *reinterpret_cast<Pack<A, 4>*>(&part[j]) = *reinterpret_cast<const Pack<A, 4>*>(from + j);
+            const Pack<T, V> xr = sh.raw_x[slot][tid], zr = z ? sh.raw_z[slot][AGG ? 0 : tid] : zero_pack<T, V>();
+            Pack<T, V> o;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+#pragma unroll
+                for (int m = P / 2; m >= 1; m /= 2)
+#pragma unroll
+                    for (int j = 0; j < m; ++j) part[i * P + j] += part[i * P + j + m];
+                A r = part[i * P] + skip[i] * up(xr.v[i]);
+                if (z) { const A g = up(zr.v[i]); r *= g * logistic(g); }
+                o.v[i] = down<T>(t < rows ? r : A(0));
+            }
+            T* to = yp + (long long)tile * TT * a.y_row;
+            if (FAST) *reinterpret_cast<Pack<T, V>*>(to) = o;
+            else store_pack<T, V>(to, o, lvalid, a.vec_y);
+        };
+        auto next = [](int slot) { return slot + 1 == SLOTS ? 0 : slot + 1; };
+#pragma unroll
+        for (int k = 0; k <= DEPTH; ++k) {
+            if (k < tiles) fetch();
+            async_commit();
         }
-        store_pack<T, V>(yp + (long long)tile * TT * a.y_row, o, lvalid, a.vec_y);
-    };
-    x0 = x1 = z0 = z1 = z2 = zero_pack<T, V>();
-    fetch(0);
-    stage(0);
-    if (tiles > 1) fetch(1);
-    __syncthreads();
-    for (int tile = 0; tile < tiles; ++tile) {
-        /* here x1, z1 are tile's, x2 .. cn (on their way) those of tile + 1 */
-        if (!AGG && tile > 0) finish(tile - 1, x0, z0);
-        if (tile + 1 < tiles) {
-            stage(tile + 1);
-            if (tile + 2 < tiles) fetch(tile + 2);
-        } else {
-            x0 = x1;
-            if (!AGG) z0 = z1;
-        }
+        async_wait<DEPTH>();
+        stage(0, 0);
         __syncthreads();
-    }
-    if (!AGG) finish(tiles - 1, x0, z0);
+        int done = SLOTS - 1, ahead = 1 % SLOTS;    /* slots of tile - 1 and tile + 1 */
+        for (int tile = 0; tile < tiles; ++tile) {
+            async_wait<DEPTH - 1>();                /* tile + 1 is there */
+            if (tile + 1 < tiles) stage(tile + 1, ahead);
+            if (!AGG && tile > 0) finish(tile - 1, done);
+            if (tile + 1 + DEPTH < tiles) fetch();  /* into the slot of tile - 1 */
+            async_commit();
+            done = next(done); ahead = next(ahead);
+            __syncthreads();
+        }
+        if (!AGG) finish(tiles - 1, done);
+    };
+    if (a.fast && pl.valid >= CH) load(std::true_type());
+    else load(std::false_type());
 }
 
 /* One token per sequence: what moves is the state, once in and once out.  P lanes per channel as above; each thread takes
@@ -407,7 +504,7 @@ __global__ void __launch_bounds__(256) token_kernel(T* __restrict__ y, typename 
  * end, and the sum of the deltas. */
 template <typename T, int P> struct BackwardShared {
     typedef typename AccOf<T>::type A;
-    typedef Shape<P> Sh;
+    typedef Shape<T, P> Sh;
     Pair<A> pairs[Sh::TT][Sh::CH];
     A dys[Sh::TT][Sh::CH];
     A Bs[Sh::TT][Sh::NP], Cs[Sh::TT][Sh::NP];
@@ -431,7 +528,7 @@ __global__ void __launch_bounds__(NT) backward_kernel(Grads<T> out, typename Acc
                                                       const typename AccOf<T>::type* __restrict__ dt_bias, const T* __restrict__ z,
                                                       const int* __restrict__ lengths, const typename AccOf<T>::type* __restrict__ saved, Args a) {
     typedef typename AccOf<T>::type A;
-    typedef Shape<P> Sh;
+    typedef Shape<T, P> Sh;
     constexpr int CH = Sh::CH, TT = Sh::TT, V = Sh::V, NP = Sh::NP;
     extern __shared__ __align__(16) unsigned char raw_shared[];
     BackwardShared<T, P>& sh = *reinterpret_cast<BackwardShared<T, P>*>(raw_shared);
@@ -744,7 +841,7 @@ Args make_args(const RpbScan* c) {
     a.blocks = (a.per_group + ch - 1) / ch;
     a.chunk = pick_chunk(c);
     a.chunks = (c->len + a.chunk - 1) / a.chunk;
-    a.vec_x = a.vec_dt = a.vec_z = a.vec_y = a.vec_dx = a.vec_ddt = a.vec_dz = a.vec_n = false;
+    a.vec_x = a.vec_dt = a.vec_z = a.vec_y = a.vec_dx = a.vec_ddt = a.vec_dz = a.vec_n = a.fast = false;
     return a;
 }
 
@@ -759,6 +856,11 @@ Rowset rows_of(const RpbScan* c, const void* x, const void* dt, const void* B, c
 template <typename T, int V> bool packs_ok(const RpbScan* c, const Rows& r) {
     const size_t bytes = sizeof(T) * V < 16 ? sizeof(T) * V : 16;
     return r.p && aligned_rows(r, c->batch, c->len, sizeof(T), bytes) && (c->groups == 1 || (c->channels / c->groups) % V == 0);
+}
+/* B and C in groups of four states */
+template <typename T> bool quads_ok(const RpbScan* c, const Rows& r) {
+    const size_t bytes = sizeof(T) * S < 16 ? sizeof(T) * S : 16;
+    return c->states % S == 0 && aligned_rows(r, c->batch, c->len, sizeof(T), bytes);
 }
 template <typename A> bool states_ok(const RpbScan* c, const void* p) {
     return !p || (c->states % S == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0);
@@ -786,16 +888,10 @@ struct Operands {
     const int* lengths;
 };
 
-/* the forward kernel's shared memory (its struct Shared) */
-template <typename A, int P, bool AGG> constexpr size_t forward_shared() {
-    typedef Shape<P> Sh;
-    return 2 * sizeof(A) * (2 * Sh::TT * Sh::CH + Sh::TT * Sh::NP + (AGG ? 1 : Sh::TT) * (Sh::NP + Sh::CH + Sh::PAD));
-}
-
 template <typename T, int P>
 int forward_p(void* y, void* h_out, void* saved, const Operands& o, const void* h_in, void* ws, const RpbScan* c, cudaStream_t s) {
     typedef typename AccOf<T>::type A;
-    typedef Shape<P> Sh;
+    typedef Shape<T, P> Sh;
     Args a = make_args(c);
     const Rowset r = rows_of(c, o.x, o.dt, o.B, o.C, o.z, y);
     const A *Am = reinterpret_cast<const A*>(o.A), *Dv = reinterpret_cast<const A*>(o.D), *bias = reinterpret_cast<const A*>(o.dt_bias);
@@ -818,18 +914,19 @@ int forward_p(void* y, void* h_out, void* saved, const Operands& o, const void* 
     a.vec_x = packs_ok<T, Sh::V>(c, r.x); a.vec_dt = packs_ok<T, Sh::V>(c, r.dt);
     a.vec_z = packs_ok<T, Sh::V>(c, r.z); a.vec_y = packs_ok<T, Sh::V>(c, r.y);
     a.vec_n = a.vec_n && states_ok<A>(c, saved) && states_ok<A>(c, ws);
+    a.fast = a.vec_x && a.vec_dt && (!z || a.vec_z) && a.vec_y && quads_ok<T>(c, r.B) && quads_ok<T>(c, r.C);
     const long long blocks = (long long)c->batch * a.chunks * c->groups * a.blocks;
     if (blocks > 0x7fffffffLL) return refuse("rp_selective_scan_ex", "too many sequences for one launch");
     A* chunk_h = reinterpret_cast<A*>(ws);
     A* chunk_s = chunk_h ? chunk_h + (long long)c->batch * a.chunks * c->channels * c->states : nullptr;
+    SEQ_CUDA(cudaFuncSetAttribute(forward_kernel<T, P, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ForwardShared<T, P, true>)));
+    SEQ_CUDA(cudaFuncSetAttribute(forward_kernel<T, P, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ForwardShared<T, P, false>)));
     if (a.chunks > 1) {
-        SEQ_CUDA(rpb_launch(forward_kernel<T, P, true>, dim3((unsigned)blocks), dim3(2 * NT), forward_shared<A, P, true>(), s, 1, reinterpret_cast<T*>(y), ho, reinterpret_cast<A*>(saved),
+        SEQ_CUDA(rpb_launch(forward_kernel<T, P, true>, dim3((unsigned)blocks), dim3(2 * NT), sizeof(ForwardShared<T, P, true>), s, 1, reinterpret_cast<T*>(y), ho, reinterpret_cast<A*>(saved),
                             chunk_h, chunk_s, x, dt, Am, B, C, Dv, bias, z, hi, o.lengths, a));
         rpb_count_launches(1);
     }
-    if (forward_shared<A, P, false>() > 48 * 1024)
-        SEQ_CUDA(cudaFuncSetAttribute(forward_kernel<T, P, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)forward_shared<A, P, false>()));
-    SEQ_CUDA(rpb_launch(forward_kernel<T, P, false>, dim3((unsigned)blocks), dim3(2 * NT), forward_shared<A, P, false>(), s, 1, reinterpret_cast<T*>(y), ho, reinterpret_cast<A*>(saved),
+    SEQ_CUDA(rpb_launch(forward_kernel<T, P, false>, dim3((unsigned)blocks), dim3(2 * NT), sizeof(ForwardShared<T, P, false>), s, 1, reinterpret_cast<T*>(y), ho, reinterpret_cast<A*>(saved),
                         chunk_h, chunk_s, x, dt, Am, B, C, Dv, bias, z, hi, o.lengths, a));
     rpb_count_launches(1);
     return 0;
@@ -844,7 +941,7 @@ template <typename T, int P>
 int backward_p(const Wanted& w, const void* dy, const void* dh_out, const Operands& o, const void* saved, void* ws, const RpbScan* c,
                cudaStream_t s) {
     typedef typename AccOf<T>::type A;
-    typedef Shape<P> Sh;
+    typedef Shape<T, P> Sh;
     Args a = make_args(c);
     const Rowset r = rows_of(c, o.x, o.dt, o.B, o.C, o.z, dy);
     const A *Am = reinterpret_cast<const A*>(o.A), *Dv = reinterpret_cast<const A*>(o.D), *bias = reinterpret_cast<const A*>(o.dt_bias);
