@@ -29,16 +29,11 @@ struct Args {
     bool fast;                      /* all operands that the call has, B and C among them, in whole packs */
 };
 
-/* P lanes per channel (4 states each), CH channels per block, tiles of TT rows: each thread loads V channels of one row of a
- * tile, and afterwards walks the whole tile for its channel's four states. */
-template <typename T, int P> struct Shape {
-    static constexpr int CH = NT / P, TT = P <= 4 ? 8 * P : sizeof(T) == 8 && P == 16 ? 16 : 32, V = CH * TT / NT, NP = S * P;
+/* P lanes per channel (4 states each), CH channels per block of NT walkers, tiles of TT rows; NL threads load a tile, V
+ * channels of one row each. */
+template <typename T, int P, int NL> struct Tile {
+    static constexpr int CH = NT / P, TT = sizeof(T) >= 4 && P >= 4 ? 16 : P <= 4 ? 8 * P : 32, V = CH * TT / NL, NP = S * P;
     static constexpr int PAD = 32 / P;          /* rows of a [TT][CH] result are this much longer: P rows of a warp in 32 banks */
-    static constexpr int ROW = CH + 2;          /* pairs of a row: 16 bytes more, so that two rows written at once share no bank */
-    /* the walkers' parts of y: a row holds the P parts of V channels, then 4 words of padding (the loaders that read 16 bytes
-     * of eight such groups at once meet no bank twice), and so on */
-    static constexpr int YG = V * P + 4, YROW = CH / V * YG;
-    static constexpr int UNITS = (TT * P + NT - 1) / NT;    /* groups of four values of B (C) that a loader brings */
 };
 
 template <typename A> struct Pair { A delta, dx; };
@@ -182,6 +177,18 @@ template <> struct Walk<float> {
 };
 
 /* ------------------------------------------------------------------------------------------------ forward
+ * The shared layouts: a row of pairs is 16 bytes longer than its channels, so that the rows a warp of loaders writes at once
+ * lie in other banks; a row of the walkers' parts of y holds the P parts of V channels, 4 words of padding, and so on, so that
+ * the loaders' 16-byte reads of eight such groups meet no bank twice. */
+template <typename T, int P> struct Forward : Tile<T, P, NT> {
+    typedef Tile<T, P, NT> Base;
+    static constexpr int NL = NT, K = Base::CH / Base::V;
+    static constexpr int ROW = Base::CH + 2;
+    static constexpr int YG = Base::V * P < 4 ? 4 : Base::V * P + 4, YROW = K * YG;
+    static constexpr int UNITS = (Base::TT * P + NL - 1) / NL;      /* groups of four values of B (C) that a loader brings */
+};
+
+/*
  * Half of a block's threads walk: P lanes per channel, four states each, one tile of rows after the other.  The other half
  * load: while tile i is walked they turn tile i + 1 into deltas and delta x in shared memory (and B and C into floats) and
  * finish tile i - 1 (skip, gate, rounding, whole packs to memory); one barrier per tile.
@@ -190,30 +197,31 @@ template <> struct Walk<float> {
  * a chunk is folded from these, and the second pass (AGG = false) runs every chunk from its own. */
 template <typename T> struct Resident { static constexpr int value = sizeof(T) <= 4 ? 2 : 1; };
 
-template <typename T> struct Ring { static constexpr int DEPTH = sizeof(T) == 2 ? 3 : sizeof(T) == 4 ? 2 : 1, SLOTS = DEPTH + 2; };
+template <typename T, int P> struct Ring { static constexpr int DEPTH = P == 16 || sizeof(T) == 8 ? 1 : sizeof(T) == 4 ? 2 : 3, SLOTS = DEPTH + 2; };
 
 template <typename T, int P, bool AGG> struct ForwardShared {
     typedef typename AccOf<T>::type A;
-    typedef Shape<T, P> Sh;
-    static constexpr int SLOTS = Ring<T>::SLOTS, ONE = AGG ? 1 : Sh::TT;
-    Pack<T, Sh::V> raw_x[SLOTS][NT], raw_dt[SLOTS][NT], raw_z[AGG ? 1 : SLOTS][AGG ? 1 : NT];
-    Pack<T, S> raw_b[SLOTS][Sh::UNITS * NT], raw_c[AGG ? 1 : SLOTS][AGG ? 1 : Sh::UNITS * NT];
+    typedef Forward<T, P> Sh;
+    static constexpr int SLOTS = Ring<T, P>::SLOTS, ONE = AGG ? 1 : Sh::TT, NL = Sh::NL;
+    Pack<T, Sh::V> raw_x[SLOTS][NL], raw_dt[SLOTS][NL], raw_z[AGG ? 1 : SLOTS][AGG ? 1 : NL];
+    Pack<T, S> raw_b[SLOTS][Sh::TT * P], raw_c[AGG ? 1 : SLOTS][AGG ? 1 : Sh::TT * P];
     alignas(16) Pair<A> pairs[2][Sh::TT][Sh::ROW];
     alignas(16) A Bs[2][Sh::TT][Sh::NP], Cs[2][ONE][Sh::NP], ys[2][ONE][Sh::YROW];
 };
 
 template <typename T, int P, bool AGG>
-__global__ void __launch_bounds__(2 * NT, Resident<T>::value)
+__global__ void __launch_bounds__(NT + Forward<T, P>::NL, Resident<T>::value)
 forward_kernel(T* __restrict__ y, typename AccOf<T>::type* h_out, typename AccOf<T>::type* __restrict__ saved, typename AccOf<T>::type* __restrict__ chunk_h,
                typename AccOf<T>::type* __restrict__ chunk_s, const T* __restrict__ x, const T* __restrict__ dt, const typename AccOf<T>::type* __restrict__ Am,
                const T* __restrict__ Bm, const T* __restrict__ Cm, const typename AccOf<T>::type* __restrict__ Dv,
                const typename AccOf<T>::type* __restrict__ dt_bias, const T* __restrict__ z, const typename AccOf<T>::type* h_in,
                const int* __restrict__ lengths, Args a) {
     typedef typename AccOf<T>::type A;
-    typedef Shape<T, P> Sh;
-    constexpr int CH = Sh::CH, TT = Sh::TT, V = Sh::V, NP = Sh::NP, YROW = Sh::YROW;
+    typedef Forward<T, P> Sh;
+    constexpr int CH = Sh::CH, TT = Sh::TT, V = Sh::V, NP = Sh::NP, YROW = Sh::YROW, NL = Sh::NL, K = Sh::K;
     extern __shared__ __align__(16) unsigned char raw_shared[];
     ForwardShared<T, P, AGG>& sh = *reinterpret_cast<ForwardShared<T, P, AGG>*>(raw_shared);
+    static_assert(sizeof(sh) <= 227 * 1024 / Resident<T>::value - 1024, "");
     rpb_pdl_trigger();
     rpb_pdl_wait();
     const Place pl = place_of<CH>(a);
@@ -259,47 +267,41 @@ forward_kernel(T* __restrict__ y, typename AccOf<T>::type* h_out, typename AccOf
             const int buf = tile & 1, left = last - first - tile * TT;
             const Pair<A>* pairs = &sh.pairs[buf][0][ch];
             const A *bs = &sh.Bs[buf][0][n0], *cs = &sh.Cs[buf][0][n0];
-            A* ys = &sh.ys[buf][0][AGG ? 0 : ch / V * Sh::YG + (ch % V) * P + p];
-            /* Four rows at a time, as a pipeline: while h takes the steps of four rows, the decays of the next four are
-             * computed, and the deltas of the four behind those are on their way from shared memory. */
+            A* ys = &sh.ys[buf][0][AGG ? 0 : ch / V * Sh::YG + ch % V * P + p];
+            /* The decays of a row are computed one row ahead of h's step; results wait in registers, since a store to shared
+             * memory would hold up the loads behind it. */
+            constexpr int BLK = TT < 16 ? TT : 16;
             typedef typename Walk<A>::Four Four;
-            Four e[4], f[4];
-            Pair<A> p0[4], p1[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) { p0[k] = pairs[k * Sh::ROW]; p1[k] = pairs[(4 + k) * Sh::ROW]; }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) w.decays(e[k], p0[k].delta);
-            auto four = [&](int t, Four (&now)[4], Four (&next)[4]) {
-                Four bv[4], cv[4];
-                A dx[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    bv[k] = *reinterpret_cast<const Four*>(bs + (t + k) * NP);
-                    if (!AGG) cv[k] = *reinterpret_cast<const Four*>(cs + (t + k) * NP);
-                    dx[k] = p0[k].dx;
-                    if (AGG) sum += p0[k].delta;
-                    p0[k] = p1[k];
-                    if (t + 8 < TT) p1[k] = pairs[(t + 8 + k) * Sh::ROW];
-                }
-                if (t + 4 < TT) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) w.decays(next[k], p0[k].delta);
-                }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    w.step(now[k], dx[k], bv[k]);
-                    if (!AGG) ys[(t + k) * YROW] = w.dot(cv[k]);
-                }
-            };
 #pragma unroll 1
-            for (int t = 0; t < TT; t += SEG) {
-                if (!AGG && keep && t < left) {
-                    w.get(h);
-                    store_states(keep, h, n0, a.states, a.vec_n);
-                    keep += (long long)a.channels * a.states;
+            for (int t = 0; t < TT; t += BLK) {
+                A v[BLK];
+                Four e[2], bv[2], cv[2];
+                Pair<A> pr[3] = {};
+                auto bring = [&](int k) {
+                    bv[k & 1] = *reinterpret_cast<const Four*>(bs + (t + k) * NP);
+                    if (!AGG) cv[k & 1] = *reinterpret_cast<const Four*>(cs + (t + k) * NP);
+                    w.decays(e[k & 1], pr[k % 3].delta);
+                };
+                pr[0] = pairs[t * Sh::ROW];
+                pr[1] = pairs[(t + 1) * Sh::ROW];
+                bring(0);
+#pragma unroll
+                for (int k = 0; k < BLK; ++k) {
+                    if (!AGG && k % SEG == 0 && keep && t + k < left) {
+                        w.get(h);
+                        store_states(keep, h, n0, a.states, a.vec_n);
+                        keep += (long long)a.channels * a.states;
+                    }
+                    if (k + 2 < BLK) pr[(k + 2) % 3] = pairs[(t + k + 2) * Sh::ROW];
+                    if (k + 1 < BLK) bring(k + 1);
+                    w.step(e[k & 1], pr[k % 3].dx, bv[k & 1]);
+                    if (AGG) sum += pr[k % 3].delta;
+                    else v[k] = w.dot(cv[k & 1]);
                 }
-                four(t, e, f);
-                four(t + 4, f, e);
+                if (!AGG) {
+#pragma unroll
+                    for (int k = 0; k < BLK; ++k) ys[(t + k) * YROW] = v[k];
+                }
             }
             __syncthreads();
         }
@@ -321,9 +323,9 @@ forward_kernel(T* __restrict__ y, typename AccOf<T>::type* h_out, typename AccOf
      * asynchronous copies; else plain loads. */
     auto load = [&](auto fast) {
         constexpr bool FAST = decltype(fast)::value;
-        constexpr int UNITS = Sh::UNITS, DEPTH = Ring<T>::DEPTH, SLOTS = Ring<T>::SLOTS;
-        const int tid = threadIdx.x - NT;
-        const int lr = tid / (CH / V), lc = (tid % (CH / V)) * V, lvalid = FAST ? V : pl.valid - lc;
+        constexpr int UNITS = Sh::UNITS, DEPTH = Ring<T, P>::DEPTH, SLOTS = Ring<T, P>::SLOTS;
+        const int tid = (int)threadIdx.x - NT;
+        const int lr = tid / K, lk = tid % K, lc = lk * V, lvalid = FAST ? V : pl.valid - lc;
         const T* xp = x + pl.b * a.x_batch + (long long)(first + lr) * a.x_row + pl.d0 + lc;
         const T* dp = dt + pl.b * a.dt_batch + (long long)(first + lr) * a.dt_row + pl.d0 + lc;
         const T* zp = z ? z + pl.b * a.z_batch + (long long)(first + lr) * a.z_row + pl.d0 + lc : nullptr;
@@ -345,8 +347,9 @@ forward_kernel(T* __restrict__ y, typename AccOf<T>::type* h_out, typename AccOf
             if (!AGG && z) bring<T, V, FAST>(&sh.raw_z[slot2][AGG ? 0 : tid], zp, row, lvalid, a.vec_z);
 #pragma unroll
             for (int k = 0; k < UNITS; ++k) {
-                const int e = tid + k * NT, r = e / P, n = (e % P) * S;
-                const bool in = e < TT * P && t2 + r < rows;
+                const int e = tid + k * NL, r = e / P, n = (e % P) * S;
+                if (e >= TT * P) break;
+                const bool in = t2 + r < rows && n < a.states;
                 bring<T, S, FAST>(&sh.raw_b[slot2][e], bp + r * a.b_row + n, in, a.states - n, false);
                 if (!AGG) bring<T, S, FAST>(&sh.raw_c[slot2][AGG ? 0 : e], cp + r * a.c_row + n, in, a.states - n, false);
             }
@@ -358,17 +361,21 @@ forward_kernel(T* __restrict__ y, typename AccOf<T>::type* h_out, typename AccOf
         auto stage = [&](int tile, int slot) {
             const bool row = tile * TT + lr < rows;
             const Pack<T, V> xr = sh.raw_x[slot][tid], dr = sh.raw_dt[slot][tid];
+            A dl[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) dl[i] = up(dr.v[i]) + bias[i];
+            if (a.softplus) softplus_all(dl);
             Pack<A, 2 * V> o;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const A dl = row && i < lvalid ? delta_of<T, A>(dr.v[i], bias[i], a.softplus) : A(0);
-                o.v[2 * i] = dl;
-                o.v[2 * i + 1] = dl * up(xr.v[i]);
+                if (!row || i >= lvalid) dl[i] = 0;
+                o.v[2 * i] = dl[i];
+                o.v[2 * i + 1] = dl[i] * up(xr.v[i]);
             }
             *reinterpret_cast<Pack<A, 2 * V>*>(&sh.pairs[tile & 1][lr][lc]) = o;
 #pragma unroll
             for (int k = 0; k < UNITS; ++k) {
-                const int e = tid + k * NT, r = e / P, n = (e % P) * S;
+                const int e = tid + k * NL, r = e / P, n = (e % P) * S;
                 if (e < TT * P) {
                     Pack<A, S> v;
                     const Pack<T, S> br = sh.raw_b[slot][e];
@@ -387,10 +394,11 @@ forward_kernel(T* __restrict__ y, typename AccOf<T>::type* h_out, typename AccOf
         auto finish = [&](int tile, int slot) {
             const int t = tile * TT + lr;
             if (first + t >= last || lvalid <= 0) return;
-            const A* from = &sh.ys[tile & 1][AGG ? 0 : lr][lc / V * Sh::YG];
-            A part[V * P];
+            const A* from = &sh.ys[tile & 1][AGG ? 0 : lr][lk * Sh::YG];
+            constexpr int PART = V * P < 4 ? V * P : 4;
+            alignas(16) A part[V * P];
 #pragma unroll
-            for (int j = 0; j < V * P; j += 4) *reinterpret_cast<Pack<A, 4>*>(&part[j]) = *reinterpret_cast<const Pack<A, 4>*>(from + j);
+            for (int j = 0; j < V * P; j += PART) *reinterpret_cast<Pack<A, PART>*>(&part[j]) = *reinterpret_cast<const Pack<A, PART>*>(from + j);
             const Pack<T, V> xr = sh.raw_x[slot][tid], zr = z ? sh.raw_z[slot][AGG ? 0 : tid] : zero_pack<T, V>();
             Pack<T, V> o;
 #pragma unroll
@@ -504,7 +512,7 @@ __global__ void __launch_bounds__(256) token_kernel(T* __restrict__ y, typename 
  * end, and the sum of the deltas. */
 template <typename T, int P> struct BackwardShared {
     typedef typename AccOf<T>::type A;
-    typedef Shape<T, P> Sh;
+    typedef Tile<T, P, NT> Sh;
     Pair<A> pairs[Sh::TT][Sh::CH];
     A dys[Sh::TT][Sh::CH];
     A Bs[Sh::TT][Sh::NP], Cs[Sh::TT][Sh::NP];
@@ -528,7 +536,7 @@ __global__ void __launch_bounds__(NT) backward_kernel(Grads<T> out, typename Acc
                                                       const typename AccOf<T>::type* __restrict__ dt_bias, const T* __restrict__ z,
                                                       const int* __restrict__ lengths, const typename AccOf<T>::type* __restrict__ saved, Args a) {
     typedef typename AccOf<T>::type A;
-    typedef Shape<T, P> Sh;
+    typedef Tile<T, P, NT> Sh;
     constexpr int CH = Sh::CH, TT = Sh::TT, V = Sh::V, NP = Sh::NP;
     extern __shared__ __align__(16) unsigned char raw_shared[];
     BackwardShared<T, P>& sh = *reinterpret_cast<BackwardShared<T, P>*>(raw_shared);
@@ -891,7 +899,7 @@ struct Operands {
 template <typename T, int P>
 int forward_p(void* y, void* h_out, void* saved, const Operands& o, const void* h_in, void* ws, const RpbScan* c, cudaStream_t s) {
     typedef typename AccOf<T>::type A;
-    typedef Shape<T, P> Sh;
+    typedef Forward<T, P> Sh;
     Args a = make_args(c);
     const Rowset r = rows_of(c, o.x, o.dt, o.B, o.C, o.z, y);
     const A *Am = reinterpret_cast<const A*>(o.A), *Dv = reinterpret_cast<const A*>(o.D), *bias = reinterpret_cast<const A*>(o.dt_bias);
@@ -922,11 +930,11 @@ int forward_p(void* y, void* h_out, void* saved, const Operands& o, const void* 
     SEQ_CUDA(cudaFuncSetAttribute(forward_kernel<T, P, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ForwardShared<T, P, true>)));
     SEQ_CUDA(cudaFuncSetAttribute(forward_kernel<T, P, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ForwardShared<T, P, false>)));
     if (a.chunks > 1) {
-        SEQ_CUDA(rpb_launch(forward_kernel<T, P, true>, dim3((unsigned)blocks), dim3(2 * NT), sizeof(ForwardShared<T, P, true>), s, 1, reinterpret_cast<T*>(y), ho, reinterpret_cast<A*>(saved),
+        SEQ_CUDA(rpb_launch(forward_kernel<T, P, true>, dim3((unsigned)blocks), dim3(NT + Forward<T, P>::NL), sizeof(ForwardShared<T, P, true>), s, 1, reinterpret_cast<T*>(y), ho, reinterpret_cast<A*>(saved),
                             chunk_h, chunk_s, x, dt, Am, B, C, Dv, bias, z, hi, o.lengths, a));
         rpb_count_launches(1);
     }
-    SEQ_CUDA(rpb_launch(forward_kernel<T, P, false>, dim3((unsigned)blocks), dim3(2 * NT), sizeof(ForwardShared<T, P, false>), s, 1, reinterpret_cast<T*>(y), ho, reinterpret_cast<A*>(saved),
+    SEQ_CUDA(rpb_launch(forward_kernel<T, P, false>, dim3((unsigned)blocks), dim3(NT + Forward<T, P>::NL), sizeof(ForwardShared<T, P, false>), s, 1, reinterpret_cast<T*>(y), ho, reinterpret_cast<A*>(saved),
                         chunk_h, chunk_s, x, dt, Am, B, C, Dv, bias, z, hi, o.lengths, a));
     rpb_count_launches(1);
     return 0;
@@ -941,7 +949,7 @@ template <typename T, int P>
 int backward_p(const Wanted& w, const void* dy, const void* dh_out, const Operands& o, const void* saved, void* ws, const RpbScan* c,
                cudaStream_t s) {
     typedef typename AccOf<T>::type A;
-    typedef Shape<T, P> Sh;
+    typedef Tile<T, P, NT> Sh;
     Args a = make_args(c);
     const Rowset r = rows_of(c, o.x, o.dt, o.B, o.C, o.z, dy);
     const A *Am = reinterpret_cast<const A*>(o.A), *Dv = reinterpret_cast<const A*>(o.D), *bias = reinterpret_cast<const A*>(o.dt_bias);

@@ -120,6 +120,25 @@ __device__ __forceinline__ float softplus_of(float v) {
 }
 __device__ __forceinline__ double softplus_of(double v) { return fmax(v, 0.0) + log1p(exp(-fabs(v))); }
 
+/* softplus of V values: in float two at a time */
+template <int V> __device__ __forceinline__ void softplus_all(double (&v)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = softplus_of(v[i]);
+}
+template <int V> __device__ __forceinline__ void softplus_all(float (&v)[V]) {
+    if (V % 2) v[V - 1] = softplus_of(v[V - 1]);
+#pragma unroll
+    for (int i = 0; i < V / 2 * 2; i += 2) {
+        const f32x2 e = pack2(__expf(-fabsf(v[i])), __expf(-fabsf(v[i + 1])));
+        const float c[9] = {0.019542528316378593f, -0.05637361481785774f, 0.10543623566627502f, -0.1526966691017151f, 0.1966327428817749f,
+                            -0.24951615929603577f, 0.33329710364341736f, -0.49999892711639404f, 1.0f};
+        f32x2 p = pack2(-0.0031760570127516985f, -0.0031760570127516985f);
+#pragma unroll
+        for (int k = 0; k < 9; ++k) p = fma2(p, e, pack2(c[k], c[k]));
+        unpack2(fma2(p, e, pack2(fmaxf(v[i], 0.0f), fmaxf(v[i + 1], 0.0f))), v[i], v[i + 1]);
+    }
+}
+
 /* Runs a call on the tensors' device and gives the caller's current device back. */
 struct DeviceScope {
     int prev = -1; bool moved = false;

@@ -226,6 +226,21 @@ def test_forward_and_backward(lib, dtype, n):
         check(lib, s, n, groups, int(k != 4), dtype, f"{dtype} n={n} {batch}x{length}x{d}/{groups}")
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n,d,groups", [(4, 256, 1), (4, 144, 2), (8, 160, 1), (12, 64, 1), (16, 96, 1), (24, 80, 2), (24, 650, 2), (28, 16, 1), (32, 48, 1),
+                                        (44, 40, 1), (60, 24, 1), (64, 16, 1)])
+def test_aligned_layouts(lib, dtype, n, d, groups):
+    """Every operand aligned for whole packs, states in whole groups of four but not in powers of two; the columns behind B and
+    C hold infinities, which nothing may reach; several tiles, the last one ragged."""
+    length = 75
+    s = make(2, length, d, n, groups, dtype, n + d, state=True)
+    for k in ("B", "C"):
+        wide = torch.full((2, length, groups * n + 16), float("inf"), dtype=s[k].dtype, device="cuda")
+        wide[:, :, :groups * n] = s[k]
+        s[k] = wide[:, :, :groups * n]
+    check(lib, s, n, groups, 1, dtype, f"{dtype} n={n} d={d}/{groups}")
+
+
 @pytest.mark.parametrize("dtype,n", [("bfloat16", 16), ("float32", 16), ("float32", 3), ("float64", 10), ("float16", 40)])
 def test_split_sequences(lib, dtype, n):
     """One sequence of few channels is split into chunks; same checks, with states entering and gradients leaving."""
