@@ -95,14 +95,17 @@ template <int BYTES> __device__ __forceinline__ void async_copy(void* to, const 
 __device__ __forceinline__ void async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-template <typename T, int V, bool FAST> __device__ __forceinline__ void bring(Pack<T, V>* to, const T* p, bool on, int valid, bool vec) {
-    if (FAST) {
-        constexpr int BYTES = sizeof(T) * V, STEP = BYTES < 16 ? BYTES : 16;
+template <typename T, int V> __device__ __forceinline__ void bring(Pack<T, V>* to, const T* p, bool on) {
+    constexpr int BYTES = sizeof(T) * V, STEP = BYTES < 16 ? BYTES : 16;
 #pragma unroll
-        for (int i = 0; i < BYTES; i += STEP) async_copy<STEP>(reinterpret_cast<char*>(to) + i, reinterpret_cast<const char*>(p) + i, on);
-    } else {
-        *to = on ? load_pack<T, V>(p, valid, vec) : zero_pack<T, V>();
-    }
+    for (int i = 0; i < BYTES; i += STEP) async_copy<STEP>(reinterpret_cast<char*>(to) + i, reinterpret_cast<const char*>(p) + i, on);
+}
+/* the same into registers, value by value: nothing is assumed about alignment */
+template <typename T, int V> __device__ __forceinline__ void pick(Pack<T, V>& to, const T* p, bool on, int valid) {
+    to = zero_pack<T, V>();
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (on && i < valid) to.v[i] = p[i];
 }
 
 /* Where a block works: sequence, group, first channel, channels left in the group, chunk of rows. */
@@ -340,23 +343,53 @@ forward_kernel(T* __restrict__ y, typename AccOf<T>::type* h_out, typename AccOf
         }
         const int rows = (end < last ? end : last) - first;
         int t2 = 0, slot2 = 0;                      /* of the next fetch: row from `first`, slot of the ring */
+        /* without FAST a tile's values wait in registers until the next iteration, which puts them into their slot */
+        Pack<T, V> hold_x, hold_dt, hold_z;
+        Pack<T, S> hold_b[UNITS], hold_c[UNITS];
+        int held = -1;
         auto fetch = [&]() {
             const bool row = t2 + lr < rows;
-            bring<T, V, FAST>(&sh.raw_x[slot2][tid], xp, row, lvalid, a.vec_x);
-            bring<T, V, FAST>(&sh.raw_dt[slot2][tid], dp, row, lvalid, a.vec_dt);
-            if (!AGG && z) bring<T, V, FAST>(&sh.raw_z[slot2][AGG ? 0 : tid], zp, row, lvalid, a.vec_z);
+            if (FAST) {
+                bring(&sh.raw_x[slot2][tid], xp, row);
+                bring(&sh.raw_dt[slot2][tid], dp, row);
+                if (!AGG && z) bring(&sh.raw_z[slot2][AGG ? 0 : tid], zp, row);
+            } else {
+                pick(hold_x, xp, row, lvalid);
+                pick(hold_dt, dp, row, lvalid);
+                if (!AGG && z) pick(hold_z, zp, row, lvalid);
+                held = slot2;
+            }
 #pragma unroll
             for (int k = 0; k < UNITS; ++k) {
                 const int e = tid + k * NL, r = e / P, n = (e % P) * S;
                 if (e >= TT * P) break;
                 const bool in = t2 + r < rows && n < a.states;
-                bring<T, S, FAST>(&sh.raw_b[slot2][e], bp + r * a.b_row + n, in, a.states - n, false);
-                if (!AGG) bring<T, S, FAST>(&sh.raw_c[slot2][AGG ? 0 : e], cp + r * a.c_row + n, in, a.states - n, false);
+                if (FAST) {
+                    bring(&sh.raw_b[slot2][e], bp + r * a.b_row + n, in);
+                    if (!AGG) bring(&sh.raw_c[slot2][AGG ? 0 : e], cp + r * a.c_row + n, in);
+                } else {
+                    pick(hold_b[k], bp + r * a.b_row + n, in, a.states - n);
+                    if (!AGG) pick(hold_c[k], cp + r * a.c_row + n, in, a.states - n);
+                }
             }
             t2 += TT;
             slot2 = slot2 + 1 == SLOTS ? 0 : slot2 + 1;
             xp += TT * a.x_row; dp += TT * a.dt_row; bp += TT * a.b_row; cp += TT * a.c_row;
             if (zp) zp += TT * a.z_row;
+        };
+        auto settle = [&]() {
+            if (FAST || held < 0) return;
+            sh.raw_x[held][tid] = hold_x;
+            sh.raw_dt[held][tid] = hold_dt;
+            if (!AGG && z) sh.raw_z[AGG ? 0 : held][AGG ? 0 : tid] = hold_z;
+#pragma unroll
+            for (int k = 0; k < UNITS; ++k) {
+                const int e = tid + k * NL;
+                if (e >= TT * P) break;
+                sh.raw_b[held][e] = hold_b[k];
+                if (!AGG) sh.raw_c[AGG ? 0 : held][AGG ? 0 : e] = hold_c[k];
+            }
+            held = -1;
         };
         auto stage = [&](int tile, int slot) {
             const bool row = tile * TT + lr < rows;
@@ -418,15 +451,18 @@ forward_kernel(T* __restrict__ y, typename AccOf<T>::type* h_out, typename AccOf
         auto next = [](int slot) { return slot + 1 == SLOTS ? 0 : slot + 1; };
 #pragma unroll
         for (int k = 0; k <= DEPTH; ++k) {
+            settle();
             if (k < tiles) fetch();
             async_commit();
         }
+        settle();
         async_wait<DEPTH>();
         stage(0, 0);
         __syncthreads();
         int done = SLOTS - 1, ahead = 1 % SLOTS;    /* slots of tile - 1 and tile + 1 */
         for (int tile = 0; tile < tiles; ++tile) {
             async_wait<DEPTH - 1>();                /* tile + 1 is there */
+            settle();
             if (tile + 1 < tiles) stage(tile + 1, ahead);
             if (!AGG && tile > 0) finish(tile - 1, done);
             if (tile + 1 + DEPTH < tiles) fetch();  /* into the slot of tile - 1 */
