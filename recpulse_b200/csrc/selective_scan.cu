@@ -539,22 +539,89 @@ __global__ void __launch_bounds__(256) token_kernel(T* __restrict__ y, typename 
     }
 }
 
+/* Four states' worth of values: in float two register pairs, so that one instruction works on two. */
+template <typename A> struct V4 {
+    A v[S];
+    __device__ __forceinline__ void set(const A (&x)[S]) { for (int i = 0; i < S; ++i) v[i] = x[i]; }
+    __device__ __forceinline__ void get(A (&x)[S]) const { for (int i = 0; i < S; ++i) x[i] = v[i]; }
+};
+template <> struct V4<float> {
+    f32x2 a, b;
+    __device__ __forceinline__ void set(const float (&x)[S]) { a = pack2(x[0], x[1]); b = pack2(x[2], x[3]); }
+    __device__ __forceinline__ void get(float (&x)[S]) const { unpack2(a, x[0], x[1]); unpack2(b, x[2], x[3]); }
+};
+__device__ __forceinline__ V4<float> mul(const V4<float>& x, const V4<float>& y) { return {mul2(x.a, y.a), mul2(x.b, y.b)}; }
+__device__ __forceinline__ V4<float> mul(const V4<float>& x, float y) { const f32x2 s = pack2(y, y); return {mul2(x.a, s), mul2(x.b, s)}; }
+__device__ __forceinline__ V4<float> mad(const V4<float>& x, const V4<float>& y, const V4<float>& z) { return {fma2(x.a, y.a, z.a), fma2(x.b, y.b, z.b)}; }
+__device__ __forceinline__ V4<float> mad(const V4<float>& x, float y, const V4<float>& z) { const f32x2 s = pack2(y, y); return {fma2(x.a, s, z.a), fma2(x.b, s, z.b)}; }
+__device__ __forceinline__ float dot(const V4<float>& x, const V4<float>& y) {
+    float lo, hi;
+    unpack2(fma2(x.a, y.a, mul2(x.b, y.b)), lo, hi);
+    return lo + hi;
+}
+__device__ __forceinline__ V4<float> decays(float delta, const V4<float>& rate) {
+    float e0, e1, e2, e3;
+    const V4<float> e = mul(rate, delta);
+    unpack2(e.a, e0, e1); unpack2(e.b, e2, e3);
+    return {pack2(ex2_fast(e0), ex2_fast(e1)), pack2(ex2_fast(e2), ex2_fast(e3))};
+}
+/* (x0, x1, x2, x3) -> (x2, x3, x0, x1) */
+__device__ __forceinline__ V4<float> swap_halves(const V4<float>& x, bool on) { return on ? V4<float>{x.b, x.a} : x; }
+/* gives the upper half to lane ^ mask and adds what comes to the lower half */
+__device__ __forceinline__ void fold_halves(const V4<float>& x, int mask, float& lo, float& hi) {
+    float g0, g1;
+    unpack2(x.b, g0, g1);
+    g0 = __shfl_xor_sync(0xffffffffu, g0, mask); g1 = __shfl_xor_sync(0xffffffffu, g1, mask);
+    unpack2(add2(x.a, pack2(g0, g1)), lo, hi);
+}
+__device__ __forceinline__ V4<double> mul(const V4<double>& x, const V4<double>& y) { V4<double> r; for (int i = 0; i < S; ++i) r.v[i] = x.v[i] * y.v[i]; return r; }
+__device__ __forceinline__ V4<double> mul(const V4<double>& x, double y) { V4<double> r; for (int i = 0; i < S; ++i) r.v[i] = x.v[i] * y; return r; }
+__device__ __forceinline__ V4<double> mad(const V4<double>& x, const V4<double>& y, const V4<double>& z) {
+    V4<double> r; for (int i = 0; i < S; ++i) r.v[i] = x.v[i] * y.v[i] + z.v[i]; return r;
+}
+__device__ __forceinline__ V4<double> mad(const V4<double>& x, double y, const V4<double>& z) { V4<double> r; for (int i = 0; i < S; ++i) r.v[i] = x.v[i] * y + z.v[i]; return r; }
+__device__ __forceinline__ double dot(const V4<double>& x, const V4<double>& y) { double r = x.v[0] * y.v[0]; for (int i = 1; i < S; ++i) r += x.v[i] * y.v[i]; return r; }
+__device__ __forceinline__ V4<double> decays(double delta, const V4<double>& rate) { V4<double> r; for (int i = 0; i < S; ++i) r.v[i] = decay(delta, rate.v[i]); return r; }
+__device__ __forceinline__ V4<double> swap_halves(const V4<double>& x, bool on) {
+    V4<double> r; for (int i = 0; i < S; ++i) r.v[i] = on ? x.v[i ^ 2] : x.v[i]; return r;
+}
+__device__ __forceinline__ void fold_halves(const V4<double>& x, int mask, double& lo, double& hi) {
+    lo = x.v[0] + __shfl_xor_sync(0xffffffffu, x.v[2], mask); hi = x.v[1] + __shfl_xor_sync(0xffffffffu, x.v[3], mask);
+}
+
 /* ------------------------------------------------------------------------------------------------ backward
- * A block walks its chunk's tiles from the last to the first.  Within a tile each thread takes segments of SEG rows: from
- * the saved state in front of the segment it runs the rows forward once more, with the states and decays of all rows in
- * registers, and then backward.  Sums over the states of a channel and over the channels of a warp are taken by exchanging
- * halves between lanes, so that every lane ends with a sum of its own.
+ * Walkers and loaders as in the forward call, over a chunk's tiles from the last to the first.  Walkers take a tile in
+ * segments of SEG rows: from the saved state in front of the segment they run the rows forward once more, with the states and
+ * decays of all rows in registers, and then backward.  Sums over the states of a channel (for dx, ddt, dz) and over the
+ * channels of a warp (for dB, dC) are taken by exchanging halves between lanes, so that every lane ends with a sum of its own.
+ * Lanes of odd channels hold their four states with the halves swapped (from copies of B and C in that order): the half to
+ * give away is then in the same registers in every lane, and the first and largest exchange needs no selection.
  * AGG: as in the forward call, from the chunk's end: the gradient that leaves the chunk's first row when none enters at its
  * end, and the sum of the deltas. */
-template <typename T, int P> struct BackwardShared {
+template <typename T, int P> struct Backward {
+    static constexpr int CH = NT / P, TT = P == 1 || sizeof(T) == 8 ? 8 : 16, NP = S * P, NL = NT;
+    static constexpr int V = CH * TT >= NL ? CH * TT / NL : 1, K = CH / V;      /* loaders behind the TT-th row have nothing to do */
+    static constexpr int ROW = CH + 2, QROW = CH + 4;
+    static constexpr int UNITS = (TT * P + NL - 1) / NL;
+    static constexpr int DEPTH = sizeof(T) == 2 ? 3 : sizeof(T) == 4 ? 2 : 1, SLOTS = DEPTH + 2;
+    /* Blocks per SM that the registers allow, and whether walkers and loaders divide them unevenly: with up to 8 states both
+     * have more to hold, and one block takes all. */
+    static constexpr int RESIDENT = P <= 2 || sizeof(T) == 8 ? 1 : 2;
+    static constexpr bool UNEVEN = RESIDENT == 2;
+    static constexpr bool PACKS = sizeof(T) * V >= 4 && sizeof(T) * S >= 4;      /* large enough for asynchronous copies */
+};
+
+template <typename T, int P, bool AGG> struct BackwardShared {
     typedef typename AccOf<T>::type A;
-    typedef Tile<T, P, NT> Sh;
-    Pair<A> pairs[Sh::TT][Sh::CH];
-    A dys[Sh::TT][Sh::CH];
-    A Bs[Sh::TT][Sh::NP], Cs[Sh::TT][Sh::NP];
-    A q[Sh::TT][Sh::CH + Sh::PAD], r[Sh::TT][Sh::CH + Sh::PAD], yc[Sh::TT][Sh::CH + Sh::PAD];
-    A dB[NT / 32][Sh::TT][Sh::NP], dC[NT / 32][Sh::TT][Sh::NP];
-    A dD[NT][Sh::V], dbias[NT][Sh::V];
+    typedef Backward<T, P> Sh;
+    static constexpr int SLOTS = Sh::SLOTS, NL = Sh::NL, TT = Sh::TT, ONE = AGG ? 1 : TT;
+    Pack<T, Sh::V> raw_x[SLOTS][NL], raw_dt[SLOTS][NL], raw_z[SLOTS][NL], raw_dy[SLOTS][NL];
+    Pack<T, S> raw_b[AGG ? 1 : SLOTS][AGG ? 1 : TT * P], raw_c[SLOTS][TT * P];
+    alignas(16) Pair<A> pairs[2][TT][Sh::ROW];
+    alignas(16) A dys[2][TT][Sh::QROW];
+    alignas(16) A Bs[2][ONE][2][Sh::NP], Cs[2][TT][2][Sh::NP];
+    alignas(16) A q[2][ONE][Sh::QROW], r[2][ONE][Sh::QROW], yc[2][ONE][Sh::QROW];
+    alignas(16) A dB[2][NT / 32][ONE][Sh::NP], dC[2][NT / 32][ONE][Sh::NP];
 };
 
 template <typename T> struct Grads {
@@ -562,251 +629,406 @@ template <typename T> struct Grads {
     T *dx, *ddt, *dz;
     A *dh_in, *parts, *part_b, *part_c;     /* parts: per (sequence, chunk) dA [channels, states], dD, ddt_bias [channels] */
     int acc_dx, acc_ddt, acc_dz;
+    bool vec_part;                          /* part_b, part_c in whole groups of four */
 };
 
+/* 256 threads launched with 128 registers each: the walkers, who keep a segment's history, take 168 and the loaders 88 (the
+ * launch makes sure of the 128: with fewer the walkers would wait for good) */
+template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
 template <typename T, int P, bool AGG>
-__global__ void __launch_bounds__(NT) backward_kernel(Grads<T> out, typename AccOf<T>::type* __restrict__ chunk_g, typename AccOf<T>::type* __restrict__ chunk_s,
-                                                      const T* __restrict__ dy, const typename AccOf<T>::type* __restrict__ dh_out,
-                                                      const T* __restrict__ x, const T* __restrict__ dt, const typename AccOf<T>::type* __restrict__ Am,
-                                                      const T* __restrict__ Bm, const T* __restrict__ Cm, const typename AccOf<T>::type* __restrict__ Dv,
-                                                      const typename AccOf<T>::type* __restrict__ dt_bias, const T* __restrict__ z,
-                                                      const int* __restrict__ lengths, const typename AccOf<T>::type* __restrict__ saved, Args a) {
+__global__ void __launch_bounds__(2 * NT, Backward<T, P>::RESIDENT)
+backward_kernel(Grads<T> out, typename AccOf<T>::type* __restrict__ chunk_g, typename AccOf<T>::type* __restrict__ chunk_s, const T* __restrict__ dy,
+                const typename AccOf<T>::type* __restrict__ dh_out, const T* __restrict__ x, const T* __restrict__ dt,
+                const typename AccOf<T>::type* __restrict__ Am, const T* __restrict__ Bm, const T* __restrict__ Cm,
+                const typename AccOf<T>::type* __restrict__ Dv, const typename AccOf<T>::type* __restrict__ dt_bias, const T* __restrict__ z,
+                const int* __restrict__ lengths, const typename AccOf<T>::type* __restrict__ saved, Args a) {
     typedef typename AccOf<T>::type A;
-    typedef Tile<T, P, NT> Sh;
-    constexpr int CH = Sh::CH, TT = Sh::TT, V = Sh::V, NP = Sh::NP;
+    typedef Backward<T, P> Sh;
+    constexpr int CH = Sh::CH, TT = Sh::TT, V = Sh::V, NP = Sh::NP, K = Sh::K, NL = Sh::NL;
+    constexpr bool SPLIT = !AGG && Sh::UNEVEN;
     extern __shared__ __align__(16) unsigned char raw_shared[];
-    BackwardShared<T, P>& sh = *reinterpret_cast<BackwardShared<T, P>*>(raw_shared);
+    BackwardShared<T, P, AGG>& sh = *reinterpret_cast<BackwardShared<T, P, AGG>*>(raw_shared);
+    static_assert(sizeof(sh) <= 226 * 1024, "");
     rpb_pdl_trigger();
     rpb_pdl_wait();
     const Place pl = place_of<CH>(a);
     if (AGG && pl.c == 0) return;       /* nothing is in front of it */
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int end = row_end(lengths, pl.b, a.len);
     const int first = pl.c * a.chunk, last = first + a.chunk < a.len ? first + a.chunk : a.len;
-    const int lr = tid / (CH / V), lc = (tid % (CH / V)) * V, lvalid = pl.valid - lc;
-    const T* xp = x + pl.b * a.x_batch + pl.d0 + lc;
-    const T* dp = dt + pl.b * a.dt_batch + pl.d0 + lc;
-    const T* zp = z ? z + pl.b * a.z_batch + pl.d0 + lc : nullptr;
-    const T* gp = dy + pl.b * a.y_batch + pl.d0 + lc;
-    const T* bp = Bm + pl.b * a.b_batch + pl.g * a.states;
-    const T* cp = Cm + pl.b * a.c_batch + pl.g * a.states;
-    const long long segs = (a.len + SEG - 1) / SEG;
-
-    const int p = tid % P, ch = tid / P, n0 = p * S;
-    const bool on = ch < pl.valid;
-    const long long d = pl.d0 + ch;
-    A rate[S], Av[S], g[S], dA[S], sum = 0;
-#pragma unroll
-    for (int i = 0; i < S; ++i) {
-        Av[i] = on && n0 + i < a.states ? Am[d * a.states + n0 + i] : A(0);
-        rate[i] = decay_rate(Av[i]);
-        g[i] = dA[i] = 0;
-    }
-    if (!AGG && on) {
-        if (dh_out) load_states(g, dh_out + (pl.b * (long long)a.channels + d) * a.states, n0, a.states, a.vec_n);
-        for (int c = a.chunks - 1; c > pl.c; --c) {
-            const long long at = (pl.b * (long long)a.chunks + c) * a.channels + d;
-            A part[S];
-            load_states(part, chunk_g + at * a.states, n0, a.states, a.vec_n);
-            const A s = chunk_s[at];
-#pragma unroll
-            for (int i = 0; i < S; ++i) g[i] = decay(s, rate[i]) * g[i] + part[i];
-        }
-    }
-    if (!AGG) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) sh.dD[tid][i] = sh.dbias[tid][i] = 0;
-    }
+    const int rows = (end < last ? end : last) - first;         /* of the sequence, in this chunk; may be negative */
     const int tiles = (last - first + TT - 1) / TT;
-    for (int tile = tiles - 1; tile >= 0; --tile) {
-        const int t0 = first + tile * TT, t = t0 + lr;
-        const bool row = t < last && t < end;
+    const long long D = a.channels;
+
+    if (threadIdx.x < NT) {
+        if (SPLIT) more_registers<168>();
+        const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+        const int p = tid % P, ch = tid / P, n0 = p * S;
+        const int odd = (lane / P) & 1;
+        const bool on = ch < pl.valid;
+        const long long d = pl.d0 + ch;
+        V4<A> rate, Av, g, dA;
+        A sum = 0;
         {
-            const Pack<T, V> xr = row ? load_pack<T, V>(xp + t * a.x_row, lvalid, a.vec_x) : zero_pack<T, V>();
-            const Pack<T, V> dr = row ? load_pack<T, V>(dp + t * a.dt_row, lvalid, a.vec_dt) : zero_pack<T, V>();
-            const Pack<T, V> zr = row && zp ? load_pack<T, V>(zp + t * a.z_row, lvalid, a.vec_z) : zero_pack<T, V>();
-            const Pack<T, V> gr = row ? load_pack<T, V>(gp + t * a.y_row, lvalid, a.vec_y) : zero_pack<T, V>();
+            A t0[S], t1[S], z0[S];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const bool in = row && i < lvalid;
-                const A bias = dt_bias && in ? dt_bias[pl.d0 + lc + i] : A(0);
-                const A dl = in ? delta_of<T, A>(dr.v[i], bias, a.softplus) : A(0);
-                A gy = up(gr.v[i]);
-                if (zp) { const A zv = up(zr.v[i]); gy *= zv * logistic(zv); }
-                sh.pairs[lr][lc + i] = Pair<A>{dl, dl * up(xr.v[i])};
-                sh.dys[lr][lc + i] = in ? gy : A(0);
+            for (int i = 0; i < S; ++i) {
+                t0[i] = on && n0 + i < a.states ? Am[d * a.states + n0 + i] : A(0);
+                t1[i] = decay_rate(t0[i]);
+                z0[i] = 0;
             }
-            for (int e = tid; e < TT * NP; e += NT) {
-                const int r = e / NP, n = e - r * NP;
-                const bool in = t0 + r < last && t0 + r < end && n < a.states;
-                if (!AGG) sh.Bs[r][n] = in ? up(bp[(t0 + r) * a.b_row + n]) : A(0);
-                sh.Cs[r][n] = in ? up(cp[(t0 + r) * a.c_row + n]) : A(0);
-            }
-        }
-        __syncthreads();
-        if constexpr (AGG) {
+            Av.set(t0); rate.set(t1); g.set(z0); dA.set(z0);
+            if (!AGG && on) {
+                if (dh_out) { load_states(t0, dh_out + (pl.b * D + d) * a.states, n0, a.states, a.vec_n); g.set(t0); }
 #pragma unroll 4
-            for (int k = TT - 1; k >= 0; --k) {
-                const A dl = sh.pairs[k][ch].delta, gy = sh.dys[k][ch];
-                const Pack<A, S> cv = *reinterpret_cast<const Pack<A, S>*>(&sh.Cs[k][n0]);
-                sum += dl;
-#pragma unroll
-                for (int i = 0; i < S; ++i) g[i] = (g[i] + cv.v[i] * gy) * decay(dl, rate[i]);
-            }
-        } else {
-        /* One segment; PARTIAL: rows from `live` on are not part of the sequence (or the chunk).  Their decay is 1 and nothing
-         * enters, so the state and its gradient pass through them, and their results are 0 whatever the state holds. */
-        auto segment = [&](int r0, int live, auto partial) {
-            constexpr bool PARTIAL = decltype(partial)::value;
-            A h0[S] = {0, 0, 0, 0}, av[SEG][S], h[SEG][S];
-            if (on && t0 + r0 < last) load_states(h0, saved + ((pl.b * segs + (t0 + r0) / SEG) * a.channels + d) * a.states, n0, a.states, a.vec_n);
-            A yv[SEG], qv[SEG], rv[SEG];
-#pragma unroll
-            for (int k = 0; k < SEG; ++k) {
-                const Pair<A> pr = sh.pairs[r0 + k][ch];
-                const Pack<A, S> bv = *reinterpret_cast<const Pack<A, S>*>(&sh.Bs[r0 + k][n0]);
-                const Pack<A, S> cv = *reinterpret_cast<const Pack<A, S>*>(&sh.Cs[r0 + k][n0]);
-                yv[k] = 0;
-#pragma unroll
-                for (int i = 0; i < S; ++i) {
-                    av[k][i] = decay(pr.delta, rate[i]);
-                    h[k][i] = av[k][i] * (k ? h[k - 1][i] : h0[i]) + pr.dx * bv.v[i];
-                    yv[k] += h[k][i] * cv.v[i];
+                for (int c = a.chunks - 1; c > pl.c; --c) {
+                    const long long at = (pl.b * (long long)a.chunks + c) * D + d;
+                    V4<A> part;
+                    load_states(t0, chunk_g + at * a.states, n0, a.states, a.vec_n);
+                    part.set(t0);
+                    g = mad(decays(chunk_s[at], rate), g, part);
                 }
             }
-            /* M lanes of a warp hold the same states of M channels; MS rows give one sum (or more) per lane */
-            constexpr int M = 32 / P, MS = M / S < 1 ? 1 : M / S;
-            static_assert(SEG % MS == 0, "");
-            A bsum[MS * S], csum[MS * S];
-#pragma unroll
-            for (int k = SEG - 1; k >= 0; --k) {
-                const Pair<A> pr = sh.pairs[r0 + k][ch];
-                const A gy = sh.dys[r0 + k][ch];
-                const Pack<A, S> bv = *reinterpret_cast<const Pack<A, S>*>(&sh.Bs[r0 + k][n0]);
-                const Pack<A, S> cv = *reinterpret_cast<const Pack<A, S>*>(&sh.Cs[r0 + k][n0]);
-                qv[k] = rv[k] = 0;
-                if (PARTIAL && k >= live) {
-#pragma unroll
-                    for (int i = 0; i < S; ++i) bsum[(k % MS) * S + i] = csum[(k % MS) * S + i] = 0;
-                } else {
-#pragma unroll
-                for (int i = 0; i < S; ++i) {
-                    const A dh = g[i] + cv.v[i] * gy;
-                    g[i] = dh * av[k][i];
-                    const A da = g[i] * (k ? h[k - 1][i] : h0[i]);
-                    qv[k] += dh * bv.v[i];
-                    rv[k] += da * Av[i];
-                    dA[i] += da * pr.delta;
-                    bsum[(k % MS) * S + i] = dh * pr.dx;
-                    csum[(k % MS) * S + i] = gy * h[k][i];
-                }
-                }
-                if (k % MS == 0) {
-                    sum_lanes<MS * S, M, P>(bsum, lane);
-                    sum_lanes<MS * S, M, P>(csum, lane);
-                    constexpr int LEFT = MS * S / M;
-                    const int m = lane / P;
-#pragma unroll
-                    for (int e = 0; e < LEFT; ++e) {
-                        const int at = m * LEFT + e;
-                        sh.dB[warp][r0 + k + at / S][n0 + at % S] = bsum[e];
-                        sh.dC[warp][r0 + k + at / S][n0 + at % S] = csum[e];
-                    }
-                }
-            }
-            /* over the P lanes of a channel: G rows at a time, each lane left with one */
-            constexpr int G = P < SEG ? P : SEG;
-#pragma unroll
-            for (int k = 0; k < SEG; k += G) {
-                A v0[G], v1[G], v2[G];
-#pragma unroll
-                for (int i = 0; i < G; ++i) { v0[i] = qv[k + i]; v1[i] = rv[k + i]; v2[i] = yv[k + i]; }
-                sum_lanes<G, P, 1>(v0, lane);
-                sum_lanes<G, P, 1>(v1, lane);
-                if (zp) sum_lanes<G, P, 1>(v2, lane);
-                const int mine = r0 + k + p / (P / G);
-                if (p % (P / G) == 0) { sh.q[mine][ch] = v0[0]; sh.r[mine][ch] = v1[0]; if (zp) sh.yc[mine][ch] = v2[0]; }
-            }
+            Av = swap_halves(Av, odd); rate = swap_halves(rate, odd); g = swap_halves(g, odd);
+        }
+        /* the states in front of the segments, the next one's on their way while one is worked on */
+        const long long seg_stride = D * a.states;
+        const A* keep = nullptr;
+        A h_next[S] = {0, 0, 0, 0};
+        auto ahead = [&](int t) {           /* of the segment that begins at row t from `first` */
+            if (keep && t >= 0 && first + t < last) load_states(h_next, keep + t / SEG * seg_stride, n0, a.states, a.vec_n);
         };
-        const int stop = (end < last ? end : last) - t0;
-        for (int r0 = TT - SEG; r0 >= 0; r0 -= SEG) {
-            if (r0 + SEG <= stop) segment(r0, SEG, std::false_type());
-            else segment(r0, stop - r0, std::true_type());
-        }
+        if (!AGG && on) keep = saved + ((pl.b * (long long)((a.len + SEG - 1) / SEG) + first / SEG) * D + d) * a.states;
+        if (!AGG) ahead(tiles * TT - SEG);
         __syncthreads();
-        if (t < last && lvalid > 0) {
-            const Pack<T, V> xr = row ? load_pack<T, V>(xp + t * a.x_row, lvalid, a.vec_x) : zero_pack<T, V>();
-            const Pack<T, V> dr = row ? load_pack<T, V>(dp + t * a.dt_row, lvalid, a.vec_dt) : zero_pack<T, V>();
-            const Pack<T, V> zr = row && zp ? load_pack<T, V>(zp + t * a.z_row, lvalid, a.vec_z) : zero_pack<T, V>();
-            const Pack<T, V> gr = row && zp ? load_pack<T, V>(gp + t * a.y_row, lvalid, a.vec_y) : zero_pack<T, V>();
-            T* dxp = out.dx ? out.dx + pl.b * a.dx_batch + t * a.dx_row + pl.d0 + lc : nullptr;
-            T* ddtp = out.ddt ? out.ddt + pl.b * a.ddt_batch + t * a.ddt_row + pl.d0 + lc : nullptr;
-            T* dzp = out.dz ? out.dz + pl.b * a.dz_batch + t * a.dz_row + pl.d0 + lc : nullptr;
-            Pack<T, V> o0 = zero_pack<T, V>(), o1 = o0, o2 = o0;
-            if (dxp && out.acc_dx) o0 = load_pack<T, V>(dxp, lvalid, a.vec_dx);
-            if (ddtp && out.acc_ddt) o1 = load_pack<T, V>(ddtp, lvalid, a.vec_ddt);
-            if (dzp && out.acc_dz) o2 = load_pack<T, V>(dzp, lvalid, a.vec_dz);
-            if (row) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    if (i >= lvalid) continue;
-                    const A xv = up(xr.v[i]), gy = sh.dys[lr][lc + i], q = sh.q[lr][lc + i];
-                    const A skip = Dv ? Dv[pl.d0 + lc + i] : A(0);
-                    A dd = sh.r[lr][lc + i] + xv * q;
-                    if (a.softplus) dd *= logistic(up(dr.v[i]) + (dt_bias ? dt_bias[pl.d0 + lc + i] : A(0)));
-                    o0.v[i] = down<T>(up(o0.v[i]) + sh.pairs[lr][lc + i].delta * q + skip * gy);
-                    o1.v[i] = down<T>(up(o1.v[i]) + dd);
-                    if (zp) {
-                        const A zv = up(zr.v[i]), s = logistic(zv);
-                        o2.v[i] = down<T>(up(o2.v[i]) + up(gr.v[i]) * (sh.yc[lr][lc + i] + skip * xv) * s * (A(1) + zv * (A(1) - s)));
-                    }
-                    sh.dD[tid][i] += gy * xv;
-                    sh.dbias[tid][i] += dd;
+        for (int it = 0; it < tiles; ++it) {
+            const int buf = it & 1, t0 = (tiles - 1 - it) * TT;
+            const Pair<A>* pairs = &sh.pairs[buf][0][ch];
+            const A* dys = &sh.dys[buf][0][ch];
+            const A *bs = &sh.Bs[buf][0][AGG ? 0 : odd][n0], *cs = &sh.Cs[buf][0][odd][n0];
+            if constexpr (AGG) {
+#pragma unroll 4
+                for (int k = TT - 1; k >= 0; --k) {
+                    const A dl = pairs[k * Sh::ROW].delta;
+                    const V4<A> cv = *reinterpret_cast<const V4<A>*>(cs + k * 2 * NP);
+                    sum += dl;
+                    g = mul(mad(cv, dys[k * Sh::QROW], g), decays(dl, rate));
                 }
-            }
-            if (dxp) store_pack<T, V>(dxp, o0, lvalid, a.vec_dx);
-            if (ddtp) store_pack<T, V>(ddtp, o1, lvalid, a.vec_ddt);
-            if (dzp) store_pack<T, V>(dzp, o2, lvalid, a.vec_dz);
-        }
-        /* the block's part of dB and dC: the warps' sums in turn */
-        const long long rows = (long long)a.batch * a.len;
-        const int blk = (pl.d0 - pl.g * a.per_group) / CH;
-        for (int e = tid; e < TT * NP; e += NT) {
-            const int r = e / NP, n = e - r * NP;
-            if (t0 + r >= last || n >= a.states) continue;
-            const long long at = ((blk * rows + (long long)pl.b * a.len + t0 + r) * a.groups + pl.g) * a.states + n;
-            A sb = sh.dB[0][r][n], sc = sh.dC[0][r][n];
+            } else {
+                /* dA of one tile, then added to the total: sums of at most 16 and of as many as there are tiles, where one sum
+                 * over all rows would have lost a digit */
+                V4<A> dA_tile = mul(dA, A(0));
+                /* PARTIAL: rows from `live` on are not part of the sequence (or the chunk).  Their decay is 1 and nothing enters,
+                 * so the state and its gradient pass through them, and their results are 0 whatever the state holds. */
+                auto segment = [&](int r0, int live, auto partial) {
+                    constexpr bool PARTIAL = decltype(partial)::value;
+                    V4<A> h0, av[SEG], h[SEG];
+                    h0.set(h_next);
+                    h0 = swap_halves(h0, odd);
+                    ahead(t0 + r0 - SEG);
+                    A yv[SEG], qv[SEG], rv[SEG];
 #pragma unroll
-            for (int w = 1; w < NT / 32; ++w) { sb += sh.dB[w][r][n]; sc += sh.dC[w][r][n]; }
-            if (out.part_b) out.part_b[at] = sb;
-            if (out.part_c) out.part_c[at] = sc;
+                    for (int k = 0; k < SEG; ++k) {
+                        const Pair<A> pr = pairs[(r0 + k) * Sh::ROW];
+                        const V4<A> bv = *reinterpret_cast<const V4<A>*>(bs + (r0 + k) * 2 * NP);
+                        const V4<A> cv = *reinterpret_cast<const V4<A>*>(cs + (r0 + k) * 2 * NP);
+                        av[k] = decays(pr.delta, rate);
+                        h[k] = mad(av[k], k ? h[k - 1] : h0, mul(bv, pr.dx));
+                        yv[k] = dot(h[k], cv);
+                    }
+                    /* M lanes of a warp hold the same states of M channels; MS rows give one sum (or two) per lane */
+                    constexpr int M = 32 / P, MS = M / S < 1 ? 1 : M / S, LEFT = MS * S / M;
+                    static_assert(SEG % MS == 0, "");
+                    A bsum[MS * 2], csum[MS * 2];
+#pragma unroll
+                    for (int k = SEG - 1; k >= 0; --k) {
+                        const Pair<A> pr = pairs[(r0 + k) * Sh::ROW];
+                        const A gy = dys[(r0 + k) * Sh::QROW];
+                        const V4<A> bv = *reinterpret_cast<const V4<A>*>(bs + (r0 + k) * 2 * NP);
+                        const V4<A> cv = *reinterpret_cast<const V4<A>*>(cs + (r0 + k) * 2 * NP);
+                        A *b2 = &bsum[k % MS * 2], *c2 = &csum[k % MS * 2];
+                        if (PARTIAL && k >= live) {
+                            qv[k] = rv[k] = yv[k] = b2[0] = b2[1] = c2[0] = c2[1] = 0;
+                        } else {
+                            const V4<A> dh = mad(cv, gy, g);
+                            g = mul(dh, av[k]);
+                            const V4<A> da = mul(g, k ? h[k - 1] : h0);
+                            qv[k] = dot(dh, bv);
+                            rv[k] = dot(da, Av);
+                            dA_tile = mad(da, pr.delta, dA_tile);
+                            fold_halves(mul(dh, pr.dx), P, b2[0], b2[1]);
+                            fold_halves(mul(h[k], gy), P, c2[0], c2[1]);
+                        }
+                        if (k % MS == 0) {
+                            sum_lanes<MS * 2, M / 2, 2 * P>(bsum, lane);
+                            sum_lanes<MS * 2, M / 2, 2 * P>(csum, lane);
+#pragma unroll
+                            for (int e = 0; e < LEFT; ++e) {
+                                const int at = lane / (2 * P) * LEFT + e, row = r0 + k + at / 2, n = n0 + 2 * odd + at % 2;
+                                sh.dB[buf][warp][row][n] = bsum[e];
+                                sh.dC[buf][warp][row][n] = csum[e];
+                            }
+                        }
+                    }
+                    /* over the P lanes of a channel: G rows at a time, each lane left with one */
+                    constexpr int G = P < SEG ? P : SEG;
+#pragma unroll
+                    for (int k = 0; k < SEG; k += G) {
+                        A v0[G], v1[G], v2[G];
+#pragma unroll
+                        for (int i = 0; i < G; ++i) { v0[i] = qv[k + i]; v1[i] = rv[k + i]; v2[i] = yv[k + i]; }
+                        sum_lanes<G, P, 1>(v0, lane);
+                        sum_lanes<G, P, 1>(v1, lane);
+                        if (z) sum_lanes<G, P, 1>(v2, lane);
+                        const int mine = r0 + k + p / (P / G);
+                        if (p % (P / G) == 0) { sh.q[buf][mine][ch] = v0[0]; sh.r[buf][mine][ch] = v1[0]; if (z) sh.yc[buf][mine][ch] = v2[0]; }
+                    }
+                };
+                const int stop = rows - t0;
+#pragma unroll 1
+                for (int r0 = TT - SEG; r0 >= 0; r0 -= SEG) {
+                    if (r0 + SEG <= stop) segment(r0, SEG, std::false_type());
+                    else segment(r0, stop - r0, std::true_type());
+                }
+                dA = mad(dA_tile, A(1), dA);
+            }
+            __syncthreads();
         }
-        }
-        __syncthreads();
-    }
-    if (AGG) {
-        if (on) {
-            const long long at = (pl.b * (long long)a.chunks + pl.c) * a.channels + d;
-            store_states(chunk_g + at * a.states, g, n0, a.states, a.vec_n);
+        if (!on) return;
+        A v[S];
+        swap_halves(g, odd).get(v);
+        if (AGG) {
+            const long long at = (pl.b * (long long)a.chunks + pl.c) * D + d;
+            store_states(chunk_g + at * a.states, v, n0, a.states, a.vec_n);
             if (p == 0) chunk_s[at] = sum;
+            return;
+        }
+        if (out.dh_in && pl.c == 0) store_states(out.dh_in + (pl.b * D + d) * a.states, v, n0, a.states, a.vec_n);
+        if (out.parts) {
+            swap_halves(dA, odd).get(v);
+            store_states(out.parts + (pl.b * (long long)a.chunks + pl.c) * D * (a.states + 2) + d * a.states, v, n0, a.states, false);
         }
         return;
     }
-    if (on && out.dh_in && pl.c == 0) store_states(out.dh_in + (pl.b * (long long)a.channels + d) * a.states, g, n0, a.states, a.vec_n);
-    if (!out.parts) return;
-    const long long D = a.channels;
-    A* part = out.parts + (pl.b * (long long)a.chunks + pl.c) * D * (a.states + 2);
-    if (on) store_states(part + d * a.states, dA, n0, a.states, false);
-    /* the loaders' sums of one channel: one per row of a tile, in turn */
-    for (int c = tid; c < CH && c < pl.valid; c += NT) {
-        A s0 = 0, s1 = 0;
-        for (int r = 0; r < TT; ++r) {
-            const int th = r * (CH / V) + c / V;
-            s0 += sh.dD[th][c % V]; s1 += sh.dbias[th][c % V];
+
+    if (SPLIT) fewer_registers<88>();
+    auto load = [&](auto fast) {
+        constexpr bool FAST = decltype(fast)::value;
+        constexpr int UNITS = Sh::UNITS, DEPTH = Sh::DEPTH, SLOTS = Sh::SLOTS;
+        const int tid = (int)threadIdx.x - NT;
+        const int lr = tid / K, lk = tid % K, lc = lk * V, lvalid = FAST ? V : pl.valid - lc;
+        const bool busy = lr < TT;
+        const int top = first + (tiles - 1) * TT;           /* first row of the tile that comes first */
+        const T* xp = x + pl.b * a.x_batch + (long long)(top + lr) * a.x_row + pl.d0 + lc;
+        const T* dp = dt + pl.b * a.dt_batch + (long long)(top + lr) * a.dt_row + pl.d0 + lc;
+        const T* zp = z ? z + pl.b * a.z_batch + (long long)(top + lr) * a.z_row + pl.d0 + lc : nullptr;
+        const T* gp = dy + pl.b * a.y_batch + (long long)(top + lr) * a.y_row + pl.d0 + lc;
+        const T* bp = Bm + pl.b * a.b_batch + pl.g * a.states + top * a.b_row;
+        const T* cp = Cm + pl.b * a.c_batch + pl.g * a.states + top * a.c_row;
+        A bias[V], skip[V], gD[V], gbias[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            bias[i] = dt_bias && i < lvalid ? dt_bias[pl.d0 + lc + i] : A(0);
+            skip[i] = !AGG && Dv && i < lvalid ? Dv[pl.d0 + lc + i] : A(0);
+            gD[i] = gbias[i] = 0;
         }
-        part[D * a.states + pl.d0 + c] = s0;
-        part[D * (a.states + 1) + pl.d0 + c] = s1;
-    }
+        int t2 = (tiles - 1) * TT, slot2 = 0;       /* of the next fetch: row from `first`, slot of the ring */
+        Pack<T, V> hold_x, hold_dt, hold_z, hold_dy;
+        Pack<T, S> hold_b[UNITS], hold_c[UNITS];
+        int held = -1;
+        auto fetch = [&]() {
+            const bool row = busy && t2 + lr < rows;
+            if constexpr (FAST) {
+                bring(&sh.raw_x[slot2][tid], xp, row);
+                bring(&sh.raw_dt[slot2][tid], dp, row);
+                if (z) bring(&sh.raw_z[slot2][tid], zp, row);
+                bring(&sh.raw_dy[slot2][tid], gp, row);
+            } else {
+                pick(hold_x, xp, row, lvalid);
+                pick(hold_dt, dp, row, lvalid);
+                if (z) pick(hold_z, zp, row, lvalid);
+                pick(hold_dy, gp, row, lvalid);
+                held = slot2;
+            }
+#pragma unroll
+            for (int k = 0; k < UNITS; ++k) {
+                const int e = tid + k * NL, r = e / P, n = (e % P) * S;
+                if (e >= TT * P) break;
+                const bool in = t2 + r < rows && n < a.states;
+                if constexpr (FAST) {
+                    if (!AGG) bring(&sh.raw_b[AGG ? 0 : slot2][AGG ? 0 : e], bp + r * a.b_row + n, in);
+                    bring(&sh.raw_c[slot2][e], cp + r * a.c_row + n, in);
+                } else {
+                    if (!AGG) pick(hold_b[k], bp + r * a.b_row + n, in, a.states - n);
+                    pick(hold_c[k], cp + r * a.c_row + n, in, a.states - n);
+                }
+            }
+            t2 -= TT;
+            slot2 = slot2 + 1 == SLOTS ? 0 : slot2 + 1;
+            xp -= TT * a.x_row; dp -= TT * a.dt_row; gp -= TT * a.y_row; bp -= TT * a.b_row; cp -= TT * a.c_row;
+            if (zp) zp -= TT * a.z_row;
+        };
+        auto settle = [&]() {
+            if (FAST || held < 0) return;
+            sh.raw_x[held][tid] = hold_x;
+            sh.raw_dt[held][tid] = hold_dt;
+            if (z) sh.raw_z[held][tid] = hold_z;
+            sh.raw_dy[held][tid] = hold_dy;
+#pragma unroll
+            for (int k = 0; k < UNITS; ++k) {
+                const int e = tid + k * NL;
+                if (e >= TT * P) break;
+                if (!AGG) sh.raw_b[AGG ? 0 : held][AGG ? 0 : e] = hold_b[k];
+                sh.raw_c[held][e] = hold_c[k];
+            }
+            held = -1;
+        };
+        auto copies = [&](A (*to)[NP], int n, const Pack<T, S>& from) {       /* both orders */
+            Pack<A, S> v, w;
+#pragma unroll
+            for (int i = 0; i < S; ++i) { v.v[i] = up(from.v[i]); w.v[i ^ 2] = v.v[i]; }
+            *reinterpret_cast<Pack<A, S>*>(&to[0][n]) = v;
+            *reinterpret_cast<Pack<A, S>*>(&to[1][n]) = w;
+        };
+        auto stage = [&](int it, int slot) {
+            const int buf = it & 1;
+            if (busy) {
+                const bool row = (tiles - 1 - it) * TT + lr < rows;
+                const Pack<T, V> xr = sh.raw_x[slot][tid], dr = sh.raw_dt[slot][tid], gr = sh.raw_dy[slot][tid];
+                const Pack<T, V> zr = z ? sh.raw_z[slot][tid] : zero_pack<T, V>();
+                A dl[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) dl[i] = up(dr.v[i]) + bias[i];
+                if (a.softplus) softplus_all(dl);
+                Pack<A, 2 * V> o;
+                Pack<A, V> gy;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    if (!row || i >= lvalid) dl[i] = 0;
+                    o.v[2 * i] = dl[i];
+                    o.v[2 * i + 1] = dl[i] * up(xr.v[i]);
+                    A v = up(gr.v[i]);
+                    if (z) { const A zv = up(zr.v[i]); v *= zv * logistic(zv); }
+                    gy.v[i] = row && i < lvalid ? v : A(0);
+                }
+                *reinterpret_cast<Pack<A, 2 * V>*>(&sh.pairs[buf][lr][lc]) = o;
+                *reinterpret_cast<Pack<A, V>*>(&sh.dys[buf][lr][lc]) = gy;
+            }
+#pragma unroll
+            for (int k = 0; k < UNITS; ++k) {
+                const int e = tid + k * NL, r = e / P, n = (e % P) * S;
+                if (e >= TT * P) break;
+                if (!AGG) copies(sh.Bs[buf][AGG ? 0 : r], n, sh.raw_b[AGG ? 0 : slot][AGG ? 0 : e]);
+                copies(sh.Cs[buf][r], n, sh.raw_c[slot][e]);
+            }
+        };
+        const long long all_rows = (long long)a.batch * a.len;
+        const int blk = (pl.d0 - pl.g * a.per_group) / CH;
+        auto finish = [&](int it, int slot) {
+            const int buf = it & 1, t0 = (tiles - 1 - it) * TT;
+            const long long t = first + t0 + lr;
+            if (busy && t < last && lvalid > 0) {
+                T* dxp = out.dx ? out.dx + pl.b * a.dx_batch + t * a.dx_row + pl.d0 + lc : nullptr;
+                T* ddtp = out.ddt ? out.ddt + pl.b * a.ddt_batch + t * a.ddt_row + pl.d0 + lc : nullptr;
+                T* dzp = out.dz ? out.dz + pl.b * a.dz_batch + t * a.dz_row + pl.d0 + lc : nullptr;
+                Pack<T, V> o0 = zero_pack<T, V>(), o1 = o0, o2 = o0;
+                if (dxp && out.acc_dx) o0 = load_pack<T, V>(dxp, lvalid, a.vec_dx);
+                if (ddtp && out.acc_ddt) o1 = load_pack<T, V>(ddtp, lvalid, a.vec_ddt);
+                if (dzp && out.acc_dz) o2 = load_pack<T, V>(dzp, lvalid, a.vec_dz);
+                if (t0 + lr < rows) {
+                    const Pack<T, V> xr = sh.raw_x[slot][tid], dr = sh.raw_dt[slot][tid], gr = sh.raw_dy[slot][tid];
+                    const Pack<T, V> zr = z ? sh.raw_z[slot][tid] : zero_pack<T, V>();
+                    const Pack<A, 2 * V> pr = *reinterpret_cast<const Pack<A, 2 * V>*>(&sh.pairs[buf][lr][lc]);
+                    const Pack<A, V> gy = *reinterpret_cast<const Pack<A, V>*>(&sh.dys[buf][lr][lc]);
+                    const Pack<A, V> q = *reinterpret_cast<const Pack<A, V>*>(&sh.q[buf][AGG ? 0 : lr][lc]);
+                    const Pack<A, V> r = *reinterpret_cast<const Pack<A, V>*>(&sh.r[buf][AGG ? 0 : lr][lc]);
+                    const Pack<A, V> yc = *reinterpret_cast<const Pack<A, V>*>(&sh.yc[buf][AGG ? 0 : lr][lc]);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        if (i >= lvalid) continue;
+                        const A xv = up(xr.v[i]);
+                        A dd = r.v[i] + xv * q.v[i];
+                        if (a.softplus) dd *= logistic(up(dr.v[i]) + bias[i]);
+                        o0.v[i] = down<T>(up(o0.v[i]) + pr.v[2 * i] * q.v[i] + skip[i] * gy.v[i]);
+                        o1.v[i] = down<T>(up(o1.v[i]) + dd);
+                        if (z) {
+                            const A zv = up(zr.v[i]), s = logistic(zv);
+                            o2.v[i] = down<T>(up(o2.v[i]) + up(gr.v[i]) * (yc.v[i] + skip[i] * xv) * s * (A(1) + zv * (A(1) - s)));
+                        }
+                        gD[i] += gy.v[i] * xv;
+                        gbias[i] += dd;
+                    }
+                }
+                if (dxp) store_pack<T, V>(dxp, o0, lvalid, a.vec_dx);
+                if (ddtp) store_pack<T, V>(ddtp, o1, lvalid, a.vec_ddt);
+                if (dzp) store_pack<T, V>(dzp, o2, lvalid, a.vec_dz);
+            }
+            /* the block's part of dB and dC: the warps' sums in turn */
+            for (int e = tid; e < TT * P; e += NL) {
+                const int r = e / P, n = (e % P) * S;
+                if (first + t0 + r >= last || n >= a.states) continue;
+                const long long at = ((blk * all_rows + (long long)pl.b * a.len + first + t0 + r) * a.groups + pl.g) * a.states + n;
+#pragma unroll
+                for (int which = 0; which < 2; ++which) {
+                    A* to = which ? out.part_c : out.part_b;
+                    if (!to) continue;
+                    Pack<A, S> v = *reinterpret_cast<const Pack<A, S>*>(which ? &sh.dC[buf][0][AGG ? 0 : r][n] : &sh.dB[buf][0][AGG ? 0 : r][n]);
+#pragma unroll
+                    for (int w = 1; w < NT / 32; ++w) {
+                        const Pack<A, S> u = *reinterpret_cast<const Pack<A, S>*>(which ? &sh.dC[buf][w][AGG ? 0 : r][n] : &sh.dB[buf][w][AGG ? 0 : r][n]);
+#pragma unroll
+                        for (int i = 0; i < S; ++i) v.v[i] += u.v[i];
+                    }
+                    store_pack<A, S>(to + at, v, a.states - n, out.vec_part);
+                }
+            }
+        };
+        auto next = [](int slot) { return slot + 1 == SLOTS ? 0 : slot + 1; };
+#pragma unroll 1
+        for (int k = 0; k <= DEPTH; ++k) {
+            settle();
+            if (k < tiles) fetch();
+            async_commit();
+        }
+        settle();
+        async_wait<DEPTH>();
+        stage(0, 0);
+        __syncthreads();
+        int done = SLOTS - 1, next_slot = 1 % SLOTS;        /* slots of the tiles before and behind the one walked */
+        for (int it = 0; it < tiles; ++it) {
+            async_wait<DEPTH - 1>();                        /* tile it + 1 is there */
+            settle();
+            if (!AGG && it > 0) finish(it - 1, done);       /* before stage: it reads pairs and dys of the same buffer */
+            if (it + 1 < tiles) stage(it + 1, next_slot);
+            if (it + 1 + DEPTH < tiles) fetch();            /* into the slot of tile it - 1 */
+            async_commit();
+            done = next(done); next_slot = next(next_slot);
+            __syncthreads();
+        }
+        if (AGG) return;
+        finish(tiles - 1, done);
+        if (!out.parts) return;
+        /* the loaders' sums of one channel, a row of loaders after the other (in the memory of the pairs) */
+        A* mine = &sh.pairs[0][0][0].delta;
+        static_assert(sizeof(sh.pairs) >= sizeof(A) * 2 * NL * V, "");
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < V; ++i) { mine[tid * V + i] = gD[i]; mine[NL * V + tid * V + i] = gbias[i]; }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        A* part = out.parts + (pl.b * (long long)a.chunks + pl.c) * D * (a.states + 2) + D * a.states;
+        for (int c = tid; c < CH && c < pl.valid; c += NL) {
+            A s0 = 0, s1 = 0;
+            for (int r = 0; r < TT; ++r) {
+                const int at = (r * K + c / V) * V + c % V;
+                s0 += mine[at]; s1 += mine[NL * V + at];
+            }
+            part[pl.d0 + c] = s0;
+            part[D + pl.d0 + c] = s1;
+        }
+    };
+    if (Sh::PACKS && a.fast && pl.valid >= CH) load(std::integral_constant<bool, Sh::PACKS>());
+    else load(std::false_type());
 }
 
 /* dB and dC (+)= the channel blocks' parts, [parts][rows][cols] -> rows of `cols` with the output's own strides */
@@ -849,7 +1071,7 @@ int lanes_for(int states) {
 /* Rows per chunk.  Splitting a sequence costs a second pass over it (all of its exponentials again), so it pays only where
  * the channels alone leave most of the chip idle. */
 int pick_chunk(const RpbScan* c) {
-    const int p = lanes_for(c->states), ch = NT / p, tt = p <= 4 ? 8 * p : 32;
+    const int ch = NT / lanes_for(c->states), tt = 32;      /* a multiple of every tile */
     const long long per_group = c->channels / c->groups;
     const long long warps = (long long)c->batch * c->groups * ((per_group + ch - 1) / ch) * (NT / 32);
     const int whole = (c->len + tt - 1) / tt * tt;
@@ -985,7 +1207,7 @@ template <typename T, int P>
 int backward_p(const Wanted& w, const void* dy, const void* dh_out, const Operands& o, const void* saved, void* ws, const RpbScan* c,
                cudaStream_t s) {
     typedef typename AccOf<T>::type A;
-    typedef Tile<T, P, NT> Sh;
+    typedef Backward<T, P> Sh;
     Args a = make_args(c);
     const Rowset r = rows_of(c, o.x, o.dt, o.B, o.C, o.z, dy);
     const A *Am = reinterpret_cast<const A*>(o.A), *Dv = reinterpret_cast<const A*>(o.D), *bias = reinterpret_cast<const A*>(o.dt_bias);
@@ -1012,19 +1234,24 @@ int backward_p(const Wanted& w, const void* dy, const void* dh_out, const Operan
     out.part_b = w.dB ? part_b : nullptr; out.part_c = w.dC ? part_c : nullptr;
     out.acc_dx = (w.accumulate & RPB_SCAN_ACC_DX) != 0; out.acc_ddt = (w.accumulate & RPB_SCAN_ACC_DDT) != 0;
     out.acc_dz = (w.accumulate & RPB_SCAN_ACC_DZ) != 0;
-    const size_t smem = sizeof(BackwardShared<T, P>);
-    if (smem > 48 * 1024) {
-        SEQ_CUDA(cudaFuncSetAttribute(backward_kernel<T, P, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        SEQ_CUDA(cudaFuncSetAttribute(backward_kernel<T, P, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    out.vec_part = c->states % S == 0 && reinterpret_cast<uintptr_t>(part_b) % 16 == 0 && reinterpret_cast<uintptr_t>(part_c) % 16 == 0;
+    a.fast = a.vec_x && a.vec_dt && (!z || a.vec_z) && a.vec_y && quads_ok<T>(c, r.B) && quads_ok<T>(c, r.C);
+    const size_t agg = sizeof(BackwardShared<T, P, true>), smem = sizeof(BackwardShared<T, P, false>);
+    SEQ_CUDA(cudaFuncSetAttribute(backward_kernel<T, P, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)agg));
+    SEQ_CUDA(cudaFuncSetAttribute(backward_kernel<T, P, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (Sh::UNEVEN) {
+        cudaFuncAttributes attr;
+        SEQ_CUDA(cudaFuncGetAttributes(&attr, backward_kernel<T, P, false>));
+        if (attr.numRegs != 128) return refuse("rp_selective_scan_grad_ex", "built with another number of registers than its kernel divides");
     }
     const A* dho = reinterpret_cast<const A*>(dh_out);
     const A* sv = reinterpret_cast<const A*>(saved);
     if (a.chunks > 1) {
-        SEQ_CUDA(rpb_launch(backward_kernel<T, P, true>, dim3((unsigned)blocks), dim3(NT), smem, s, 1, out, chunk_g, chunk_s, g, dho, x, dt, Am, B, C, Dv, bias,
+        SEQ_CUDA(rpb_launch(backward_kernel<T, P, true>, dim3((unsigned)blocks), dim3(2 * NT), agg, s, 1, out, chunk_g, chunk_s, g, dho, x, dt, Am, B, C, Dv, bias,
                             z, o.lengths, sv, a));
         rpb_count_launches(1);
     }
-    SEQ_CUDA(rpb_launch(backward_kernel<T, P, false>, dim3((unsigned)blocks), dim3(NT), smem, s, 1, out, chunk_g, chunk_s, g, dho, x, dt, Am, B, C, Dv, bias, z,
+    SEQ_CUDA(rpb_launch(backward_kernel<T, P, false>, dim3((unsigned)blocks), dim3(2 * NT), smem, s, 1, out, chunk_g, chunk_s, g, dho, x, dt, Am, B, C, Dv, bias, z,
                         o.lengths, sv, a));
     rpb_count_launches(1);
     if (w.dB || w.dC) {
