@@ -280,7 +280,7 @@ int rp_selective_scan_grad_ex(void* dx, void* ddt, void* dA, void* dB, void* dC,
                               const void* saved, void* ws, const RpbScan* c, DType dtype, int device_id, void* stream);
 
 /* ---- additive: the norms around a block ----------------------------------------
- * What stands between two blocks of a residual network, one pass over each row of [rows, channels] (up to 16384 channels):
+ * What stands between two blocks of a residual network, one pass over each row of [rows, channels] (up to 8192 channels):
  *   v = u z / (1 + exp(-z))   (z NULL: u)                       the block's output behind its gate
  *   s = v / sqrt(mean v^2 + eps_after) * w_after   (NULL: v)     the norm after the block
  *   out = r + scale * s       (scale NULL: 1, r NULL: 0)         the residual stream, scale per channel

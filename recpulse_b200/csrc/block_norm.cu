@@ -11,14 +11,13 @@ namespace rpb_norm {
 
 using namespace rpb_seq;
 
-constexpr int MAX_CHANNELS = 16384;
+constexpr int MAX_CHANNELS = 8192;
 
 struct Args {
     long long rows;
-    int channels;
+    int channels, classes;      /* rows r, r + classes, ... begin at the same offset from a 16-byte boundary */
     double eps_after, eps_before;
     long long u_row, z_row, r_row, out_row, y_row, du_row, dz_row, dr_row;
-    bool vec;               /* every operand can be moved in whole packs */
 };
 
 template <typename T> struct Width { static constexpr int v = 16 / sizeof(T); };
@@ -26,190 +25,320 @@ template <typename T> struct Width { static constexpr int v = 16 / sizeof(T); };
 __device__ __forceinline__ float rsqrt_of(float v) { return rsqrtf(v); }
 __device__ __forceinline__ double rsqrt_of(double v) { return rsqrt(v); }
 
-/* Sum over the block; every thread gets it.  The two halves of the buffer take turns, so that one barrier per
- * sum is enough: a half is written again only behind the next sum's barrier. */
-template <typename A> __device__ __forceinline__ A block_sum(A v, A (*buffer)[32], int& turn) {
+/* Sums over the block of N values per thread; every thread gets them.  The two halves of the buffer take turns, so that one
+ * barrier is enough: a half is written again only behind the next sum's barrier. */
+template <int N, typename A> __device__ __forceinline__ void block_sums(A (&v)[N], A (*buffer)[N][32], int& turn) {
 #pragma unroll
-    for (int m = 16; m >= 1; m /= 2) v += __shfl_xor_sync(0xffffffffu, v, m);
-    const int warps = blockDim.x >> 5;
-    if (warps == 1) return v;
-    A* slots = buffer[turn];
+    for (int m = 16; m >= 1; m /= 2)
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] += __shfl_xor_sync(0xffffffffu, v[j], m);
+    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+    if (warps == 1) return;
+    A (*slots)[32] = buffer[turn];
     turn ^= 1;
-    if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
-    __syncthreads();
-    A s = (threadIdx.x & 31) < warps ? slots[threadIdx.x & 31] : A(0);
+    if (lane == 0)
 #pragma unroll
-    for (int m = 16; m >= 1; m /= 2) s += __shfl_xor_sync(0xffffffffu, s, m);
-    return s;
+        for (int j = 0; j < N; ++j) slots[j][threadIdx.x >> 5] = v[j];
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = lane < warps ? slots[j][lane] : A(0);
+#pragma unroll
+    for (int m = 16; m >= 1; m /= 2)
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] += __shfl_xor_sync(0xffffffffu, v[j], m);
 }
 
-/* pack k of a thread: channels (k * blockDim + thread) * V .. */
-template <int V> __device__ __forceinline__ int channel_of(int k) { return (k * blockDim.x + threadIdx.x) * V; }
+/* A thread's channels: NV packs of V.  PACKS: pack k lies on a 16-byte boundary of the row, at channel (k threads + thread) V
+ * minus the row's offset from such a boundary (the first and the last pack may stick out of the row); else value i of pack k is
+ * channel (k V + i) threads + thread, so that a warp's single values are neighbours. */
+template <typename T, int NV, bool PACKS> struct Span {
+    static constexpr int V = Width<T>::v;
+    static constexpr unsigned ALL = (1u << V) - 1;
+    int base, step;
+    unsigned mask[NV];          /* which values of a pack are channels of the row */
+    bool ragged;                /* some pack of the row is not whole */
+    __device__ __forceinline__ Span(const T* row, int channels) {
+        const int off = PACKS ? (int)(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T)) : 0;
+        base = PACKS ? (int)threadIdx.x * V - off : (int)threadIdx.x;
+        step = PACKS ? (int)blockDim.x * V : (int)blockDim.x;
+        ragged = off != 0 || channels % V != 0;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            mask[k] = 0;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const int c = channel(k, i);
+                if (c >= 0 && c < channels) mask[k] |= 1u << i;
+            }
+        }
+    }
+    __device__ __forceinline__ int channel(int k, int i) const { return PACKS ? base + k * step + i : base + (k * V + i) * step; }
+    __device__ __forceinline__ bool has(int k, int i) const { return mask[k] >> i & 1; }
+    /* `edge`: nothing outside the row may be read (the first and the last row of an operand); elsewhere a pack that sticks out
+     * reads its neighbours, which tidy() takes out again before use: no load waits for a decision */
+    __device__ __forceinline__ void load(Pack<T, V> (&p)[NV], const T* row, bool given, bool edge) const {
+        const bool packs = PACKS && !(edge && ragged);
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            p[k] = zero_pack<T, V>();
+            if (packs) {
+                if (given && mask[k]) p[k] = *reinterpret_cast<const Pack<T, V>*>(row + channel(k, 0));
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (given && has(k, i)) p[k].v[i] = row[channel(k, i)];
+            }
+        }
+    }
+    __device__ __forceinline__ void tidy(Pack<T, V> (&p)[NV]) const {
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+            if (PACKS && ragged && mask[k] != ALL) {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (!has(k, i)) p[k].v[i] = down<T>(typename AccOf<T>::type(0));
+            }
+    }
+    __device__ __forceinline__ Pack<T, V> load_one(const T* row, int k) const {
+        Pack<T, V> p = zero_pack<T, V>();
+        if (PACKS && mask[k] == ALL) return *reinterpret_cast<const Pack<T, V>*>(row + channel(k, 0));
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (has(k, i)) p.v[i] = row[channel(k, i)];
+        return p;
+    }
+    __device__ __forceinline__ void store(T* row, int k, const Pack<T, V>& p) const {
+        if (PACKS && mask[k] == ALL) { *reinterpret_cast<Pack<T, V>*>(row + channel(k, 0)) = p; return; }
+        if (PACKS && mask[k] == 0) return;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (has(k, i)) row[channel(k, i)] = p.v[i];
+    }
+};
 
-template <typename T, int NV, typename A = typename AccOf<T>::type>
-__device__ __forceinline__ void load_row(Pack<T, Width<T>::v> (&p)[NV], const T* row, const Args& a) {
-    constexpr int V = Width<T>::v;
+/* The weights of a thread's channels stay in shared memory as the thread needs them. */
+template <typename T> __device__ __forceinline__ Pack<T, Width<T>::v>* weight_slots() {
+    extern __shared__ __align__(16) unsigned char raw_shared[];
+    return reinterpret_cast<Pack<T, Width<T>::v>*>(raw_shared);
+}
+template <typename T, int NV, bool PACKS>
+__device__ __forceinline__ void keep_weights(Pack<T, Width<T>::v>* slots, const T* w, const Span<T, NV, PACKS>& span) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        const int c = channel_of<V>(k);
-        p[k] = row ? load_pack<T, V>(row + c, a.channels - c, a.vec) : zero_pack<T, V>();
+        Pack<T, Width<T>::v> p = zero_pack<T, Width<T>::v>();
+#pragma unroll
+        for (int i = 0; i < Width<T>::v; ++i)
+            if (w && span.has(k, i)) p.v[i] = w[span.channel(k, i)];
+        slots[k * blockDim.x + threadIdx.x] = p;
     }
 }
 
-template <typename T, int NV>
-__global__ void __launch_bounds__(512) forward_kernel(T* __restrict__ out, T* __restrict__ y, const T* __restrict__ u, const T* __restrict__ z, const T* __restrict__ w_after,
-                               const T* __restrict__ scale, const T* __restrict__ r, const T* __restrict__ w_before, Args a) {
+/* Block b takes the rows of class b % classes, every (gridDim / classes)-th of them. */
+struct Turn { long long row, step; };
+__device__ __forceinline__ Turn turn_of(const Args& a) {
+    const int per_class = gridDim.x / a.classes;
+    return {(long long)(blockIdx.x / a.classes) * a.classes + blockIdx.x % a.classes, (long long)per_class * a.classes};
+}
+
+template <typename T, int NV, bool PACKS>
+__global__ void __launch_bounds__(512, NV == 1 ? 2 : 1)
+forward_kernel(T* __restrict__ out, T* __restrict__ y, const T* __restrict__ u, const T* __restrict__ z, const T* __restrict__ w_after,
+               const T* __restrict__ scale, const T* __restrict__ r, const T* __restrict__ w_before, Args a) {
     typedef typename AccOf<T>::type A;
     constexpr int V = Width<T>::v;
-    __shared__ A buffer[2][32];
+    __shared__ A buffer[2][1][32];
     int turn = 0;
     rpb_pdl_trigger();
     rpb_pdl_wait();
     const A inv = A(1) / A(a.channels);
-    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        Pack<T, V> up_[NV], zp[NV], rp[NV];
-        load_row<T, NV>(up_, u + row * a.u_row, a);
-        load_row<T, NV>(zp, z ? z + row * a.z_row : nullptr, a);
-        load_row<T, NV>(rp, r ? r + row * a.r_row : nullptr, a);
-        A v[NV][V], sq = 0;
+    const Turn t = turn_of(a);
+    if (t.row >= a.rows) return;
+    const Span<T, NV, PACKS> span(u + t.row * a.u_row, a.channels);
+    const int nt = blockDim.x, tid = threadIdx.x;
+    Pack<T, V>* ws = weight_slots<T>();
+    keep_weights(ws, w_after, span);
+    keep_weights(ws + NV * nt, scale, span);
+    keep_weights(ws + 2 * NV * nt, w_before, span);
+    /* the next row's operands are on their way while a row is worked on, where the registers reach */
+    constexpr bool AHEAD = NV * V <= 8;
+    Pack<T, V> un[NV], zn[NV], rn[NV];
+    auto fetch = [&](long long row) {
+        const bool in = row < a.rows, edge = row == 0 || row == a.rows - 1;
+        span.load(un, u + row * a.u_row, in, edge);
+        span.load(zn, z + row * a.z_row, z && in, edge);
+        span.load(rn, r + row * a.r_row, r && in, edge);
+    };
+    if (AHEAD) fetch(t.row);
+    for (long long row = t.row; row < a.rows; row += t.step) {
+        if (!AHEAD) fetch(row);
+        A v[NV][V], o[NV][V], sq[1] = {0};
+        span.tidy(un); span.tidy(zn); span.tidy(rn);
 #pragma unroll
         for (int k = 0; k < NV; ++k)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                v[k][i] = up(up_[k].v[i]);
-                if (z) { const A g = up(zp[k].v[i]); v[k][i] *= g * logistic(g); }
-                sq += v[k][i] * v[k][i];
+                v[k][i] = up(un[k].v[i]);
+                if (z) { const A g = up(zn[k].v[i]); v[k][i] *= g * logistic(g); }
+                o[k][i] = up(rn[k].v[i]);
+                sq[0] += v[k][i] * v[k][i];
             }
-        const A i1 = w_after ? rsqrt_of(block_sum(sq, buffer, turn) * inv + A(a.eps_after)) : A(1);
-        sq = 0;
+        if (AHEAD) fetch(row + t.step);
+        A i1 = 1;
+        if (w_after) {
+            block_sums(sq, buffer, turn);
+            i1 = rsqrt_of(sq[0] * inv + A(a.eps_after));
+        }
+        sq[0] = 0;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            const int c = channel_of<V>(k), valid = a.channels - c;
-            const Pack<T, V> wp = w_after ? load_pack<T, V>(w_after + c, valid, a.vec) : zero_pack<T, V>();
-            const Pack<T, V> sp = scale ? load_pack<T, V>(scale + c, valid, a.vec) : zero_pack<T, V>();
-            Pack<T, V> o;
+            const Pack<T, V> wp = ws[k * nt + tid], sp = ws[(NV + k) * nt + tid];
+            Pack<T, V> q;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 A s = v[k][i];
                 if (w_after) s = s * i1 * up(wp.v[i]);
                 if (scale) s *= up(sp.v[i]);
-                v[k][i] = i < valid ? up(rp[k].v[i]) + s : A(0);
-                o.v[i] = down<T>(v[k][i]);
-                sq += v[k][i] * v[k][i];
+                o[k][i] += s;
+                q.v[i] = down<T>(o[k][i]);
+                sq[0] += o[k][i] * o[k][i];
             }
-            if (out) store_pack<T, V>(out + row * a.out_row + c, o, valid, a.vec);
+            if (out) span.store(out + row * a.out_row, k, q);
         }
         if (!y) continue;
-        const A i2 = rsqrt_of(block_sum(sq, buffer, turn) * inv + A(a.eps_before));
+        block_sums(sq, buffer, turn);
+        const A i2 = rsqrt_of(sq[0] * inv + A(a.eps_before));
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            const int c = channel_of<V>(k), valid = a.channels - c;
-            const Pack<T, V> wp = load_pack<T, V>(w_before + c, valid, a.vec);
-            Pack<T, V> o;
+            const Pack<T, V> wp = ws[(2 * NV + k) * nt + tid];
+            Pack<T, V> q;
 #pragma unroll
-            for (int i = 0; i < V; ++i) o.v[i] = down<T>(v[k][i] * i2 * up(wp.v[i]));
-            store_pack<T, V>(y + row * a.y_row + c, o, valid, a.vec);
+            for (int i = 0; i < V; ++i) q.v[i] = down<T>(o[k][i] * i2 * up(wp.v[i]));
+            span.store(y + row * a.y_row, k, q);
         }
     }
 }
 
-/* Each block takes every gridDim-th row and keeps its part of the weights' gradients in registers; sum_parts adds the
- * blocks' parts [3][channels]: w_after, scale, w_before. */
-template <typename T, int NV>
-__global__ void __launch_bounds__(512) backward_kernel(T* du, T* dz, T* dr, typename AccOf<T>::type* __restrict__ parts, int acc_du, int acc_dz, int acc_dr,
-                                const T* __restrict__ dout, const T* __restrict__ dy, const T* __restrict__ u, const T* __restrict__ z,
-                                const T* __restrict__ w_after, const T* __restrict__ scale, const T* __restrict__ r, const T* __restrict__ w_before, Args a) {
+/* Each block keeps its part of the weights' gradients in registers; sum_parts adds the blocks' parts [3][channels]: w_after,
+ * scale, w_before. */
+template <typename T, int NV, bool PACKS>
+__global__ void __launch_bounds__(512)
+backward_kernel(T* du, T* dz, T* dr, typename AccOf<T>::type* __restrict__ parts, int acc_du, int acc_dz, int acc_dr, const T* __restrict__ dout,
+                const T* __restrict__ dy, const T* __restrict__ u, const T* __restrict__ z, const T* __restrict__ w_after, const T* __restrict__ scale,
+                const T* __restrict__ r, const T* __restrict__ w_before, Args a) {
     typedef typename AccOf<T>::type A;
     constexpr int V = Width<T>::v;
-    __shared__ A buffer[2][32];
+    __shared__ A buffer[2][2][32];
     int turn = 0;
     rpb_pdl_trigger();
     rpb_pdl_wait();
     const A inv = A(1) / A(a.channels);
+    const Turn t = turn_of(a);
+    const int nt = blockDim.x, tid = threadIdx.x;
+    Pack<T, V>* ws = weight_slots<T>();
+    const Span<T, NV, PACKS> span(u + t.row * a.u_row, a.channels);
+    keep_weights(ws, w_after, span);
+    keep_weights(ws + NV * nt, scale, span);
+    keep_weights(ws + 2 * NV * nt, dy ? w_before : nullptr, span);
     A gwa[NV][V], gsc[NV][V], gwb[NV][V];
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int i = 0; i < V; ++i) gwa[k][i] = gsc[k][i] = gwb[k][i] = 0;
-    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        Pack<T, V> up_[NV], zp[NV], rp[NV], op[NV], yp[NV], wa[NV], sc[NV], wb[NV];
-        load_row<T, NV>(up_, u + row * a.u_row, a);
-        load_row<T, NV>(zp, z ? z + row * a.z_row : nullptr, a);
-        load_row<T, NV>(rp, r ? r + row * a.r_row : nullptr, a);
-        load_row<T, NV>(op, dout ? dout + row * a.out_row : nullptr, a);
-        load_row<T, NV>(yp, dy ? dy + row * a.y_row : nullptr, a);
-        load_row<T, NV>(wa, w_after, a);
-        load_row<T, NV>(sc, scale, a);
-        load_row<T, NV>(wb, dy ? w_before : nullptr, a);
-        A v[NV][V], sq = 0;
+    constexpr bool AHEAD = NV * V <= 8;
+    Pack<T, V> un[NV], zn[NV], rn[NV], on[NV], yn[NV];
+    auto fetch = [&](long long row) {
+        const bool in = row < a.rows, edge = row == 0 || row == a.rows - 1;
+        span.load(un, u + row * a.u_row, in, edge);
+        span.load(zn, z + row * a.z_row, z && in, edge);
+        span.load(rn, r + row * a.r_row, r && in, edge);
+        span.load(on, dout + row * a.out_row, dout && in, edge);
+        span.load(yn, dy + row * a.y_row, dy && in, edge);
+    };
+    if (AHEAD) fetch(t.row);
+    for (long long row = t.row; row < a.rows; row += t.step) {
+        if (!AHEAD) fetch(row);
+        Pack<T, V> up_[NV], zp[NV], rp[NV], op[NV], yp[NV];
+        A v[NV][V], sq[2] = {0, 0};
+        span.tidy(un); span.tidy(zn); span.tidy(rn); span.tidy(on); span.tidy(yn);
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
+        for (int k = 0; k < NV; ++k) {
+            up_[k] = un[k]; zp[k] = zn[k]; rp[k] = rn[k]; op[k] = on[k]; yp[k] = yn[k];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 v[k][i] = up(up_[k].v[i]);
                 if (z) { const A g = up(zp[k].v[i]); v[k][i] *= g * logistic(g); }
-                sq += v[k][i] * v[k][i];
+                sq[0] += v[k][i] * v[k][i];
             }
-        const A i1 = w_after ? rsqrt_of(block_sum(sq, buffer, turn) * inv + A(a.eps_after)) : A(1);
+        }
+        if (AHEAD) fetch(row + t.step);
+        A i1 = 1;
+        if (w_after) {
+            block_sums(sq, buffer, turn);
+            i1 = rsqrt_of(sq[0] * inv + A(a.eps_after));
+        }
         /* the gradient of out */
         A total[NV][V];
         if (dy) {
-            A o[NV][V], dot = 0;
-            sq = 0;
+            sq[0] = sq[1] = 0;
 #pragma unroll
-            for (int k = 0; k < NV; ++k)
+            for (int k = 0; k < NV; ++k) {
+                const Pack<T, V> wa = ws[k * nt + tid], sc = ws[(NV + k) * nt + tid], wb = ws[(2 * NV + k) * nt + tid];
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     A s = v[k][i] * i1;
-                    if (w_after) s *= up(wa[k].v[i]);
-                    if (scale) s *= up(sc[k].v[i]);
-                    o[k][i] = up(rp[k].v[i]) + s;
-                    sq += o[k][i] * o[k][i];
-                    dot += up(yp[k].v[i]) * up(wb[k].v[i]) * o[k][i];
+                    if (w_after) s *= up(wa.v[i]);
+                    if (scale) s *= up(sc.v[i]);
+                    total[k][i] = up(rp[k].v[i]) + s;           /* out itself, for now */
+                    sq[0] += total[k][i] * total[k][i];
+                    sq[1] += up(yp[k].v[i]) * up(wb.v[i]) * total[k][i];
                 }
-            const A i2 = rsqrt_of(block_sum(sq, buffer, turn) * inv + A(a.eps_before));
-            const A pull = block_sum(dot, buffer, turn) * inv * i2 * i2;
+            }
+            block_sums(sq, buffer, turn);
+            const A i2 = rsqrt_of(sq[0] * inv + A(a.eps_before)), pull = sq[1] * inv * i2 * i2;
 #pragma unroll
-            for (int k = 0; k < NV; ++k)
+            for (int k = 0; k < NV; ++k) {
+                const Pack<T, V> wb = ws[(2 * NV + k) * nt + tid];
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    gwb[k][i] += up(yp[k].v[i]) * o[k][i] * i2;
-                    total[k][i] = up(op[k].v[i]) + i2 * (up(yp[k].v[i]) * up(wb[k].v[i]) - o[k][i] * pull);
+                    const A o = total[k][i], g = up(yp[k].v[i]);
+                    gwb[k][i] += g * o * i2;
+                    total[k][i] = up(op[k].v[i]) + i2 * (g * up(wb.v[i]) - o * pull);
                 }
+            }
         } else {
 #pragma unroll
             for (int k = 0; k < NV; ++k)
 #pragma unroll
                 for (int i = 0; i < V; ++i) total[k][i] = up(op[k].v[i]);
         }
-        A dot = 0;
+        sq[0] = sq[1] = 0;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            const int c = channel_of<V>(k), valid = a.channels - c;
             if (dr) {
-                T* to = dr + row * a.dr_row + c;
-                const Pack<T, V> have = acc_dr ? load_pack<T, V>(to, valid, a.vec) : zero_pack<T, V>();
-                Pack<T, V> o;
+                Pack<T, V> q = acc_dr ? span.load_one(dr + row * a.dr_row, k) : zero_pack<T, V>();
 #pragma unroll
-                for (int i = 0; i < V; ++i) o.v[i] = down<T>(total[k][i] + up(have.v[i]));
-                store_pack<T, V>(to, o, valid, a.vec);
+                for (int i = 0; i < V; ++i) q.v[i] = down<T>(total[k][i] + up(q.v[i]));
+                span.store(dr + row * a.dr_row, k, q);
             }
+            const Pack<T, V> wa = ws[k * nt + tid], sc = ws[(NV + k) * nt + tid];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const A t = v[k][i] * i1, w = w_after ? up(wa[k].v[i]) : A(1), s = scale ? up(sc[k].v[i]) : A(1);
-                gwa[k][i] += total[k][i] * s * t;
-                gsc[k][i] += total[k][i] * w * t;
-                total[k][i] *= s * w;               /* now the gradient of t (of v where there is no norm) */
-                dot += total[k][i] * v[k][i];
+                const A m = v[k][i] * i1, w = w_after ? up(wa.v[i]) : A(1), s = scale ? up(sc.v[i]) : A(1);
+                gwa[k][i] += total[k][i] * s * m;
+                gsc[k][i] += total[k][i] * w * m;
+                total[k][i] *= s * w;               /* now the gradient of v i1 (of v where there is no norm) */
+                sq[0] += total[k][i] * v[k][i];
             }
         }
-        const A pull = w_after ? block_sum(dot, buffer, turn) * inv * i1 * i1 : A(0);
+        A pull = 0;
+        if (w_after) {
+            block_sums(sq, buffer, turn);
+            pull = sq[0] * inv * i1 * i1;
+        }
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            const int c = channel_of<V>(k), valid = a.channels - c;
-            T *to_u = du ? du + row * a.du_row + c : nullptr, *to_z = dz ? dz + row * a.dz_row + c : nullptr;
-            Pack<T, V> o = to_u && acc_du ? load_pack<T, V>(to_u, valid, a.vec) : zero_pack<T, V>();
-            Pack<T, V> q = to_z && acc_dz ? load_pack<T, V>(to_z, valid, a.vec) : zero_pack<T, V>();
+            Pack<T, V> o = du && acc_du ? span.load_one(du + row * a.du_row, k) : zero_pack<T, V>();
+            Pack<T, V> q = dz && acc_dz ? span.load_one(dz + row * a.dz_row, k) : zero_pack<T, V>();
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 A dv = i1 * (total[k][i] - v[k][i] * pull);
@@ -220,70 +349,83 @@ __global__ void __launch_bounds__(512) backward_kernel(T* du, T* dz, T* dr, type
                 }
                 o.v[i] = down<T>(up(o.v[i]) + dv);
             }
-            if (to_u) store_pack<T, V>(to_u, o, valid, a.vec);
-            if (to_z) store_pack<T, V>(to_z, q, valid, a.vec);
+            if (du) span.store(du + row * a.du_row, k, o);
+            if (dz) span.store(dz + row * a.dz_row, k, q);
         }
     }
     if (!parts) return;
     A* part = parts + (long long)blockIdx.x * 3 * a.channels;
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const int c = channel_of<V>(k);
+    for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            if (c + i < a.channels) {
-                part[c + i] = gwa[k][i];
-                part[a.channels + c + i] = gsc[k][i];
-                part[2 * a.channels + c + i] = gwb[k][i];
+            if (span.has(k, i)) {
+                const int c = span.channel(k, i);
+                part[c] = gwa[k][i];
+                part[a.channels + c] = gsc[k][i];
+                part[2 * a.channels + c] = gwb[k][i];
             }
-    }
 }
 
-/* packs per thread, and threads: the fewest packs that at most `most` threads cover the row with */
-template <typename T> void shape_of(int channels, int most, int* packs, int* threads) {
-    const int n = (channels + Width<T>::v - 1) / Width<T>::v;
-    int p = 1;
-    while ((n + p - 1) / p > most) p *= 2;
-    *packs = p;
-    *threads = ((n + p - 1) / p + 31) / 32 * 32;
+/* packs per thread, and threads: the fewest packs that at most 512 threads cover the row with; `spare`: rows that begin between
+ * two 16-byte boundaries stick out into one pack more */
+template <typename T> void shape_of(int channels, bool spare, int* packs, int* threads) {
+    constexpr int most[] = {1, 2, sizeof(T) == 2 ? 3 : 4, sizeof(T) == 4 ? 5 : 8, 9};
+    const int n = (channels + Width<T>::v - 1) / Width<T>::v + spare;
+    int i = 0;
+    while ((n + most[i] - 1) / most[i] > 512) ++i;
+    *packs = most[i];
+    *threads = ((n + most[i] - 1) / most[i] + 31) / 32 * 32;
 }
 
-/* Blocks of the backward call: each leaves one part of the weights' gradients behind. */
+/* Blocks of the backward call: each leaves one part of the weights' gradients behind.  A multiple of 8, so that the classes of
+ * rows (8 at most) share them evenly. */
 long long backward_blocks(const RpbBlockNorm* c) {
-    const long long most = SM_COUNT * 4;
-    return c->rows < most ? c->rows : most;
+    const long long most = c->channels > 2048 ? SM_COUNT / 8 * 8 : SM_COUNT * 2;        /* as many as the registers hold at once */
+    const long long rows = (c->rows + 7) / 8 * 8;
+    return rows < most ? rows : most;
+}
+
+struct Operand { const void* p; long long row; };
+
+/* Whether the rows can be moved in packs, and how many rows on they begin at the same offset from a 16-byte boundary: all
+ * operands must have their rows at the same offsets. */
+template <typename T> bool packs_of(const RpbBlockNorm* c, const Operand* o, int n, int* classes) {
+    constexpr int V = Width<T>::v;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(o[0].p) % 16;
+    if (at % sizeof(T)) return false;
+    for (int i = 1; i < n; ++i) {
+        if (!o[i].p) continue;
+        if (reinterpret_cast<uintptr_t>(o[i].p) % 16 != at) return false;
+        if (c->rows > 1 && (o[i].row - o[0].row) % V != 0) return false;
+    }
+    int k = 1;
+    while (c->rows > 1 && o[0].row * k % V != 0) k *= 2;
+    *classes = k;
+    return true;
 }
 
 Args make_args(const RpbBlockNorm* c) {
     Args a;
-    a.rows = c->rows; a.channels = c->channels; a.eps_after = c->eps_after; a.eps_before = c->eps_before;
+    a.rows = c->rows; a.channels = c->channels; a.classes = 1; a.eps_after = c->eps_after; a.eps_before = c->eps_before;
     a.u_row = c->u_row; a.z_row = c->z_row; a.r_row = c->r_row; a.out_row = c->out_row; a.y_row = c->y_row;
     a.du_row = c->du_row; a.dz_row = c->dz_row; a.dr_row = c->dr_row;
-    a.vec = true;
     return a;
-}
-
-/* rows as sequences of one row: a batch of `rows` */
-Rows rows_of(const RpbBlockNorm* c, const void* p, long long row) { return {p, row, c->channels, c->channels}; }
-int batch_of(const RpbBlockNorm* c) { return c->rows > 1 ? 2 : 1; }
-template <typename T> bool whole(const RpbBlockNorm* c, const void* p, long long row) {
-    return !p || aligned_rows(rows_of(c, p, row), batch_of(c), 1, sizeof(T), 16);
 }
 
 struct Operands { const void *u, *z, *w_after, *scale, *r, *w_before; };
 
-template <typename T> bool weights_whole(const RpbBlockNorm* c, const Operands& o) {
-    return whole<T>(c, o.u, c->u_row) && whole<T>(c, o.z, c->z_row) && whole<T>(c, o.r, c->r_row) && whole<T>(c, o.w_after, 0) &&
-           whole<T>(c, o.scale, 0) && whole<T>(c, o.w_before, 0);
-}
-
-template <typename T, int NV>
-int forward_n(void* out, void* y, const Operands& o, const RpbBlockNorm* c, int threads, cudaStream_t s) {
-    Args a = make_args(c);
-    a.vec = weights_whole<T>(c, o) && whole<T>(c, out, c->out_row) && whole<T>(c, y, c->y_row);
-    const long long most = (long long)SM_COUNT * (2048 / threads) * 4;
-    const unsigned blocks = (unsigned)(c->rows < most ? c->rows : most);
-    SEQ_CUDA(rpb_launch(forward_kernel<T, NV>, dim3(blocks), dim3(threads), 0, s, 1, reinterpret_cast<T*>(out), reinterpret_cast<T*>(y),
+template <typename T, int NV, bool PACKS>
+int forward_n(void* out, void* y, const Operands& o, const Args& a, int threads, cudaStream_t s) {
+    const size_t smem = (size_t)3 * NV * threads * 16;
+    if (smem > 40 * 1024)
+        SEQ_CUDA(cudaFuncSetAttribute(forward_kernel<T, NV, PACKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    /* as many blocks as the chip holds at once, at least one row each; a multiple of 8 for the classes */
+    long long most = (long long)SM_COUNT * (NV > 1 ? 1 : 1024 / threads < 16 ? 1024 / threads : 16);
+    most -= most % 8;
+    const long long rows = (a.rows + 7) / 8 * 8;
+    const unsigned blocks = (unsigned)(rows < most ? rows : most);
+    SEQ_CUDA(rpb_launch(forward_kernel<T, NV, PACKS>, dim3(blocks), dim3(threads), smem, s, 1, reinterpret_cast<T*>(out), reinterpret_cast<T*>(y),
                         reinterpret_cast<const T*>(o.u), reinterpret_cast<const T*>(o.z), reinterpret_cast<const T*>(o.w_after),
                         reinterpret_cast<const T*>(o.scale), reinterpret_cast<const T*>(o.r), reinterpret_cast<const T*>(o.w_before), a));
     rpb_count_launches(1);
@@ -292,23 +434,23 @@ int forward_n(void* out, void* y, const Operands& o, const RpbBlockNorm* c, int 
 
 struct Wanted { void *du, *dz, *dr, *dw_after, *dscale, *dw_before; int accumulate; };
 
-template <typename T, int NV>
-int backward_n(const Wanted& w, const void* dout, const void* dy, const Operands& o, void* ws, const RpbBlockNorm* c, int threads, cudaStream_t s) {
+template <typename T, int NV, bool PACKS>
+int backward_n(const Wanted& w, const void* dout, const void* dy, const Operands& o, void* ws, const Args& a, long long blocks, int threads,
+               cudaStream_t s) {
     typedef typename AccOf<T>::type A;
-    Args a = make_args(c);
-    a.vec = weights_whole<T>(c, o) && whole<T>(c, dout, c->out_row) && whole<T>(c, dy, c->y_row) && whole<T>(c, w.du, c->du_row) &&
-            whole<T>(c, w.dz, c->dz_row) && whole<T>(c, w.dr, c->dr_row);
     const bool weights = w.dw_after || w.dscale || w.dw_before;
-    const long long blocks = backward_blocks(c);
-    SEQ_CUDA(rpb_launch(backward_kernel<T, NV>, dim3((unsigned)blocks), dim3(threads), 0, s, 1, reinterpret_cast<T*>(w.du), reinterpret_cast<T*>(w.dz),
-                        reinterpret_cast<T*>(w.dr), weights ? reinterpret_cast<A*>(ws) : nullptr, (w.accumulate & RPB_NORM_ACC_DU) != 0,
-                        (w.accumulate & RPB_NORM_ACC_DZ) != 0, (w.accumulate & RPB_NORM_ACC_DR) != 0, reinterpret_cast<const T*>(dout),
-                        reinterpret_cast<const T*>(dy), reinterpret_cast<const T*>(o.u), reinterpret_cast<const T*>(o.z),
+    const size_t smem = (size_t)3 * NV * threads * 16;
+    if (smem > 40 * 1024)
+        SEQ_CUDA(cudaFuncSetAttribute(backward_kernel<T, NV, PACKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    SEQ_CUDA(rpb_launch(backward_kernel<T, NV, PACKS>, dim3((unsigned)blocks), dim3(threads), smem, s, 1, reinterpret_cast<T*>(w.du),
+                        reinterpret_cast<T*>(w.dz), reinterpret_cast<T*>(w.dr), weights ? reinterpret_cast<A*>(ws) : nullptr,
+                        (w.accumulate & RPB_NORM_ACC_DU) != 0, (w.accumulate & RPB_NORM_ACC_DZ) != 0, (w.accumulate & RPB_NORM_ACC_DR) != 0,
+                        reinterpret_cast<const T*>(dout), reinterpret_cast<const T*>(dy), reinterpret_cast<const T*>(o.u), reinterpret_cast<const T*>(o.z),
                         reinterpret_cast<const T*>(o.w_after), reinterpret_cast<const T*>(o.scale), reinterpret_cast<const T*>(o.r),
                         reinterpret_cast<const T*>(o.w_before), a));
     rpb_count_launches(1);
     if (!weights) return 0;
-    const long long D = c->channels;
+    const long long D = a.channels;
     PartSums d = {};
     d.out[0] = w.dw_after; d.first[0] = 0; d.accumulate[0] = (w.accumulate & RPB_NORM_ACC_DW_AFTER) != 0;
     d.out[1] = w.dscale; d.first[1] = D; d.accumulate[1] = (w.accumulate & RPB_NORM_ACC_DSCALE) != 0;
@@ -317,36 +459,41 @@ int backward_n(const Wanted& w, const void* dout, const void* dy, const Operands
     return sum_parts<T>(d, ws, (int)blocks, 3 * D, s);
 }
 
+template <typename T, typename F> int by_packs(int packs, bool whole, F f) {
+#define CASE(n) if (packs == n) return whole ? f(std::integral_constant<int, n>(), std::true_type()) : f(std::integral_constant<int, n>(), std::false_type());
+    CASE(1) CASE(2)
+    if constexpr (sizeof(T) == 2) { CASE(3) }
+    if constexpr (sizeof(T) == 4) { CASE(4) CASE(5) }
+    if constexpr (sizeof(T) == 8) { CASE(4) CASE(8) CASE(9) }
+#undef CASE
+    return -1;
+}
+
 template <typename T> int run_forward(void* out, void* y, const Operands& o, const RpbBlockNorm* c, cudaStream_t s) {
     int packs, threads;
-    shape_of<T>(c->channels, 512, &packs, &threads);
-    switch (packs) {
-        case 1: return forward_n<T, 1>(out, y, o, c, threads, s);
-        case 2: return forward_n<T, 2>(out, y, o, c, threads, s);
-        case 4: return forward_n<T, 4>(out, y, o, c, threads, s);
-        case 8: return forward_n<T, 8>(out, y, o, c, threads, s);
-        case 16: return forward_n<T, 16>(out, y, o, c, threads, s);
-    }
-    return -1;
+    Args a = make_args(c);
+    const Operand rows[5] = {{o.u, c->u_row}, {o.z, c->z_row}, {o.r, c->r_row}, {out, c->out_row}, {y, c->y_row}};
+    const bool whole = packs_of<T>(c, rows, 5, &a.classes);
+    shape_of<T>(c->channels, whole && (a.classes > 1 || reinterpret_cast<uintptr_t>(o.u) % 16), &packs, &threads);
+    return by_packs<T>(packs, whole, [&](auto n, auto p) { return forward_n<T, decltype(n)::value, decltype(p)::value>(out, y, o, a, threads, s); });
 }
 template <typename T> int run_backward(const Wanted& w, const void* dout, const void* dy, const Operands& o, void* ws, const RpbBlockNorm* c, cudaStream_t s) {
     int packs, threads;
-    shape_of<T>(c->channels, 512, &packs, &threads);
-    switch (packs) {
-        case 1: return backward_n<T, 1>(w, dout, dy, o, ws, c, threads, s);
-        case 2: return backward_n<T, 2>(w, dout, dy, o, ws, c, threads, s);
-        case 4: return backward_n<T, 4>(w, dout, dy, o, ws, c, threads, s);
-        case 8: return backward_n<T, 8>(w, dout, dy, o, ws, c, threads, s);
-        case 16: return backward_n<T, 16>(w, dout, dy, o, ws, c, threads, s);
-    }
-    return -1;
+    Args a = make_args(c);
+    const Operand rows[8] = {{o.u, c->u_row}, {o.z, c->z_row}, {o.r, c->r_row}, {dout, c->out_row}, {dy, c->y_row}, {w.du, c->du_row},
+                             {w.dz, c->dz_row}, {w.dr, c->dr_row}};
+    const bool whole = packs_of<T>(c, rows, 8, &a.classes);
+    shape_of<T>(c->channels, whole && (a.classes > 1 || reinterpret_cast<uintptr_t>(o.u) % 16), &packs, &threads);
+    return by_packs<T>(packs, whole, [&](auto n, auto p) {
+        return backward_n<T, decltype(n)::value, decltype(p)::value>(w, dout, dy, o, ws, a, backward_blocks(c), threads, s);
+    });
 }
 
 const char* bad_geometry(const RpbBlockNorm* c, DType dtype) {
     if (!c) return "no geometry";
     if (!rpb_dtype_size((int)dtype)) return "unknown element type";
     if (c->rows <= 0 || c->channels <= 0) return "rows and channels must be positive";
-    if (c->channels > MAX_CHANNELS) return "rows longer than 16384 channels";
+    if (c->channels > MAX_CHANNELS) return "rows longer than 8192 channels";
     if (!(c->eps_after >= 0) || !(c->eps_before >= 0)) return "eps must not be negative";
     return nullptr;
 }

@@ -94,18 +94,23 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
     return r;
 }
 
-__device__ __forceinline__ float exp_of(float v) { return __expf(v); }
-__device__ __forceinline__ double exp_of(double v) { return exp(v); }
+/* exp(v) through the hardware's base-2 exponential, results below the normal range as 0: within (2 + |v|) steps */
+__device__ __forceinline__ float exp_of(float v) { return ex2_fast(v * 1.44269504088896341f); }
+__device__ __forceinline__ float reciprocal(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
 
-/* 1 / (1 + exp(-v)); the quotient of a finite numerator by +inf is 0, so both ends are exact */
-__device__ __forceinline__ float logistic(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
+/* 1 / (1 + exp(-v)); the reciprocal of +inf is 0, so both ends are exact */
+__device__ __forceinline__ float logistic(float v) { return reciprocal(1.0f + exp_of(-v)); }
 __device__ __forceinline__ double logistic(double v) { return 1.0 / (1.0 + exp(-v)); }
 
 /* log(1 + exp(v)) = max(v, 0) + log(1 + e) with e = exp(-|v|) in (0, 1]; log(1 + e) / e as a polynomial of degree 9
  * (Chebyshev interpolation on [0, 1]), within 2.2 half-steps of float32 as computed here: a third of log1pf's instructions,
  * and no cancellation for small e */
 __device__ __forceinline__ float softplus_of(float v) {
-    const float e = __expf(-fabsf(v));
+    const float e = exp_of(-fabsf(v));
     float p = -0.0031760570127516985f;
     p = fmaf(p, e, 0.019542528316378593f);
     p = fmaf(p, e, -0.05637361481785774f);
@@ -129,7 +134,7 @@ template <int V> __device__ __forceinline__ void softplus_all(float (&v)[V]) {
     if (V % 2) v[V - 1] = softplus_of(v[V - 1]);
 #pragma unroll
     for (int i = 0; i < V / 2 * 2; i += 2) {
-        const f32x2 e = pack2(__expf(-fabsf(v[i])), __expf(-fabsf(v[i + 1])));
+        const f32x2 e = pack2(exp_of(-fabsf(v[i])), exp_of(-fabsf(v[i + 1])));
         const float c[9] = {0.019542528316378593f, -0.05637361481785774f, 0.10543623566627502f, -0.1526966691017151f, 0.1966327428817749f,
                             -0.24951615929603577f, 0.33329710364341736f, -0.49999892711639404f, 1.0f};
         f32x2 p = pack2(-0.0031760570127516985f, -0.0031760570127516985f);

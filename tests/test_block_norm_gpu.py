@@ -151,7 +151,7 @@ def check(lib, s, dtype, what):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
-@pytest.mark.parametrize("rows,d", [(1, 1), (3, 7), (2, 8), (5, 64), (33, 200), (2, 1000), (7, 1531), (3, 4096), (2, 8192), (1, 16384), (700, 40)])
+@pytest.mark.parametrize("rows,d", [(1, 1), (3, 7), (2, 8), (5, 64), (33, 200), (2, 1000), (7, 1531), (3, 4096), (2, 8192), (9, 8191), (5, 4095), (700, 40), (40, 2999), (1300, 257)])
 def test_forward_and_backward(lib, dtype, rows, d):
     check(lib, make(rows, d, dtype, rows * d), dtype, f"{dtype} {rows}x{d}")
 

@@ -125,7 +125,7 @@ def norm(rows=4, channels=8, eps=1e-5, **over):
     return c
 
 
-@pytest.mark.parametrize("wrong", [dict(rows=0), dict(channels=0), dict(channels=16385), dict(eps=-1.0), dict(eps=float("nan")), dict(out_row=7),
+@pytest.mark.parametrize("wrong", [dict(rows=0), dict(channels=0), dict(channels=8193), dict(eps=-1.0), dict(eps=float("nan")), dict(out_row=7),
                                    dict(y_row=-8), dict(u_row=-1), dict(r_row=-1)])
 def test_norm_refuses_bad_geometry(wrong):
     lib, c = rpb.load(), norm(**wrong)
