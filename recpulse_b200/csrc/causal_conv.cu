@@ -10,14 +10,14 @@ namespace rpb_conv1d {
 using namespace rpb_seq;
 
 struct Args {
-    int batch, len, channels, silu;
+    int batch, len, channels, silu, width;
     long long x_batch, x_row, y_batch, y_row, dx_batch, dx_row;
     int run, runs;          /* rows per thread, and such runs per sequence */
-    int n_vec;              /* packs of channels */
-    bool vec_x, vec_y, vec_dx, vec_p;       /* whole packs may be moved: x, y (dy), dx, packed operands (state, bias) */
+    int vec_blocks;         /* warps that cover the channels */
 };
 
-template <typename T> struct Width { static constexpr int fwd = 16 / sizeof(T), bwd = sizeof(T) == 2 ? 4 : 16 / sizeof(T); };
+/* Channels of a thread: 8 bytes of a 16-bit row (16 bytes needed twice the registers and ran at half the warps), 16 of others. */
+template <typename T> struct Width { static constexpr int v = sizeof(T) == 2 ? 4 : 16 / sizeof(T); };
 
 __device__ __forceinline__ int row_end(const int* lengths, int b, int len) {
     if (!lengths) return len;
@@ -32,90 +32,143 @@ template <typename A> __device__ __forceinline__ A act_slope(A pre, int silu) {
     return s * (A(1) + pre * (A(1) - s));
 }
 
-/* w[V][W] and bias[V] of the channels from d0 on, 0 behind the last one */
-template <typename T, int W, int V, typename A>
-__device__ __forceinline__ void load_taps(A (&w)[V][W], A (&bias)[V], const T* wt, const T* bt, int d0, int channels) {
+/* A thread's V channels.  VEC: neighbours, moved as one pack (every row aligned, V divides the channels); else every 32nd one, so
+ * that a warp's single values are neighbours. */
+template <typename T, bool VEC> struct Lane {
+    static constexpr int V = Width<T>::v;
+    int d0, channels;
+    __device__ __forceinline__ int channel(int i) const { return VEC ? d0 + i : d0 + 32 * i; }
+    __device__ __forceinline__ bool has(int i) const { return VEC ? d0 < channels : channel(i) < channels; }
+    /* `row`: the row's first channel */
+    __device__ __forceinline__ Pack<T, V> load(const T* row, bool on) const {
+        Pack<T, V> p = zero_pack<T, V>();
+        if (VEC) {
+            if (on && has(0)) p = *reinterpret_cast<const Pack<T, V>*>(row + d0);
+        } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const bool on = d0 + i < channels;
+            for (int i = 0; i < V; ++i)
+                if (on && has(i)) p.v[i] = row[channel(i)];
+        }
+        return p;
+    }
+    __device__ __forceinline__ void store(T* row, const Pack<T, V>& p) const {
+        if (VEC) {
+            if (has(0)) *reinterpret_cast<Pack<T, V>*>(row + d0) = p;
+        } else {
 #pragma unroll
-        for (int j = 0; j < W; ++j) w[i][j] = on ? up(wt[(long long)(d0 + i) * W + j]) : A(0);
-        bias[i] = on && bt ? up(bt[d0 + i]) : A(0);
+            for (int i = 0; i < V; ++i)
+                if (has(i)) row[channel(i)] = p.v[i];
+        }
+    }
+};
+
+/* Where a thread works: one warp per run of rows, four runs per block. */
+template <typename T, bool VEC> struct Place {
+    Lane<T, VEC> lane;
+    long long group, seq;
+    int b, t0, t1;
+    bool on;
+    __device__ __forceinline__ explicit Place(const Args& a) {
+        const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5, first = (int)(blockIdx.x % a.vec_blocks) * 32 * Width<T>::v;
+        lane.channels = a.channels;
+        lane.d0 = VEC ? first + tx * Width<T>::v : first + tx;
+        group = blockIdx.x / a.vec_blocks;
+        seq = group * (blockDim.x >> 5) + ty;
+        on = seq < (long long)a.batch * a.runs;
+        b = on ? (int)(seq / a.runs) : 0;
+        t0 = on ? (int)(seq - (long long)b * a.runs) * a.run : 0;
+        t1 = t0 + a.run < a.len ? t0 + a.run : a.len;
+    }
+};
+
+/* The filter of up to W taps, behind W - width zeros that no product is formed with (`skip`), and the bias. */
+template <typename T, int W, bool VEC, typename A>
+__device__ __forceinline__ void load_taps(A (&w)[W][Width<T>::v], A (&bias)[Width<T>::v], const T* wt, const T* bt, const Lane<T, VEC>& lane, int width) {
+#pragma unroll
+    for (int i = 0; i < Width<T>::v; ++i) {
+        const bool on = lane.has(i);
+        const long long c = lane.channel(i);
+#pragma unroll
+        for (int j = 0; j < W; ++j) w[j][i] = on && j >= W - width ? up(wt[c * width + j - (W - width)]) : A(0);
+        bias[i] = on && bt ? up(bt[c]) : A(0);
     }
 }
 
-/* Row p of xp before row 0 of x: row p + W - 1 of the sequence's state, zeros without one. */
-template <typename T, int W, int V>
-__device__ __forceinline__ Pack<T, V> state_row(const T* state, int b, int p, int d0, const Args& a) {
-    if (!state) return zero_pack<T, V>();
-    return load_pack<T, V>(state + ((long long)b * (W - 1) + p + W - 1) * a.channels + d0, a.channels - d0, a.vec_p);
+/* Row p of xp: of x within the sequence, in front of it of the sequence's state (row p + width - 1), else zeros. */
+template <typename T, bool VEC>
+__device__ __forceinline__ Pack<T, Width<T>::v> row_of(const T* x, const T* state, int p, int end, const Lane<T, VEC>& lane, const Args& a) {
+    const int s = p + a.width - 1;
+    if (p >= 0) return lane.load(x + p * a.x_row, p < end);
+    return lane.load(state + (long long)s * a.channels, state && s >= 0);
 }
 
-/* One thread: V channels (16 bytes) of `run` consecutive rows, the last W - 1 rows in registers, so that x is read
- * once but for W - 1 rows in front of each run. */
-template <typename T, int W>
+constexpr int U = 4;        /* rows at a time, the next ones' values on their way meanwhile */
+
+/* The last W - 1 rows of x are kept in registers, so that x is read once but for W - 1 rows in front of each run. */
+template <typename T, int W, bool VEC>
 __global__ void __launch_bounds__(128) forward_kernel(T* __restrict__ y, T* state_out, const T* __restrict__ x, const T* __restrict__ wt,
                                                       const T* __restrict__ bt, const T* state_in, const int* __restrict__ lengths, Args a) {
     typedef typename AccOf<T>::type A;
-    constexpr int V = Width<T>::fwd, H = W - 1, U = 4;
+    constexpr int V = Width<T>::v, H = W - 1;
     rpb_pdl_trigger();
     rpb_pdl_wait();
-    const long long item = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    const long long seq = item / a.n_vec;
-    if (seq >= (long long)a.batch * a.runs) return;
-    const int d0 = (int)(item - seq * a.n_vec) * V, valid = a.channels - d0;
-    const int b = (int)(seq / a.runs), t0 = (int)(seq - (long long)b * a.runs) * a.run;
-    const int t1 = t0 + a.run < a.len ? t0 + a.run : a.len, end = row_end(lengths, b, a.len);
-    const T* xs = x + b * a.x_batch + d0;
-    T* ys = y + b * a.y_batch + d0;
-
-    A w[V][W], bias[V], win[W][V];          /* win[j]: row t - H + j */
-    load_taps<T, W, V>(w, bias, wt, bt, d0, a.channels);
+    const Place<T, VEC> pl(a);
+    if (!pl.on) return;
+    const Lane<T, VEC>& lane = pl.lane;
+    const int end = row_end(lengths, pl.b, a.len), skip = W - a.width, keep = a.width - 1;
+    const T* xs = x + pl.b * a.x_batch;
+    T* ys = y + pl.b * a.y_batch;
+    const T* first = state_in ? state_in + (long long)pl.b * keep * a.channels : nullptr;
+    int t = pl.t0;
+    if (t < end) {
+        A w[W][V], bias[V], win[H + U][V];          /* win[j]: row t - H + j */
+        load_taps<T, W, VEC>(w, bias, wt, bt, lane, a.width);
+        Pack<T, V> next[U], early[H];
 #pragma unroll
-    for (int j = 0; j < H; ++j) {
-        const int p = t0 - H + j;
-        const Pack<T, V> r = p < 0 ? state_row<T, W, V>(state_in, b, p, d0, a)
-                                   : p < end ? load_pack<T, V>(xs + p * a.x_row, valid, a.vec_x) : zero_pack<T, V>();
+        for (int j = 0; j < H; ++j) early[j] = j >= skip ? row_of(xs, first, t - H + j, end, lane, a) : zero_pack<T, V>();
 #pragma unroll
-        for (int i = 0; i < V; ++i) win[j][i] = up(r.v[i]);
-    }
-    if (state_out && t0 == 0) {
-        /* the last W - 1 rows of xp; all read before the first is written: state_out may be state_in */
-        Pack<T, V> last[H > 0 ? H : 1];
+        for (int k = 0; k < U; ++k) next[k] = lane.load(xs + (t + k) * a.x_row, t + k < pl.t1 && t + k < end);
 #pragma unroll
-        for (int j = 0; j < H; ++j) {
-            const int p = end - H + j;
-            last[j] = p < 0 ? state_row<T, W, V>(state_in, b, p, d0, a) : load_pack<T, V>(xs + p * a.x_row, valid, a.vec_x);
-        }
+        for (int j = 0; j < H; ++j)
 #pragma unroll
-        for (int j = 0; j < H; ++j) store_pack<T, V>(state_out + ((long long)b * H + j) * a.channels + d0, last[j], valid, a.vec_p);
-    }
-    for (int t = t0; t < t1; t += U) {
-        Pack<T, V> rows[U];
+            for (int i = 0; i < V; ++i) win[j][i] = up(early[j].v[i]);
+        for (; t < pl.t1 && t < end; t += U) {
 #pragma unroll
-        for (int k = 0; k < U; ++k)
-            rows[k] = t + k < t1 && t + k < end ? load_pack<T, V>(xs + (t + k) * a.x_row, valid, a.vec_x) : zero_pack<T, V>();
+            for (int k = 0; k < U; ++k)
 #pragma unroll
-        for (int k = 0; k < U; ++k) {
-            if (t + k >= t1) break;
-            Pack<T, V> o = zero_pack<T, V>();
+                for (int i = 0; i < V; ++i) win[H + k][i] = up(next[k].v[i]);
 #pragma unroll
-            for (int i = 0; i < V; ++i) win[H][i] = up(rows[k].v[i]);
-            if (t + k < end) {
+            for (int k = 0; k < U; ++k) next[k] = lane.load(xs + (t + U + k) * a.x_row, t + U + k < pl.t1 && t + U + k < end);
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                if (t + k >= pl.t1) break;
+                Pack<T, V> o;
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     A pre = bias[i];
 #pragma unroll
-                    for (int j = 0; j < W; ++j) pre += w[i][j] * win[j][i];
-                    o.v[i] = down<T>(act(pre, a.silu));
+                    for (int j = 0; j < W; ++j)
+                        if (j >= skip) pre += w[j][i] * win[k + j][i];
+                    o.v[i] = down<T>(t + k < end ? act(pre, a.silu) : A(0));
                 }
+                lane.store(ys + (t + k) * a.y_row, o);
             }
-            store_pack<T, V>(ys + (t + k) * a.y_row, o, valid, a.vec_y);
 #pragma unroll
             for (int j = 0; j < H; ++j)
 #pragma unroll
-                for (int i = 0; i < V; ++i) win[j][i] = win[j + 1][i];
+                for (int i = 0; i < V; ++i) win[j][i] = win[j + U][i];
         }
+    }
+    for (; t < pl.t1; ++t) lane.store(ys + t * a.y_row, zero_pack<T, V>());
+    if (state_out && pl.t0 == 0) {
+        /* the last rows of xp, by the only run that reads the old state; all read before the first is written: state_out may be
+         * state_in */
+        Pack<T, V> last[H];
+#pragma unroll
+        for (int j = 0; j < H; ++j) last[j] = j < keep ? row_of(xs, first, end - keep + j, end, lane, a) : zero_pack<T, V>();
+#pragma unroll
+        for (int j = 0; j < H; ++j)
+            if (j < keep) lane.store(state_out + ((long long)pl.b * keep + j) * a.channels, last[j]);
     }
 }
 
@@ -124,114 +177,139 @@ __global__ void __launch_bounds__(128) forward_kernel(T* __restrict__ y, T* stat
  * A thread walks its rows upwards and W - 1 rows further, computes dpre of each row again from x and emits the gradient
  * of the row W - 1 behind; the run that begins a sequence emits the state's gradient in the same way.  The filter's
  * gradients of a block's four runs are added in shared memory and written as one part; sum_parts adds the parts. */
-template <typename T, int W>
+template <typename T, int W, bool VEC>
 __global__ void __launch_bounds__(128) backward_kernel(T* dx, T* dstate_in, typename AccOf<T>::type* __restrict__ parts, int acc_dx,
                                                        const T* __restrict__ dy, const T* __restrict__ dstate_out, const T* __restrict__ x,
                                                        const T* __restrict__ wt, const T* __restrict__ bt, const T* __restrict__ state_in,
-                                                       const int* __restrict__ lengths, Args a, int vec_blocks) {
+                                                       const int* __restrict__ lengths, Args a) {
     typedef typename AccOf<T>::type A;
-    constexpr int V = Width<T>::bwd, H = W - 1;
+    constexpr int V = Width<T>::v, H = W - 1;
     __shared__ A red[4][W + 1][32 * V + 1];
     rpb_pdl_trigger();
     rpb_pdl_wait();
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const long long group = blockIdx.x / vec_blocks;
-    const int d0 = ((int)(blockIdx.x - group * vec_blocks) * 32 + tx) * V, valid = a.channels - d0;
-    const long long seq = group * 4 + ty;
-    A dw[V][W], db[V];
+    const Place<T, VEC> pl(a);
+    const Lane<T, VEC>& lane = pl.lane;
+    const int skip = W - a.width, keep = a.width - 1;
+    A dw[W][V], db[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         db[i] = 0;
 #pragma unroll
-        for (int j = 0; j < W; ++j) dw[i][j] = 0;
+        for (int j = 0; j < W; ++j) dw[j][i] = 0;
     }
-    if (valid > 0 && seq < (long long)a.batch * a.runs) {
-        const int b = (int)(seq / a.runs), t0 = (int)(seq - (long long)b * a.runs) * a.run;
-        const int t1 = t0 + a.run < a.len ? t0 + a.run : a.len, end = row_end(lengths, b, a.len);
-        const T* xs = x + b * a.x_batch + d0;
-        const T* gs = dy + b * a.y_batch + d0;
-        T* ds = dx ? dx + b * a.dx_batch + d0 : nullptr;
-        A w[V][W], bias[V], win[W][V], dp[W][V];        /* dp[j]: dpre of row s - H + j */
-        load_taps<T, W, V>(w, bias, wt, bt, d0, a.channels);
+    if (pl.on) {
+        const int end = row_end(lengths, pl.b, a.len);
+        const T* xs = x + pl.b * a.x_batch;
+        const T* gs = dy + pl.b * a.y_batch;
+        T* ds = dx ? dx + pl.b * a.dx_batch : nullptr;
+        const T* first = state_in ? state_in + (long long)pl.b * keep * a.channels : nullptr;
+        const T* more_from = dstate_out ? dstate_out + (long long)pl.b * keep * a.channels : nullptr;
+        T* to_state = dstate_in ? dstate_in + (long long)pl.b * keep * a.channels : nullptr;
+        A w[W][V], bias[V], win[H + U][V], dp[H + U][V];        /* row t - H + j; dp: of dpre */
+        load_taps<T, W, VEC>(w, bias, wt, bt, lane, a.width);
+        Pack<T, V> xn[U], gn[U], early[H];
+        int t = pl.t0;
+        const int stop = pl.t1 + H;
+        auto fetch = [&](int s) {
 #pragma unroll
-        for (int j = 0; j < H; ++j) {
-            const int p = t0 - H + j;
-            const Pack<T, V> r = p < 0 ? state_row<T, W, V>(state_in, b, p, d0, a)
-                                       : p < end ? load_pack<T, V>(xs + p * a.x_row, valid, a.vec_x) : zero_pack<T, V>();
-#pragma unroll
-            for (int i = 0; i < V; ++i) { win[j][i] = up(r.v[i]); dp[j][i] = 0; }
-        }
-        const int last = t1 + H;
-        for (int s = t0; s < last; s += 4) {
-            Pack<T, V> xr[4], gr[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const bool on = s + k < last && s + k < end;
-                xr[k] = on ? load_pack<T, V>(xs + (s + k) * a.x_row, valid, a.vec_x) : zero_pack<T, V>();
-                gr[k] = on ? load_pack<T, V>(gs + (s + k) * a.y_row, valid, a.vec_y) : zero_pack<T, V>();
+            for (int k = 0; k < U; ++k) {
+                const bool on = s + k < stop && s + k < end;
+                xn[k] = lane.load(xs + (s + k) * a.x_row, on);
+                gn[k] = lane.load(gs + (s + k) * a.y_row, on);
             }
+        };
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if (s + k >= last) break;
-                const bool on = s + k < end;
+        for (int j = 0; j < H; ++j) early[j] = j >= skip ? row_of(xs, first, t - H + j, end, lane, a) : zero_pack<T, V>();
+        fetch(t);
+#pragma unroll
+        for (int j = 0; j < H; ++j)
+#pragma unroll
+            for (int i = 0; i < V; ++i) { win[j][i] = up(early[j].v[i]); dp[j][i] = 0; }
+        for (; t < stop; t += U) {
+            Pack<T, V> g[U];
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                g[k] = gn[k];
+#pragma unroll
+                for (int i = 0; i < V; ++i) win[H + k][i] = up(xn[k].v[i]);
+            }
+            fetch(t + U);
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                const int s = t + k;
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    win[H][i] = up(xr[k].v[i]);
                     A pre = bias[i];
 #pragma unroll
-                    for (int j = 0; j < W; ++j) pre += w[i][j] * win[j][i];
-                    dp[H][i] = on ? up(gr[k].v[i]) * act_slope(pre, a.silu) : A(0);
-                    if (s + k < t1) {
-                        db[i] += dp[H][i];
+                    for (int j = 0; j < W; ++j)
+                        if (j >= skip) pre += w[j][i] * win[k + j][i];
+                    const A d = s < stop && s < end ? up(g[k].v[i]) * act_slope(pre, a.silu) : A(0);
+                    dp[H + k][i] = d;
+                    const A own = s < pl.t1 ? d : A(0);
+                    db[i] += own;
+                    if (s < end) {
 #pragma unroll
-                        for (int j = 0; j < W; ++j) dw[i][j] += dp[H][i] * win[j][i];
+                        for (int j = 0; j < W; ++j)
+                            if (j >= skip) dw[j][i] += own * win[k + j][i];
                     }
                 }
-                const int t = s + k - H;            /* the row whose gradient is complete now */
+                const int r = s - H;                /* the row whose gradient is complete now */
                 T* to = nullptr;
-                if (t >= t0) { if (ds) to = ds + t * a.dx_row; }
-                else if (t0 == 0 && dstate_in) to = dstate_in + ((long long)b * H + t + H) * a.channels + d0;
-                if (to) {
-                    const bool whole = t >= 0 ? a.vec_dx : a.vec_p, add = t >= 0 && acc_dx;
-                    const int from_end = t - (end - H);             /* row of the final state that is this row of xp */
-                    Pack<T, V> more = zero_pack<T, V>(), have = zero_pack<T, V>(), o;
-                    if (dstate_out && from_end >= 0 && from_end < H)
-                        more = load_pack<T, V>(dstate_out + ((long long)b * H + from_end) * a.channels + d0, valid, a.vec_p);
-                    if (add) have = load_pack<T, V>(to, valid, whole);
+                if (r >= pl.t1) break;
+                if (r >= pl.t0) { if (ds) to = ds + r * a.dx_row; }
+                else if (pl.t0 == 0 && to_state && r >= -keep) to = to_state + (long long)(r + keep) * a.channels;
+                if (!to) continue;
+                const int from_end = r - (end - keep);              /* row of the final state that is this row of xp */
+                Pack<T, V> o;
+                A v[V];
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        A g = up(more.v[i]);
+                for (int i = 0; i < V; ++i) {
+                    v[i] = 0;
 #pragma unroll
-                        for (int j = 0; j < W; ++j) g += w[i][j] * dp[H - j][i];
-                        o.v[i] = down<T>(g + up(have.v[i]));
-                    }
-                    store_pack<T, V>(to, o, valid, whole);
+                    for (int j = 0; j < W; ++j)
+                        if (j >= skip) v[i] += w[j][i] * dp[H + k - j][i];
+                }
+                if (more_from && from_end >= 0 && from_end < keep) {
+                    const Pack<T, V> more = lane.load(more_from + (long long)from_end * a.channels, true);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) v[i] += up(more.v[i]);
+                }
+                if (r >= 0 && acc_dx) {
+                    const Pack<T, V> have = lane.load(to, true);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) v[i] += up(have.v[i]);
                 }
 #pragma unroll
-                for (int j = 0; j < H; ++j)
-#pragma unroll
-                    for (int i = 0; i < V; ++i) { win[j][i] = win[j + 1][i]; dp[j][i] = dp[j + 1][i]; }
+                for (int i = 0; i < V; ++i) o.v[i] = down<T>(v[i]);
+                lane.store(to, o);
             }
+#pragma unroll
+            for (int j = 0; j < H; ++j)
+#pragma unroll
+                for (int i = 0; i < V; ++i) { win[j][i] = win[j + U][i]; dp[j][i] = dp[j + U][i]; }
         }
     }
     if (!parts) return;
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        red[ty][W][tx * V + i] = db[i];
+        const int c = VEC ? tx * V + i : tx + 32 * i;
+        red[ty][W][c] = db[i];
 #pragma unroll
-        for (int j = 0; j < W; ++j) red[ty][j][tx * V + i] = dw[i][j];
+        for (int j = 0; j < W; ++j) red[ty][j][c] = dw[j][i];
     }
     __syncthreads();
-    /* part: [channels][W] filter gradients, then [channels] bias gradients */
-    A* part = parts + group * (long long)a.channels * (W + 1);
-    const int base = d0 - tx * V;
-    for (int e = threadIdx.x; e < 32 * V * (W + 1); e += 128) {
+    /* part: [channels][width] filter gradients, then [channels] bias gradients */
+    A* part = parts + pl.group * (long long)a.channels * (a.width + 1);
+    const int base = (int)(blockIdx.x % a.vec_blocks) * 32 * V;
+    for (int e = threadIdx.x; e < 32 * V * (a.width + 1); e += 128) {
         int c, j;
-        if (e < 32 * V * W) { c = e / W; j = e - c * W; } else { c = e - 32 * V * W; j = W; }
+        if (e < 32 * V * a.width) { c = e / a.width; j = e - c * a.width; } else { c = e - 32 * V * a.width; j = a.width; }
         if (base + c >= a.channels) continue;
-        const A v = ((red[0][j][c] + red[1][j][c]) + red[2][j][c]) + red[3][j][c];
-        if (j < W) part[(long long)(base + c) * W + j] = v;
-        else part[(long long)a.channels * W + base + c] = v;
+        const int from = j < a.width ? j + skip : W;
+        const A v = ((red[0][from][c] + red[1][from][c]) + red[2][from][c]) + red[3][from][c];
+        if (j < a.width) part[(long long)(base + c) * a.width + j] = v;
+        else part[(long long)a.channels * a.width + base + c] = v;
     }
 }
 
@@ -245,8 +323,7 @@ int pick_run(long long batch, int len, long long n_vec, int longest, int warps) 
 }
 
 template <typename T> int backward_run(const RpbCausalConv* c) {
-    const long long n_vec = (c->channels + Width<T>::bwd - 1) / Width<T>::bwd;
-    return pick_run(c->batch, c->len, n_vec, 64, SM_COUNT * 16);
+    return pick_run(c->batch, c->len, (c->channels + Width<T>::v - 1) / Width<T>::v, 64, SM_COUNT * 16);
 }
 template <typename T> long long backward_groups(const RpbCausalConv* c) {
     const int run = backward_run<T>(c);
@@ -256,79 +333,87 @@ template <typename T> long long backward_groups(const RpbCausalConv* c) {
 Rows x_rows(const RpbCausalConv* c, const void* x) { return {x, c->x_batch, c->x_row, c->channels}; }
 Rows y_rows(const RpbCausalConv* c, const void* y) { return {y, c->y_batch, c->y_row, c->channels}; }
 Rows dx_rows(const RpbCausalConv* c, const void* dx) { return {dx, c->dx_batch, c->dx_row, c->channels}; }
-bool packed_ok(const RpbCausalConv* c, const void* p, size_t bytes, size_t es) { return aligned_rows({p, 0, c->channels, c->channels}, 2, 2, es, bytes); }
 
-Args make_args(const RpbCausalConv* c, int v, size_t es, int run) {
+/* Whether every row of an operand (a packed state: p, 0 strides) can be moved in packs. */
+template <typename T> bool packs_ok(const RpbCausalConv* c, const Rows& r) {
+    return !r.p || aligned_rows(r, c->batch, c->len, sizeof(T), sizeof(T) * Width<T>::v);
+}
+template <typename T> bool state_ok(const RpbCausalConv* c, const void* p) {
+    return !p || reinterpret_cast<uintptr_t>(p) % (sizeof(T) * Width<T>::v) == 0;
+}
+
+template <typename T> Args make_args(const RpbCausalConv* c, int run) {
     Args a;
-    a.batch = c->batch; a.len = c->len; a.channels = c->channels; a.silu = c->activation;
+    a.batch = c->batch; a.len = c->len; a.channels = c->channels; a.silu = c->activation; a.width = c->width;
     a.x_batch = c->x_batch; a.x_row = c->x_row; a.y_batch = c->y_batch; a.y_row = c->y_row;
     a.dx_batch = c->dx_batch; a.dx_row = c->dx_row;
     a.run = run; a.runs = (c->len + run - 1) / run;
-    a.n_vec = (c->channels + v - 1) / v;
-    a.vec_x = a.vec_y = a.vec_dx = a.vec_p = false;
+    a.vec_blocks = (c->channels + 32 * Width<T>::v - 1) / (32 * Width<T>::v);
     return a;
 }
 
-template <typename T, int W>
+template <typename T, int W, bool VEC>
 int forward_w(void* y, void* state_out, const void* x, const void* w, const void* bias, const void* state_in, const int* lengths,
               const RpbCausalConv* c, cudaStream_t s) {
-    constexpr int V = Width<T>::fwd;
-    const long long n_vec = (c->channels + V - 1) / V;
-    Args a = make_args(c, V, sizeof(T), pick_run(c->batch, c->len, n_vec, 32, SM_COUNT * 16));
-    const size_t bytes = sizeof(T) * V;
-    a.vec_x = aligned_rows(x_rows(c, x), c->batch, c->len, sizeof(T), bytes);
-    a.vec_y = aligned_rows(y_rows(c, y), c->batch, c->len, sizeof(T), bytes);
-    a.vec_p = packed_ok(c, state_in, bytes, sizeof(T)) && packed_ok(c, state_out, bytes, sizeof(T));
-    const long long items = (long long)c->batch * a.runs * n_vec;
-    const int block = items < (long long)SM_COUNT * 128 ? 32 : 128;     /* few items: one warp per block, on more SMs */
-    const long long blocks = (items + block - 1) / block;
+    const Args a = make_args<T>(c, pick_run(c->batch, c->len, (c->channels + Width<T>::v - 1) / Width<T>::v, 32, SM_COUNT * 16));
+    const long long warps = (long long)c->batch * a.runs * a.vec_blocks;
+    const int per = warps < SM_COUNT * 4 ? 1 : 4;                  /* few warps: one per block, on more SMs */
+    const long long blocks = ((long long)c->batch * a.runs + per - 1) / per * a.vec_blocks;
     if (blocks > 0x7fffffffLL) return refuse("rp_causal_conv_ex", "too many rows for one launch");
-    SEQ_CUDA(rpb_launch(forward_kernel<T, W>, dim3((unsigned)blocks), dim3(block), 0, s, 1, reinterpret_cast<T*>(y), reinterpret_cast<T*>(state_out),
+    SEQ_CUDA(rpb_launch(forward_kernel<T, W, VEC>, dim3((unsigned)blocks), dim3(32 * per), 0, s, 1, reinterpret_cast<T*>(y), reinterpret_cast<T*>(state_out),
                         reinterpret_cast<const T*>(x), reinterpret_cast<const T*>(w), reinterpret_cast<const T*>(bias),
                         reinterpret_cast<const T*>(state_in), lengths, a));
     rpb_count_launches(1);
     return 0;
 }
 
-template <typename T, int W>
+template <typename T, int W, bool VEC>
 int backward_w(void* dx, void* dw, void* dbias, void* dstate_in, int accumulate, const void* dy, const void* dstate_out, const void* x,
                const void* w, const void* bias, const void* state_in, const int* lengths, void* ws, const RpbCausalConv* c, cudaStream_t s) {
     typedef typename AccOf<T>::type A;
-    constexpr int V = Width<T>::bwd;
-    Args a = make_args(c, V, sizeof(T), backward_run<T>(c));
-    const size_t bytes = sizeof(T) * V;
-    a.vec_x = aligned_rows(x_rows(c, x), c->batch, c->len, sizeof(T), bytes);
-    a.vec_y = aligned_rows(y_rows(c, dy), c->batch, c->len, sizeof(T), bytes);
-    a.vec_dx = aligned_rows(dx_rows(c, dx), c->batch, c->len, sizeof(T), bytes);
-    a.vec_p = packed_ok(c, state_in, bytes, sizeof(T)) && packed_ok(c, dstate_in, bytes, sizeof(T)) && packed_ok(c, dstate_out, bytes, sizeof(T));
+    const Args a = make_args<T>(c, backward_run<T>(c));
     const long long groups = backward_groups<T>(c);
-    const int vec_blocks = (a.n_vec + 31) / 32;
-    if (groups * vec_blocks > 0x7fffffffLL) return refuse("rp_causal_conv_grad_ex", "too many rows for one launch");
+    if (groups * a.vec_blocks > 0x7fffffffLL) return refuse("rp_causal_conv_grad_ex", "too many rows for one launch");
     const bool filter = dw || dbias;
-    SEQ_CUDA(rpb_launch(backward_kernel<T, W>, dim3((unsigned)(groups * vec_blocks)), dim3(128), 0, s, 1, reinterpret_cast<T*>(dx),
+    SEQ_CUDA(rpb_launch(backward_kernel<T, W, VEC>, dim3((unsigned)(groups * a.vec_blocks)), dim3(128), 0, s, 1, reinterpret_cast<T*>(dx),
                         reinterpret_cast<T*>(dstate_in), filter ? reinterpret_cast<A*>(ws) : nullptr, (accumulate & RPB_CONV_ACC_DX) != 0,
                         reinterpret_cast<const T*>(dy), reinterpret_cast<const T*>(dstate_out), reinterpret_cast<const T*>(x),
-                        reinterpret_cast<const T*>(w), reinterpret_cast<const T*>(bias), reinterpret_cast<const T*>(state_in), lengths, a, vec_blocks));
+                        reinterpret_cast<const T*>(w), reinterpret_cast<const T*>(bias), reinterpret_cast<const T*>(state_in), lengths, a));
     rpb_count_launches(1);
     if (!filter) return 0;
+    const long long D = c->channels;
     PartSums d = {};
-    d.out[0] = dw; d.first[0] = 0; d.cols[0] = (long long)c->channels * W; d.accumulate[0] = (accumulate & RPB_CONV_ACC_DW) != 0;
-    d.out[1] = dbias; d.first[1] = (long long)c->channels * W; d.cols[1] = c->channels; d.accumulate[1] = (accumulate & RPB_CONV_ACC_DBIAS) != 0;
-    return sum_parts<T>(d, ws, (int)groups, (long long)c->channels * (W + 1), s);
+    d.out[0] = dw; d.first[0] = 0; d.cols[0] = D * c->width; d.accumulate[0] = (accumulate & RPB_CONV_ACC_DW) != 0;
+    d.out[1] = dbias; d.first[1] = D * c->width; d.cols[1] = D; d.accumulate[1] = (accumulate & RPB_CONV_ACC_DBIAS) != 0;
+    return sum_parts<T>(d, ws, (int)groups, D * (c->width + 1), s);
 }
 
-template <typename T, typename F> int by_width(int width, F f) {
-    switch (width) {
-        case 1: return f(std::integral_constant<int, 1>());
-        case 2: return f(std::integral_constant<int, 2>());
-        case 3: return f(std::integral_constant<int, 3>());
-        case 4: return f(std::integral_constant<int, 4>());
-        case 5: return f(std::integral_constant<int, 5>());
-        case 6: return f(std::integral_constant<int, 6>());
-        case 7: return f(std::integral_constant<int, 7>());
-        case 8: return f(std::integral_constant<int, 8>());
-    }
+/* The kernels are built for 2, 3, 4 and 8 taps; fewer are the last ones of these. */
+template <typename T, typename F> int by_width(int width, bool vec, F f) {
+#define CASE(n) if (width <= n) return vec ? f(std::integral_constant<int, n>(), std::true_type()) : f(std::integral_constant<int, n>(), std::false_type());
+    CASE(2) CASE(3) CASE(4) CASE(8)
+#undef CASE
     return -1;
+}
+
+template <typename T>
+int run_forward(void* y, void* state_out, const void* x, const void* w, const void* bias, const void* state_in, const int* lengths,
+                const RpbCausalConv* c, cudaStream_t s) {
+    const bool vec = c->channels % Width<T>::v == 0 && packs_ok<T>(c, x_rows(c, x)) && packs_ok<T>(c, y_rows(c, y)) && state_ok<T>(c, state_in) &&
+                     state_ok<T>(c, state_out);
+    return by_width<T>(c->width, vec, [&](auto n, auto p) {
+        return forward_w<T, decltype(n)::value, decltype(p)::value>(y, state_out, x, w, bias, state_in, lengths, c, s);
+    });
+}
+template <typename T>
+int run_backward(void* dx, void* dw, void* dbias, void* dstate_in, int accumulate, const void* dy, const void* dstate_out, const void* x,
+                 const void* w, const void* bias, const void* state_in, const int* lengths, void* ws, const RpbCausalConv* c, cudaStream_t s) {
+    const bool vec = c->channels % Width<T>::v == 0 && packs_ok<T>(c, x_rows(c, x)) && packs_ok<T>(c, y_rows(c, dy)) && packs_ok<T>(c, dx_rows(c, dx)) &&
+                     state_ok<T>(c, state_in) && state_ok<T>(c, dstate_in) && state_ok<T>(c, dstate_out);
+    return by_width<T>(c->width, vec, [&](auto n, auto p) {
+        return backward_w<T, decltype(n)::value, decltype(p)::value>(dx, dw, dbias, dstate_in, accumulate, dy, dstate_out, x, w, bias, state_in, lengths,
+                                                                     ws, c, s);
+    });
 }
 
 const char* bad_geometry(const RpbCausalConv* c, DType dtype) {
@@ -373,7 +458,7 @@ int rp_causal_conv_ex(void* y, void* state_out, const void* x, const void* w, co
     if (scope.enter(device_id)) return refuse(name, "no such device");
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     switch ((int)dtype) {
-#define CASE(code, T) case code: return by_width<T>(c->width, [&](auto W) { return forward_w<T, decltype(W)::value>(y, state_out, x, w, bias, state_in, lengths, c, s); });
+#define CASE(code, T) case code: return run_forward<T>(y, state_out, x, w, bias, state_in, lengths, c, s);
         CASE(DTYPE_FLOAT32, float) CASE(DTYPE_FLOAT64, double) CASE(DTYPE_FLOAT16, __half) CASE(DTYPE_BFLOAT16, __nv_bfloat16)
 #undef CASE
     }
@@ -411,7 +496,7 @@ int rp_causal_conv_grad_ex(void* dx, void* dw, void* dbias, void* dstate_in, int
     if (scope.enter(device_id)) return refuse(name, "no such device");
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     switch ((int)dtype) {
-#define CASE(code, T) case code: return by_width<T>(c->width, [&](auto W) { return backward_w<T, decltype(W)::value>(dx, dw, dbias, dstate_in, accumulate, dy, dstate_out, x, w, bias, state_in, lengths, ws, c, s); });
+#define CASE(code, T) case code: return run_backward<T>(dx, dw, dbias, dstate_in, accumulate, dy, dstate_out, x, w, bias, state_in, lengths, ws, c, s);
         CASE(DTYPE_FLOAT32, float) CASE(DTYPE_FLOAT64, double) CASE(DTYPE_FLOAT16, __half) CASE(DTYPE_BFLOAT16, __nv_bfloat16)
 #undef CASE
     }
