@@ -113,7 +113,7 @@ class Tensor:
         """Borrowed view of the accumulated gradient (None before backward)."""
         if not self._t.metadata or not self._t.metadata.contents.grad:
             return None
-        g = self._t.metadata.contents.grad
+        g = C.pointer(self._t.metadata.contents.grad.contents)      # a pointer of its own: the field may be cleared or freed later
         g.contents.refcount += 1
         return Tensor(g, keepalive=self)
 
@@ -176,6 +176,38 @@ class Tensor:
         if not p:
             raise RuntimeError("op_gru_cell operation failed")
         return Tensor(p, keepalive=(self, w_ih, h, w_hh, b_ih, b_hh))
+
+    def op_causal_conv(self, weight: "Tensor", bias: "Tensor | None" = None, silu: bool = True) -> "Tensor":
+        """Short causal convolution of [batch, len, channels], one filter of ``weight`` [channels, width] per channel."""
+        p = _lib.load().op_causal_conv(self._p, weight._p, bias._p if bias is not None else None, int(silu))
+        if not p:
+            raise RuntimeError("op_causal_conv operation failed")
+        return Tensor(p, keepalive=(self, weight, bias))
+
+    def op_selective_scan(self, dt: "Tensor", A: "Tensor", B: "Tensor", C: "Tensor", D: "Tensor | None" = None,
+                          dt_bias: "Tensor | None" = None, z: "Tensor | None" = None, softplus: bool = True) -> "Tensor":
+        """Selective state space scan of [batch, len, channels] along len, behind the gate z when one is given."""
+        opt = [t._p if t is not None else None for t in (D, dt_bias, z)]
+        p = _lib.load().op_selective_scan(self._p, dt._p, A._p, B._p, C._p, *opt, int(softplus))
+        if not p:
+            raise RuntimeError("op_selective_scan operation failed")
+        return Tensor(p, keepalive=(self, dt, A, B, C, D, dt_bias, z))
+
+    def op_gated_norm(self, z: "Tensor | None", weight: "Tensor | None", scale: "Tensor | None" = None, residual: "Tensor | None" = None,
+                      eps: float = 1e-5) -> "Tensor":
+        """residual + scale * (RMS norm of self silu(z)) * weight; every part but self may be None."""
+        opt = [t._p if t is not None else None for t in (z, weight, scale, residual)]
+        p = _lib.load().op_gated_norm(self._p, *opt, eps)
+        if not p:
+            raise RuntimeError("op_gated_norm operation failed")
+        return Tensor(p, keepalive=(self, z, weight, scale, residual))
+
+    def op_rms_norm(self, weight: "Tensor", eps: float = 1e-5) -> "Tensor":
+        """self / sqrt(mean self^2 + eps) * weight over the last dimension."""
+        p = _lib.load().op_rms_norm(self._p, weight._p, eps)
+        if not p:
+            raise RuntimeError("op_rms_norm operation failed")
+        return Tensor(p, keepalive=(self, weight))
 
     def backward(self, grad_output: "Tensor") -> None:
         """Run this node's backward with an explicit upstream gradient and free the node."""
