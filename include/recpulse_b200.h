@@ -316,6 +316,21 @@ int rp_block_norm_grad_ex(void* du, void* dz, void* dr, void* dw_after, void* ds
                           const void* r, const void* w_before, void* ws, const RpbBlockNorm* c, DType dtype, int device_id,
                           void* stream);
 
+/* ---- additive: the operators along a sequence as nodes --------------------------
+ * Autograd nodes like op_linear's, on the node stream (rpb_node_stream); outputs are new packed tensors, gradients are assigned or
+ * added to existing ones.  A sequence operand is [batch, len, channels] with unit stride within a row (a column block of a wider
+ * tensor will do).  One tensor in two places of a node is refused when it requires a gradient (a view of it is another tensor).
+ * op_causal_conv: w [channels, width], bias [channels] or NULL, activation as in RpbCausalConv; starts from zeros.
+ * op_selective_scan: A, D, dt_bias float32 (float64 for float64 data); groups = columns of B / columns of A; starts from zeros.
+ * op_gated_norm: r + scale * (norm of u behind its gate) w; z, w, scale and r may each be NULL.  op_rms_norm: x / rms(x) * w. */
+Tensor* op_causal_conv(Tensor* x, Tensor* w, Tensor* bias, int activation);
+void backward_causal_conv_fn(GradFn* self, Tensor* grad_output);
+Tensor* op_selective_scan(Tensor* x, Tensor* dt, Tensor* A, Tensor* B, Tensor* C, Tensor* D, Tensor* dt_bias, Tensor* z, int softplus);
+void backward_selective_scan_fn(GradFn* self, Tensor* grad_output);
+Tensor* op_gated_norm(Tensor* u, Tensor* z, Tensor* w, Tensor* scale, Tensor* r, float eps);
+Tensor* op_rms_norm(Tensor* x, Tensor* w, float eps);
+void backward_block_norm_fn(GradFn* self, Tensor* grad_output);
+
 /* ---- additive: strided / batched GEMM on raw pointers ----------------------*/
 
 typedef struct {

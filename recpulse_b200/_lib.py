@@ -111,6 +111,13 @@ SYMBOLS = {
     "rp_block_norm_ws_bytes": (C.c_longlong, [C.POINTER(RpbBlockNorm), C.c_int]),
     "rp_block_norm_grad_ex": (C.c_int, [C.c_void_p] * 6 + [C.c_int] + [C.c_void_p] * 9 +
                               [C.POINTER(RpbBlockNorm), C.c_int, C.c_int, C.c_void_p]),
+    "op_causal_conv": (TP, [TP, TP, TP, C.c_int]),
+    "backward_causal_conv_fn": (None, [C.POINTER(GradFn), TP]),
+    "op_selective_scan": (TP, [TP] * 8 + [C.c_int]),
+    "backward_selective_scan_fn": (None, [C.POINTER(GradFn), TP]),
+    "op_gated_norm": (TP, [TP] * 5 + [C.c_float]),
+    "op_rms_norm": (TP, [TP, TP, C.c_float]),
+    "backward_block_norm_fn": (None, [C.POINTER(GradFn), TP]),
     "rp_colsum_ex": (C.c_int, [C.c_void_p, C.c_void_p, C.c_longlong, C.c_int, C.c_longlong, C.c_int, C.c_int, C.c_int,
                                C.c_void_p]),
     "rpb_gemm_packed": (None, [C.POINTER(RpbGemm), C.c_int, C.c_int, C.c_int]),

@@ -733,3 +733,8 @@ int rpb_backward_node(Tensor* out, Tensor* grad_output) {
     out->metadata->grad_fn = NULL;
     return 0;
 }
+
+/* what op_sequence.c's nodes share with these */
+cudaStream_t rpb_current_node_stream(void) { return t_stream; }
+int rpb_finish_node(int device_id) { return node_finish(device_id); }
+int rpb_attach_node(Tensor* out, BackwardFunction backward, Tensor** in, int n_in) { return attach_node(out, backward, in, n_in); }
