@@ -17,7 +17,7 @@ struct Args {
     long long rows;
     int channels, classes;      /* rows r, r + classes, ... begin at the same offset from a 16-byte boundary */
     double eps_after, eps_before;
-    long long u_row, z_row, r_row, out_row, y_row, du_row, dz_row, dr_row;
+    int u_row, z_row, r_row, out_row, y_row, du_row, dz_row, dr_row;        /* below 2^31; their products with a row are 64 bits */
 };
 
 template <typename T> struct Width { static constexpr int v = 16 / sizeof(T); };
@@ -56,12 +56,12 @@ template <typename T, int NV, bool PACKS> struct Span {
     static constexpr unsigned ALL = (1u << V) - 1;
     int base, step;
     unsigned mask[NV];          /* which values of a pack are channels of the row */
-    bool ragged;                /* some pack of the row is not whole */
+    int bytes[NV];              /* of a pack up to the row's end */
+    int off;                    /* channels that the first pack begins in front of the row */
     __device__ __forceinline__ Span(const T* row, int channels) {
-        const int off = PACKS ? (int)(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T)) : 0;
+        off = PACKS ? (int)(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T)) : 0;
         base = PACKS ? (int)threadIdx.x * V - off : (int)threadIdx.x;
         step = PACKS ? (int)blockDim.x * V : (int)blockDim.x;
-        ragged = off != 0 || channels % V != 0;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             mask[k] = 0;
@@ -70,34 +70,38 @@ template <typename T, int NV, bool PACKS> struct Span {
                 const int c = channel(k, i);
                 if (c >= 0 && c < channels) mask[k] |= 1u << i;
             }
+            const int left = channels - channel(k, 0);
+            bytes[k] = (int)sizeof(T) * (left < 0 ? 0 : left > V ? V : left);
         }
     }
     __device__ __forceinline__ int channel(int k, int i) const { return PACKS ? base + k * step + i : base + (k * V + i) * step; }
     __device__ __forceinline__ bool has(int k, int i) const { return mask[k] >> i & 1; }
-    /* `edge`: nothing outside the row may be read (the first and the last row of an operand); elsewhere a pack that sticks out
-     * reads its neighbours, which tidy() takes out again before use: no load waits for a decision */
-    __device__ __forceinline__ void load(Pack<T, V> (&p)[NV], const T* row, bool given, bool edge) const {
-        const bool packs = PACKS && !(edge && ragged);
+    /* The thread's packs of a row into its slots, which nobody else reads, asynchronously where they lie on boundaries.  A pack
+     * that begins in front of the row brings the end of the row before along (take() leaves it out); the operand's first row,
+     * with nothing in front of it, is read value by value, as are rows off the boundaries. */
+    __device__ __forceinline__ void bring(Pack<T, V>* slots, const T* row, bool given, bool first) const {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            p[k] = zero_pack<T, V>();
-            if (packs) {
-                if (given && mask[k]) p[k] = *reinterpret_cast<const Pack<T, V>*>(row + channel(k, 0));
+            Pack<T, V>* to = slots + k * blockDim.x + threadIdx.x;
+            if (PACKS && !(first && off)) {
+                async_copy_part<16>(to, row + channel(k, 0), given ? bytes[k] : 0);
             } else {
+                Pack<T, V> p = zero_pack<T, V>();
 #pragma unroll
                 for (int i = 0; i < V; ++i)
-                    if (given && has(k, i)) p[k].v[i] = row[channel(k, i)];
+                    if (given && has(k, i)) p.v[i] = row[channel(k, i)];
+                *to = p;
             }
         }
     }
-    __device__ __forceinline__ void tidy(Pack<T, V> (&p)[NV]) const {
+    __device__ __forceinline__ Pack<T, V> take(const Pack<T, V>* slots, int k) const {
+        Pack<T, V> p = slots[k * blockDim.x + threadIdx.x];
+        if (PACKS && off && k == 0 && threadIdx.x == 0) {
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
-            if (PACKS && ragged && mask[k] != ALL) {
-#pragma unroll
-                for (int i = 0; i < V; ++i)
-                    if (!has(k, i)) p[k].v[i] = down<T>(typename AccOf<T>::type(0));
-            }
+            for (int i = 0; i < V; ++i)
+                if (!has(k, i)) p.v[i] = down<T>(typename AccOf<T>::type(0));
+        }
+        return p;
     }
     __device__ __forceinline__ Pack<T, V> load_one(const T* row, int k) const {
         Pack<T, V> p = zero_pack<T, V>();
@@ -140,12 +144,16 @@ __device__ __forceinline__ Turn turn_of(const Args& a) {
     return {(long long)(blockIdx.x / a.classes) * a.classes + blockIdx.x % a.classes, (long long)per_class * a.classes};
 }
 
+/* Rows of a block in shared memory: the one worked on and the next two or one; 0 for rows too wide for that (over 1024 packs),
+ * whose values are read where they lie each time they are needed. */
+template <int NV> struct Slots { static constexpr int forward = NV <= 2 ? 3 : 0, backward = NV == 1 ? 3 : NV == 2 ? 2 : 0; };
+
 template <typename T, int NV, bool PACKS>
 __global__ void __launch_bounds__(512, NV == 1 ? 2 : 1)
 forward_kernel(T* __restrict__ out, T* __restrict__ y, const T* __restrict__ u, const T* __restrict__ z, const T* __restrict__ w_after,
                const T* __restrict__ scale, const T* __restrict__ r, const T* __restrict__ w_before, Args a) {
     typedef typename AccOf<T>::type A;
-    constexpr int V = Width<T>::v;
+    constexpr int V = Width<T>::v, SLOTS = Slots<NV>::forward;
     __shared__ A buffer[2][1][32];
     int turn = 0;
     rpb_pdl_trigger();
@@ -154,35 +162,42 @@ forward_kernel(T* __restrict__ out, T* __restrict__ y, const T* __restrict__ u, 
     const Turn t = turn_of(a);
     if (t.row >= a.rows) return;
     const Span<T, NV, PACKS> span(u + t.row * a.u_row, a.channels);
-    const int nt = blockDim.x, tid = threadIdx.x;
-    Pack<T, V>* ws = weight_slots<T>();
-    keep_weights(ws, w_after, span);
-    keep_weights(ws + NV * nt, scale, span);
-    keep_weights(ws + 2 * NV * nt, w_before, span);
-    /* the next row's operands are on their way while a row is worked on, where the registers reach */
-    constexpr bool AHEAD = NV * V <= 8;
-    Pack<T, V> un[NV], zn[NV], rn[NV];
-    auto fetch = [&](long long row) {
-        const bool in = row < a.rows, edge = row == 0 || row == a.rows - 1;
-        span.load(un, u + row * a.u_row, in, edge);
-        span.load(zn, z + row * a.z_row, z && in, edge);
-        span.load(rn, r + row * a.r_row, r && in, edge);
+    const int nt = blockDim.x, tid = threadIdx.x, per = NV * nt;
+    Pack<T, V> *ws = weight_slots<T>(), *ring = ws + 3 * per;
+    auto fetch = [&](long long row, int slot) {
+        const bool in = row < a.rows;
+        Pack<T, V>* to = ring + slot * 3 * per;
+        span.bring(to, u + (long long)(int)row * a.u_row, in, row == 0);
+        if (z) span.bring(to + per, z + (long long)(int)row * a.z_row, in, row == 0);
+        if (r) span.bring(to + 2 * per, r + (long long)(int)row * a.r_row, in, row == 0);
+        async_commit();
     };
-    if (AHEAD) fetch(t.row);
-    for (long long row = t.row; row < a.rows; row += t.step) {
-        if (!AHEAD) fetch(row);
-        A v[NV][V], o[NV][V], sq[1] = {0};
-        span.tidy(un); span.tidy(zn); span.tidy(rn);
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
+    for (int k = 0; k + 1 < SLOTS; ++k) fetch(t.row + k * t.step, k);
+    if (SLOTS) {
+    keep_weights(ws, w_after, span);
+    keep_weights(ws + per, scale, span);
+    keep_weights(ws + 2 * per, w_before, span);
+    }
+    int slot = 0;
+    for (long long row = t.row; row < a.rows; row += t.step) {
+        if (SLOTS) async_wait<SLOTS ? SLOTS - 2 : 0>();
+        const Pack<T, V>* from = ring + slot * 3 * per;
+        const T* rows[3] = {u + (long long)(int)row * a.u_row, z + (long long)(int)row * a.z_row, r + (long long)(int)row * a.r_row};
+        auto take = [&](int n, int k) { return SLOTS ? span.take(from + n * per, k) : span.load_one(rows[n], k); };
+        auto weight = [&](int n, const T* w, int k) { return SLOTS ? ws[n * per + k * nt + tid] : w ? span.load_one(w, k) : zero_pack<T, V>(); };
+        A o[NV][V], sq[1] = {0};
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const Pack<T, V> up_ = take(0, k), zp = z ? take(1, k) : up_;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                v[k][i] = up(un[k].v[i]);
-                if (z) { const A g = up(zn[k].v[i]); v[k][i] *= g * logistic(g); }
-                o[k][i] = up(rn[k].v[i]);
-                sq[0] += v[k][i] * v[k][i];
+                o[k][i] = up(up_.v[i]);
+                if (z) { const A g = up(zp.v[i]); o[k][i] *= g * logistic(g); }
+                sq[0] += o[k][i] * o[k][i];
             }
-        if (AHEAD) fetch(row + t.step);
+        }
+        if (SLOTS) fetch(row + (SLOTS - 1) * t.step, slot == 0 ? SLOTS - 1 : slot - 1);
         A i1 = 1;
         if (w_after) {
             block_sums(sq, buffer, turn);
@@ -191,31 +206,39 @@ forward_kernel(T* __restrict__ out, T* __restrict__ y, const T* __restrict__ u, 
         sq[0] = 0;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            const Pack<T, V> wp = ws[k * nt + tid], sp = ws[(NV + k) * nt + tid];
-            Pack<T, V> q;
+            const Pack<T, V> wp = weight(0, w_after, k), sp = weight(1, scale, k);
+            if (w_after) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                A s = v[k][i];
-                if (w_after) s = s * i1 * up(wp.v[i]);
-                if (scale) s *= up(sp.v[i]);
-                o[k][i] += s;
-                q.v[i] = down<T>(o[k][i]);
-                sq[0] += o[k][i] * o[k][i];
+                for (int i = 0; i < V; ++i) o[k][i] = o[k][i] * i1 * up(wp.v[i]);
             }
-            if (out) span.store(out + row * a.out_row, k, q);
-        }
-        if (!y) continue;
-        block_sums(sq, buffer, turn);
-        const A i2 = rsqrt_of(sq[0] * inv + A(a.eps_before));
+            if (scale) {
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const Pack<T, V> wp = ws[(2 * NV + k) * nt + tid];
-            Pack<T, V> q;
+                for (int i = 0; i < V; ++i) o[k][i] *= up(sp.v[i]);
+            }
+            if (r) {
+                const Pack<T, V> rp = take(2, k);
 #pragma unroll
-            for (int i = 0; i < V; ++i) q.v[i] = down<T>(o[k][i] * i2 * up(wp.v[i]));
-            span.store(y + row * a.y_row, k, q);
+                for (int i = 0; i < V; ++i) o[k][i] += up(rp.v[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) sq[0] += o[k][i] * o[k][i];
+            if (out) span.store(out + (long long)(int)row * a.out_row, k, store_form<T, V>(o[k]));
         }
+        if (y) {
+            block_sums(sq, buffer, turn);
+            const A i2 = rsqrt_of(sq[0] * inv + A(a.eps_before));
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const Pack<T, V> wp = weight(2, w_before, k);
+                A q[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) q[i] = o[k][i] * i2 * up(wp.v[i]);
+                span.store(y + (long long)(int)row * a.y_row, k, store_form<T, V>(q));
+            }
+        }
+        slot = slot + 1 >= SLOTS ? 0 : slot + 1;
     }
+    async_wait<0>();
 }
 
 /* Each block keeps its part of the weights' gradients in registers; sum_parts adds the blocks' parts [3][channels]: w_after,
@@ -226,101 +249,127 @@ backward_kernel(T* du, T* dz, T* dr, typename AccOf<T>::type* __restrict__ parts
                 const T* __restrict__ dy, const T* __restrict__ u, const T* __restrict__ z, const T* __restrict__ w_after, const T* __restrict__ scale,
                 const T* __restrict__ r, const T* __restrict__ w_before, Args a) {
     typedef typename AccOf<T>::type A;
-    constexpr int V = Width<T>::v;
+    constexpr int V = Width<T>::v, SLOTS = Slots<NV>::backward;
     __shared__ A buffer[2][2][32];
     int turn = 0;
     rpb_pdl_trigger();
     rpb_pdl_wait();
     const A inv = A(1) / A(a.channels);
     const Turn t = turn_of(a);
-    const int nt = blockDim.x, tid = threadIdx.x;
-    Pack<T, V>* ws = weight_slots<T>();
+    const int nt = blockDim.x, tid = threadIdx.x, per = NV * nt;
     const Span<T, NV, PACKS> span(u + t.row * a.u_row, a.channels);
+    Pack<T, V> *ws = weight_slots<T>(), *ring = ws + 3 * per;
+    auto fetch = [&](long long row, int slot) {
+        const bool in = row < a.rows;
+        Pack<T, V>* to = ring + slot * 5 * per;
+        span.bring(to, u + (long long)(int)row * a.u_row, in, row == 0);
+        if (z) span.bring(to + per, z + (long long)(int)row * a.z_row, in, row == 0);
+        if (r) span.bring(to + 2 * per, r + (long long)(int)row * a.r_row, in, row == 0);
+        if (dout) span.bring(to + 3 * per, dout + (long long)(int)row * a.out_row, in, row == 0);
+        if (dy) span.bring(to + 4 * per, dy + (long long)(int)row * a.y_row, in, row == 0);
+        async_commit();
+    };
+#pragma unroll
+    for (int k = 0; k + 1 < SLOTS; ++k) fetch(t.row + k * t.step, k);
+    if (SLOTS) {
     keep_weights(ws, w_after, span);
-    keep_weights(ws + NV * nt, scale, span);
-    keep_weights(ws + 2 * NV * nt, dy ? w_before : nullptr, span);
+    keep_weights(ws + per, scale, span);
+    keep_weights(ws + 2 * per, dy ? w_before : nullptr, span);
+    }
     A gwa[NV][V], gsc[NV][V], gwb[NV][V];
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int i = 0; i < V; ++i) gwa[k][i] = gsc[k][i] = gwb[k][i] = 0;
-    constexpr bool AHEAD = NV * V <= 8;
-    Pack<T, V> un[NV], zn[NV], rn[NV], on[NV], yn[NV];
-    auto fetch = [&](long long row) {
-        const bool in = row < a.rows, edge = row == 0 || row == a.rows - 1;
-        span.load(un, u + row * a.u_row, in, edge);
-        span.load(zn, z + row * a.z_row, z && in, edge);
-        span.load(rn, r + row * a.r_row, r && in, edge);
-        span.load(on, dout + row * a.out_row, dout && in, edge);
-        span.load(yn, dy + row * a.y_row, dy && in, edge);
-    };
-    if (AHEAD) fetch(t.row);
+    int slot = 0;
     for (long long row = t.row; row < a.rows; row += t.step) {
-        if (!AHEAD) fetch(row);
-        Pack<T, V> up_[NV], zp[NV], rp[NV], op[NV], yp[NV];
-        A v[NV][V], sq[2] = {0, 0};
-        span.tidy(un); span.tidy(zn); span.tidy(rn); span.tidy(on); span.tidy(yn);
+        if (SLOTS) async_wait<SLOTS ? SLOTS - 2 : 0>();
+        const Pack<T, V>* from = ring + slot * 5 * per;
+        const T* rows[5] = {u + (long long)(int)row * a.u_row, z + (long long)(int)row * a.z_row, r + (long long)(int)row * a.r_row, dout + (long long)(int)row * a.out_row, dy + (long long)(int)row * a.y_row};
+        auto take = [&](int n, int k) { return SLOTS ? span.take(from + n * per, k) : span.load_one(rows[n], k); };
+        auto weight = [&](int n, const T* w, int k) { return SLOTS ? ws[n * per + k * nt + tid] : w ? span.load_one(w, k) : zero_pack<T, V>(); };
+        A v[NV][V], total[NV][V], sq[2] = {0, 0};
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            up_[k] = un[k]; zp[k] = zn[k]; rp[k] = rn[k]; op[k] = on[k]; yp[k] = yn[k];
+            const Pack<T, V> up_ = take(0, k), zp = z ? take(1, k) : up_;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                v[k][i] = up(up_[k].v[i]);
-                if (z) { const A g = up(zp[k].v[i]); v[k][i] *= g * logistic(g); }
+                v[k][i] = up(up_.v[i]);
+                if (z) { const A g = up(zp.v[i]); v[k][i] *= g * logistic(g); }
                 sq[0] += v[k][i] * v[k][i];
             }
         }
-        if (AHEAD) fetch(row + t.step);
+        if (SLOTS) fetch(row + (SLOTS - 1) * t.step, slot == 0 ? SLOTS - 1 : slot - 1);
         A i1 = 1;
         if (w_after) {
             block_sums(sq, buffer, turn);
             i1 = rsqrt_of(sq[0] * inv + A(a.eps_after));
         }
-        /* the gradient of out */
-        A total[NV][V];
+        /* total: the gradient of out */
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) total[k][i] = 0;
         if (dy) {
             sq[0] = sq[1] = 0;
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                const Pack<T, V> wa = ws[k * nt + tid], sc = ws[(NV + k) * nt + tid], wb = ws[(2 * NV + k) * nt + tid];
+                const Pack<T, V> wa = weight(0, w_after, k), sc = weight(1, scale, k), wb = weight(2, dy ? w_before : nullptr, k), yp = take(4, k);
+#pragma unroll
+                for (int i = 0; i < V; ++i) total[k][i] = v[k][i] * i1;         /* out itself, for now */
+                if (w_after) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) total[k][i] *= up(wa.v[i]);
+                }
+                if (scale) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) total[k][i] *= up(sc.v[i]);
+                }
+                if (r) {
+                    const Pack<T, V> rp = take(2, k);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) total[k][i] += up(rp.v[i]);
+                }
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    A s = v[k][i] * i1;
-                    if (w_after) s *= up(wa.v[i]);
-                    if (scale) s *= up(sc.v[i]);
-                    total[k][i] = up(rp[k].v[i]) + s;           /* out itself, for now */
                     sq[0] += total[k][i] * total[k][i];
-                    sq[1] += up(yp[k].v[i]) * up(wb.v[i]) * total[k][i];
+                    sq[1] += up(yp.v[i]) * up(wb.v[i]) * total[k][i];
                 }
             }
             block_sums(sq, buffer, turn);
             const A i2 = rsqrt_of(sq[0] * inv + A(a.eps_before)), pull = sq[1] * inv * i2 * i2;
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                const Pack<T, V> wb = ws[(2 * NV + k) * nt + tid];
+                const Pack<T, V> wb = weight(2, dy ? w_before : nullptr, k), yp = take(4, k);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const A o = total[k][i], g = up(yp[k].v[i]);
+                    const A o = total[k][i], g = up(yp.v[i]);
                     gwb[k][i] += g * o * i2;
-                    total[k][i] = up(op[k].v[i]) + i2 * (g * up(wb.v[i]) - o * pull);
+                    total[k][i] = i2 * (g * up(wb.v[i]) - o * pull);
                 }
             }
-        } else {
-#pragma unroll
-            for (int k = 0; k < NV; ++k)
-#pragma unroll
-                for (int i = 0; i < V; ++i) total[k][i] = up(op[k].v[i]);
         }
         sq[0] = sq[1] = 0;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            if (dr) {
-                Pack<T, V> q = acc_dr ? span.load_one(dr + row * a.dr_row, k) : zero_pack<T, V>();
+            if (dout) {
+                const Pack<T, V> op = take(3, k);
 #pragma unroll
-                for (int i = 0; i < V; ++i) q.v[i] = down<T>(total[k][i] + up(q.v[i]));
-                span.store(dr + row * a.dr_row, k, q);
+                for (int i = 0; i < V; ++i) total[k][i] += up(op.v[i]);
             }
-            const Pack<T, V> wa = ws[k * nt + tid], sc = ws[(NV + k) * nt + tid];
+            if (dr) {
+                T* to = dr + (long long)(int)row * a.dr_row;
+                A sum[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) sum[i] = total[k][i];
+                if (acc_dr) {
+                    const Pack<T, V> have = span.load_one(to, k);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) sum[i] += up(have.v[i]);
+                }
+                span.store(to, k, store_form<T, V>(sum));
+            }
+            const Pack<T, V> wa = weight(0, w_after, k), sc = weight(1, scale, k);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const A m = v[k][i] * i1, w = w_after ? up(wa.v[i]) : A(1), s = scale ? up(sc.v[i]) : A(1);
@@ -337,22 +386,40 @@ backward_kernel(T* du, T* dz, T* dr, typename AccOf<T>::type* __restrict__ parts
         }
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            Pack<T, V> o = du && acc_du ? span.load_one(du + row * a.du_row, k) : zero_pack<T, V>();
-            Pack<T, V> q = dz && acc_dz ? span.load_one(dz + row * a.dz_row, k) : zero_pack<T, V>();
+            A gu[V], gz[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                A dv = i1 * (total[k][i] - v[k][i] * pull);
-                if (z) {
-                    const A g = up(zp[k].v[i]), s = logistic(g);
-                    q.v[i] = down<T>(up(q.v[i]) + dv * up(up_[k].v[i]) * s * (A(1) + g * (A(1) - s)));
-                    dv *= g * s;
+            for (int i = 0; i < V; ++i) gu[i] = i1 * (total[k][i] - v[k][i] * pull);
+            if (z) {
+                const Pack<T, V> up_ = take(0, k), zp = take(1, k);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const A g = up(zp.v[i]), s = logistic(g);
+                    gz[i] = gu[i] * up(up_.v[i]) * s * (A(1) + g * (A(1) - s));
+                    gu[i] *= g * s;
                 }
-                o.v[i] = down<T>(up(o.v[i]) + dv);
             }
-            if (du) span.store(du + row * a.du_row, k, o);
-            if (dz) span.store(dz + row * a.dz_row, k, q);
+            if (du) {
+                T* to = du + (long long)(int)row * a.du_row;
+                if (acc_du) {
+                    const Pack<T, V> have = span.load_one(to, k);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) gu[i] += up(have.v[i]);
+                }
+                span.store(to, k, store_form<T, V>(gu));
+            }
+            if (dz && z) {
+                T* to = dz + (long long)(int)row * a.dz_row;
+                if (acc_dz) {
+                    const Pack<T, V> have = span.load_one(to, k);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) gz[i] += up(have.v[i]);
+                }
+                span.store(to, k, store_form<T, V>(gz));
+            }
         }
+        slot = slot + 1 >= SLOTS ? 0 : slot + 1;
     }
+    async_wait<0>();
     if (!parts) return;
     A* part = parts + (long long)blockIdx.x * 3 * a.channels;
 #pragma unroll
@@ -408,8 +475,8 @@ template <typename T> bool packs_of(const RpbBlockNorm* c, const Operand* o, int
 Args make_args(const RpbBlockNorm* c) {
     Args a;
     a.rows = c->rows; a.channels = c->channels; a.classes = 1; a.eps_after = c->eps_after; a.eps_before = c->eps_before;
-    a.u_row = c->u_row; a.z_row = c->z_row; a.r_row = c->r_row; a.out_row = c->out_row; a.y_row = c->y_row;
-    a.du_row = c->du_row; a.dz_row = c->dz_row; a.dr_row = c->dr_row;
+    a.u_row = (int)c->u_row; a.z_row = (int)c->z_row; a.r_row = (int)c->r_row; a.out_row = (int)c->out_row; a.y_row = (int)c->y_row;
+    a.du_row = (int)c->du_row; a.dz_row = (int)c->dz_row; a.dr_row = (int)c->dr_row;
     return a;
 }
 
@@ -417,11 +484,13 @@ struct Operands { const void *u, *z, *w_after, *scale, *r, *w_before; };
 
 template <typename T, int NV, bool PACKS>
 int forward_n(void* out, void* y, const Operands& o, const Args& a, int threads, cudaStream_t s) {
-    const size_t smem = (size_t)3 * NV * threads * 16;
-    if (smem > 40 * 1024)
-        SEQ_CUDA(cudaFuncSetAttribute(forward_kernel<T, NV, PACKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const size_t smem = Slots<NV>::forward ? (size_t)(3 + Slots<NV>::forward * 3) * NV * threads * 16 : 0;
+    static unsigned char done[64];
+    int device = 0;
+    SEQ_CUDA(cudaGetDevice(&device));
+    if (allow_shared(forward_kernel<T, NV, PACKS>, smem, device, done)) return -1;
     /* as many blocks as the chip holds at once, at least one row each; a multiple of 8 for the classes */
-    long long most = (long long)SM_COUNT * (NV > 1 ? 1 : 1024 / threads < 16 ? 1024 / threads : 16);
+    long long most = (long long)SM_COUNT * (NV > 1 ? 1 : 1024 / threads < 8 ? 1024 / threads : 8);
     most -= most % 8;
     const long long rows = (a.rows + 7) / 8 * 8;
     const unsigned blocks = (unsigned)(rows < most ? rows : most);
@@ -439,9 +508,11 @@ int backward_n(const Wanted& w, const void* dout, const void* dy, const Operands
                cudaStream_t s) {
     typedef typename AccOf<T>::type A;
     const bool weights = w.dw_after || w.dscale || w.dw_before;
-    const size_t smem = (size_t)3 * NV * threads * 16;
-    if (smem > 40 * 1024)
-        SEQ_CUDA(cudaFuncSetAttribute(backward_kernel<T, NV, PACKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const size_t smem = Slots<NV>::backward ? (size_t)(3 + Slots<NV>::backward * 5) * NV * threads * 16 : 0;
+    static unsigned char done[64];
+    int device = 0;
+    SEQ_CUDA(cudaGetDevice(&device));
+    if (allow_shared(backward_kernel<T, NV, PACKS>, smem, device, done)) return -1;
     SEQ_CUDA(rpb_launch(backward_kernel<T, NV, PACKS>, dim3((unsigned)blocks), dim3(threads), smem, s, 1, reinterpret_cast<T*>(w.du),
                         reinterpret_cast<T*>(w.dz), reinterpret_cast<T*>(w.dr), weights ? reinterpret_cast<A*>(ws) : nullptr,
                         (w.accumulate & RPB_NORM_ACC_DU) != 0, (w.accumulate & RPB_NORM_ACC_DZ) != 0, (w.accumulate & RPB_NORM_ACC_DR) != 0,
@@ -494,6 +565,9 @@ const char* bad_geometry(const RpbBlockNorm* c, DType dtype) {
     if (!rpb_dtype_size((int)dtype)) return "unknown element type";
     if (c->rows <= 0 || c->channels <= 0) return "rows and channels must be positive";
     if (c->channels > MAX_CHANNELS) return "rows longer than 8192 channels";
+    const long long strides[8] = {c->u_row, c->z_row, c->r_row, c->out_row, c->y_row, c->du_row, c->dz_row, c->dr_row};
+    for (long long r : strides)
+        if (c->rows > 0x7fffffffLL || r > 0x7fffffffLL || r < -0x7fffffffLL) return "rows and row strides must be below 2^31";
     if (!(c->eps_after >= 0) || !(c->eps_before >= 0)) return "eps must not be negative";
     return nullptr;
 }

@@ -25,7 +25,6 @@ __device__ __forceinline__ int row_end(const int* lengths, int b, int len) {
     return n < 0 ? 0 : n > len ? len : n;
 }
 
-template <typename A> __device__ __forceinline__ A act(A pre, int silu) { return silu ? pre * logistic(pre) : pre; }
 template <typename A> __device__ __forceinline__ A act_slope(A pre, int silu) {
     if (!silu) return A(1);
     const A s = logistic(pre);
@@ -120,46 +119,55 @@ __global__ void __launch_bounds__(128) forward_kernel(T* __restrict__ y, T* stat
     T* ys = y + pl.b * a.y_batch;
     const T* first = state_in ? state_in + (long long)pl.b * keep * a.channels : nullptr;
     int t = pl.t0;
+    const int stop = pl.t1 < end ? pl.t1 : end;
     if (t < end) {
+        const T* xn = xs + (t + U) * a.x_row;
+        T* yt = ys + t * a.y_row;
         A w[W][V], bias[V], win[H + U][V];          /* win[j]: row t - H + j */
         load_taps<T, W, VEC>(w, bias, wt, bt, lane, a.width);
         Pack<T, V> next[U], early[H];
 #pragma unroll
         for (int j = 0; j < H; ++j) early[j] = j >= skip ? row_of(xs, first, t - H + j, end, lane, a) : zero_pack<T, V>();
 #pragma unroll
-        for (int k = 0; k < U; ++k) next[k] = lane.load(xs + (t + k) * a.x_row, t + k < pl.t1 && t + k < end);
+        for (int k = 0; k < U; ++k) next[k] = lane.load(xs + (t + k) * a.x_row, t + k < stop);
 #pragma unroll
         for (int j = 0; j < H; ++j)
 #pragma unroll
             for (int i = 0; i < V; ++i) win[j][i] = up(early[j].v[i]);
-        for (; t < pl.t1 && t < end; t += U) {
+        for (; t < stop; t += U) {
 #pragma unroll
             for (int k = 0; k < U; ++k)
 #pragma unroll
                 for (int i = 0; i < V; ++i) win[H + k][i] = up(next[k].v[i]);
 #pragma unroll
-            for (int k = 0; k < U; ++k) next[k] = lane.load(xs + (t + U + k) * a.x_row, t + U + k < pl.t1 && t + U + k < end);
+            for (int k = 0; k < U; ++k) next[k] = lane.load(xn + k * a.x_row, t + U + k < stop);
+            xn += U * a.x_row;
 #pragma unroll
             for (int k = 0; k < U; ++k) {
-                if (t + k >= pl.t1) break;
-                Pack<T, V> o;
+                if (t + k >= stop) break;
+                A o[V];
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     A pre = bias[i];
 #pragma unroll
                     for (int j = 0; j < W; ++j)
                         if (j >= skip) pre += w[j][i] * win[k + j][i];
-                    o.v[i] = down<T>(t + k < end ? act(pre, a.silu) : A(0));
+                    o[i] = pre;
                 }
-                lane.store(ys + (t + k) * a.y_row, o);
+                if (a.silu) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) o[i] *= logistic(o[i]);
+                }
+                lane.store(yt + k * a.y_row, store_form<T, V>(o));
             }
+            yt += U * a.y_row;
 #pragma unroll
             for (int j = 0; j < H; ++j)
 #pragma unroll
                 for (int i = 0; i < V; ++i) win[j][i] = win[j + U][i];
         }
     }
-    for (; t < pl.t1; ++t) lane.store(ys + t * a.y_row, zero_pack<T, V>());
+    for (t = pl.t0 > end ? pl.t0 : end; t < pl.t1; ++t) lane.store(ys + t * a.y_row, zero_pack<T, V>());
     if (state_out && pl.t0 == 0) {
         /* the last rows of xp, by the only run that reads the old state; all read before the first is written: state_out may be
          * state_in */
@@ -260,7 +268,6 @@ __global__ void __launch_bounds__(128) backward_kernel(T* dx, T* dstate_in, type
                 else if (pl.t0 == 0 && to_state && r >= -keep) to = to_state + (long long)(r + keep) * a.channels;
                 if (!to) continue;
                 const int from_end = r - (end - keep);              /* row of the final state that is this row of xp */
-                Pack<T, V> o;
                 A v[V];
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
@@ -279,9 +286,7 @@ __global__ void __launch_bounds__(128) backward_kernel(T* dx, T* dstate_in, type
 #pragma unroll
                     for (int i = 0; i < V; ++i) v[i] += up(have.v[i]);
                 }
-#pragma unroll
-                for (int i = 0; i < V; ++i) o.v[i] = down<T>(v[i]);
-                lane.store(to, o);
+                lane.store(to, store_form<T, V>(v));
             }
 #pragma unroll
             for (int j = 0; j < H; ++j)

@@ -90,16 +90,7 @@ template <int G, int M, int UNIT, typename A> __device__ __forceinline__ void su
     }
 }
 
-/* V values at p when `on`, else zeros, into shared memory; FAST: all of them exist and p is aligned, asynchronously */
-template <int BYTES> __device__ __forceinline__ void async_copy(void* to, const void* from, bool on) {
-    const unsigned dst = (unsigned)__cvta_generic_to_shared(to);
-    const int size = on ? BYTES : 0;            /* the rest of the BYTES is filled with zeros; nothing is read for 0 */
-    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(from), "r"(size) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(from), "n"(BYTES), "r"(size) : "memory");
-}
-__device__ __forceinline__ void async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
+/* V values at p, which is aligned for them, when `on`, else zeros: asynchronously into shared memory */
 template <typename T, int V> __device__ __forceinline__ void bring(Pack<T, V>* to, const T* p, bool on) {
     constexpr int BYTES = sizeof(T) * V, STEP = BYTES < 16 ? BYTES : 16;
 #pragma unroll
@@ -1191,8 +1182,11 @@ int forward_p(void* y, void* h_out, void* saved, const Operands& o, const void* 
     if (blocks > 0x7fffffffLL) return refuse("rp_selective_scan_ex", "too many sequences for one launch");
     A* chunk_h = reinterpret_cast<A*>(ws);
     A* chunk_s = chunk_h ? chunk_h + (long long)c->batch * a.chunks * c->channels * c->states : nullptr;
-    SEQ_CUDA(cudaFuncSetAttribute(forward_kernel<T, P, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ForwardShared<T, P, true>)));
-    SEQ_CUDA(cudaFuncSetAttribute(forward_kernel<T, P, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(ForwardShared<T, P, false>)));
+    static unsigned char done[2][64];
+    int device = 0;
+    SEQ_CUDA(cudaGetDevice(&device));
+    if (allow_shared(forward_kernel<T, P, true>, sizeof(ForwardShared<T, P, true>), device, done[0]) ||
+        allow_shared(forward_kernel<T, P, false>, sizeof(ForwardShared<T, P, false>), device, done[1])) return -1;
     if (a.chunks > 1) {
         SEQ_CUDA(rpb_launch(forward_kernel<T, P, true>, dim3((unsigned)blocks), dim3(NT + Forward<T, P>::NL), sizeof(ForwardShared<T, P, true>), s, 1, reinterpret_cast<T*>(y), ho, reinterpret_cast<A*>(saved),
                             chunk_h, chunk_s, x, dt, Am, B, C, Dv, bias, z, hi, o.lengths, a));
@@ -1243,12 +1237,18 @@ int backward_p(const Wanted& w, const void* dy, const void* dh_out, const Operan
     out.vec_part = c->states % S == 0 && reinterpret_cast<uintptr_t>(part_b) % 16 == 0 && reinterpret_cast<uintptr_t>(part_c) % 16 == 0;
     a.fast = a.vec_x && a.vec_dt && (!z || a.vec_z) && a.vec_y && quads_ok<T>(c, r.B) && quads_ok<T>(c, r.C);
     const size_t agg = sizeof(BackwardShared<T, P, true>), smem = sizeof(BackwardShared<T, P, false>);
-    SEQ_CUDA(cudaFuncSetAttribute(backward_kernel<T, P, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)agg));
-    SEQ_CUDA(cudaFuncSetAttribute(backward_kernel<T, P, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    static unsigned char done[2][64];
+    int device = 0;
+    SEQ_CUDA(cudaGetDevice(&device));
+    if (allow_shared(backward_kernel<T, P, true>, agg, device, done[0]) || allow_shared(backward_kernel<T, P, false>, smem, device, done[1])) return -1;
     if (Sh::UNEVEN) {
-        cudaFuncAttributes attr;
-        SEQ_CUDA(cudaFuncGetAttributes(&attr, backward_kernel<T, P, false>));
-        if (attr.numRegs != 128) return refuse("rp_selective_scan_grad_ex", "built with another number of registers than its kernel divides");
+        static int registers = 0;       /* the same on every device */
+        if (registers == 0) {
+            cudaFuncAttributes attr;
+            SEQ_CUDA(cudaFuncGetAttributes(&attr, backward_kernel<T, P, false>));
+            registers = attr.numRegs;
+        }
+        if (registers != 128) return refuse("rp_selective_scan_grad_ex", "built with another number of registers than its kernel divides");
     }
     const A* dho = reinterpret_cast<const A*>(dh_out);
     const A* sv = reinterpret_cast<const A*>(saved);

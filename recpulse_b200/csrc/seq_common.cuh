@@ -49,6 +49,30 @@ template <typename T, int V> __device__ __forceinline__ Pack<T, V> zero_pack() {
     return p;
 }
 
+/* V sums rounded to the stored type, two at a time where the type is half as wide */
+template <typename T, int V, typename A> __device__ __forceinline__ Pack<T, V> narrow(const A (&v)[V]) {
+    Pack<T, V> p;
+#pragma unroll
+    for (int i = 0; i < V; ++i) p.v[i] = down<T>(v[i]);
+    return p;
+}
+template <int V> __device__ __forceinline__ Pack<__nv_bfloat16, V> narrow_pairs(const float (&v)[V], __nv_bfloat16) {
+    Pack<__nv_bfloat16, V> p;
+#pragma unroll
+    for (int i = 0; i < V; i += 2) *reinterpret_cast<__nv_bfloat162*>(&p.v[i]) = __floats2bfloat162_rn(v[i], v[i + 1]);
+    return p;
+}
+template <int V> __device__ __forceinline__ Pack<__half, V> narrow_pairs(const float (&v)[V], __half) {
+    Pack<__half, V> p;
+#pragma unroll
+    for (int i = 0; i < V; i += 2) *reinterpret_cast<__half2*>(&p.v[i]) = __floats2half2_rn(v[i], v[i + 1]);
+    return p;
+}
+template <typename T, int V, typename A> __device__ __forceinline__ Pack<T, V> store_form(const A (&v)[V]) {
+    if constexpr (sizeof(T) == 2 && V % 2 == 0) return narrow_pairs<V>(v, T());
+    else return narrow<T, V>(v);
+}
+
 /* Reads `valid` (<= V, may be <= 0) channels at p, zeros behind them; `vec`: p is aligned for the whole pack. */
 template <typename T, int V> __device__ __forceinline__ Pack<T, V> load_pack(const T* p, int valid, bool vec) {
     if (vec && valid >= V) return *reinterpret_cast<const Pack<T, V>*>(p);
@@ -144,6 +168,17 @@ template <int V> __device__ __forceinline__ void softplus_all(float (&v)[V]) {
     }
 }
 
+/* Asynchronous copies into shared memory: the first `size` of BYTES bytes (nothing is read for 0), zeros for the rest. */
+template <int BYTES> __device__ __forceinline__ void async_copy_part(void* to, const void* from, int size) {
+    const unsigned dst = (unsigned)__cvta_generic_to_shared(to);
+    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(from), "r"(size) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(from), "n"(BYTES), "r"(size) : "memory");
+}
+template <int BYTES> __device__ __forceinline__ void async_copy(void* to, const void* from, bool on) { async_copy_part<BYTES>(to, from, on ? BYTES : 0); }
+__device__ __forceinline__ void async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+
 /* Runs a call on the tensors' device and gives the caller's current device back. */
 struct DeviceScope {
     int prev = -1; bool moved = false;
@@ -154,6 +189,14 @@ struct DeviceScope {
     }
     ~DeviceScope() { if (moved) cudaSetDevice(prev); }
 };
+
+/* Lets a kernel use `bytes` of dynamic shared memory on the current device; the driver is asked once per kernel and device. */
+template <typename K> int allow_shared(K kernel, size_t bytes, int device, unsigned char (&done)[64]) {
+    if (bytes <= 40 * 1024 || (device < 64 && done[device])) return 0;
+    SEQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024));
+    if (device < 64) done[device] = 1;
+    return 0;
+}
 
 inline int refuse(const char* what, const char* why) {
     fprintf(stderr, "recpulse_b200: %s: %s\n", what, why);
