@@ -267,6 +267,7 @@ __global__ void __launch_bounds__(256) sum_parts_kernel(PartSums d, const typena
     A s = 0;
     if (col < d.cols[k]) {
         const A* p = parts + d.first[k] + col;
+#pragma unroll 8
         for (int i = ty; i < n_parts; i += 8) s += p[i * part_stride];
     }
     sums[ty][tx] = s;
