@@ -470,6 +470,10 @@ template <typename T> bool packs_of(const RpbBlockNorm* c, const Operand* o, int
     }
     int k = 1;
     while (c->rows > 1 && o[0].row * k % V != 0) k *= 2;
+    /* rows off the boundaries: their first pack reaches up to V - 1 channels in front of the row, which the row before must hold */
+    if (k > 1 || at != 0)
+        for (int i = 0; i < n; ++i)
+            if (o[i].p && c->rows > 1 && o[i].row < V) return false;
     *classes = k;
     return true;
 }

@@ -427,6 +427,7 @@ const char* bad_geometry(const RpbCausalConv* c, DType dtype) {
     if (!c) return "no geometry";
     if (!rpb_dtype_size((int)dtype)) return "unknown element type";
     if (c->batch <= 0 || c->len <= 0 || c->channels <= 0) return "batch, len and channels must be positive";
+    if (c->batch > 1 << 30 || c->len > 1 << 30 || c->channels > 1 << 24) return "batch or len above 2^30, or channels above 2^24";
     if (c->width < 1 || c->width > 8) return "width must be 1 to 8";
     if (c->activation != 0 && c->activation != 1) return "activation must be 0 (none) or 1 (SiLU)";
     return nullptr;

@@ -1089,6 +1089,7 @@ const char* bad_geometry(const RpbScan* c, DType dtype) {
     if (!c) return "no geometry";
     if (!rpb_dtype_size((int)dtype)) return "unknown element type";
     if (c->batch <= 0 || c->len <= 0 || c->channels <= 0) return "batch, len and channels must be positive";
+    if (c->batch > 1 << 30 || c->len > 1 << 30 || c->channels > 1 << 24) return "batch or len above 2^30, or channels above 2^24";
     if (c->states < 1 || c->states > MAX_STATES) return "states must be 1 to 64";
     if (c->groups < 1 || c->channels % c->groups != 0) return "groups must divide the channels";
     if (c->softplus != 0 && c->softplus != 1) return "softplus must be 0 or 1";

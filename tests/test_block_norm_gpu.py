@@ -175,6 +175,23 @@ def test_y_alone_is_a_plain_norm(lib):
     assert wide[:, 0].isnan().all() and wide[:, 51:].isnan().all()
 
 
+@pytest.mark.parametrize("d", [40, 37])
+@pytest.mark.parametrize("shift", [0, 3])
+def test_one_row_for_all(lib, d, shift):
+    """A row stride of 0 (one residual row under every row), at an offset from a boundary: nothing in front of it is read."""
+    s = make(12, d, "bfloat16", 5)
+    memory = torch.full((shift + d,), float("inf"), dtype=torch.bfloat16, device="cuda")
+    memory[shift:] = s["r"][0]
+    s["r"] = memory[shift:].expand(12, d)
+    s["u"], s["z"] = s["u"].contiguous(), s["z"].contiguous()
+    check(lib, s, "bfloat16", f"one row {d} {shift}")
+    first = torch.full((shift + 12 * d,), float("nan"), dtype=torch.bfloat16, device="cuda")
+    first[shift:] = s["u"].reshape(-1)
+    s = make(12, d, "bfloat16", 5, ("z", "r"))
+    s["u"] = first[shift:].view(12, d)
+    check(lib, s, "bfloat16", f"offset rows {d} {shift}")
+
+
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
 def test_accumulates_and_leaves_out(lib, dtype):
     s = make(19, 136, dtype, 6)

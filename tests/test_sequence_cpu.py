@@ -28,7 +28,7 @@ def test_packed_convolution_geometry():
 
 
 @pytest.mark.parametrize("wrong", [dict(batch=0), dict(length=0), dict(length=-1), dict(channels=0), dict(width=0), dict(width=9),
-                                   dict(activation=2), dict(x_row=7), dict(y_row=7), dict(y_batch=39), dict(x_batch=-40), dict(y_batch=0)])
+                                   dict(activation=2), dict(batch=(1 << 30) + 1), dict(length=(1 << 30) + 1), dict(channels=(1 << 24) + 1), dict(x_row=7), dict(y_row=7), dict(y_batch=39), dict(x_batch=-40), dict(y_batch=0)])
 def test_convolution_refuses_bad_geometry(wrong):
     lib = rpb.load()
     c = conv(**wrong)
@@ -76,7 +76,7 @@ def test_packed_scan_geometry_and_sizes():
 
 
 @pytest.mark.parametrize("wrong", [dict(batch=0), dict(length=0), dict(channels=0), dict(states=0), dict(states=65), dict(groups=0), dict(groups=3),
-                                   dict(softplus=2), dict(x_row=7), dict(dt_row=1), dict(b_row=7), dict(c_row=7), dict(z_row=7), dict(y_row=7),
+                                   dict(softplus=2), dict(batch=(1 << 30) + 1), dict(length=(1 << 30) + 1), dict(channels=(1 << 24) + 2), dict(x_row=7), dict(dt_row=1), dict(b_row=7), dict(c_row=7), dict(z_row=7), dict(y_row=7),
                                    dict(y_batch=39), dict(x_batch=-1)])
 def test_scan_refuses_bad_geometry(wrong):
     lib, c = rpb.load(), scan(**wrong)
@@ -126,7 +126,7 @@ def norm(rows=4, channels=8, eps=1e-5, **over):
 
 
 @pytest.mark.parametrize("wrong", [dict(rows=0), dict(channels=0), dict(channels=8193), dict(eps=-1.0), dict(eps=float("nan")), dict(out_row=7),
-                                   dict(y_row=-8), dict(u_row=-1), dict(r_row=-1)])
+                                   dict(y_row=-8), dict(u_row=-1), dict(r_row=-1), dict(rows=1 << 31), dict(u_row=1 << 31)])
 def test_norm_refuses_bad_geometry(wrong):
     lib, c = rpb.load(), norm(**wrong)
     a = [at(2048 * i) for i in range(6)]
