@@ -103,14 +103,16 @@ __device__ __forceinline__ Pack<T, Width<T>::v> row_of(const T* x, const T* stat
     return lane.load(state + (long long)s * a.channels, state && s >= 0);
 }
 
-constexpr int U = 4;        /* rows at a time, the next ones' values on their way meanwhile */
+/* rows at a time, the next ones' values on their way meanwhile: 4 forward (2: 79 us instead of 71 at 4 x 4096 x 4096 bf16, 8: 103),
+ * 2 backward (forward and backward of 3 x 1999 x 1531 f16: 56 us instead of 73, by its registers) */
+constexpr int FORWARD_ROWS = 4, BACKWARD_ROWS = 2;
 
 /* The last W - 1 rows of x are kept in registers, so that x is read once but for W - 1 rows in front of each run. */
 template <typename T, int W, bool VEC>
 __global__ void __launch_bounds__(128) forward_kernel(T* __restrict__ y, T* state_out, const T* __restrict__ x, const T* __restrict__ wt,
                                                       const T* __restrict__ bt, const T* state_in, const int* __restrict__ lengths, Args a) {
     typedef typename AccOf<T>::type A;
-    constexpr int V = Width<T>::v, H = W - 1;
+    constexpr int V = Width<T>::v, H = W - 1, U = FORWARD_ROWS;
     rpb_pdl_trigger();
     rpb_pdl_wait();
     const Place<T, VEC> pl(a);
@@ -193,7 +195,7 @@ __global__ void __launch_bounds__(128) backward_kernel(T* dx, T* dstate_in, type
                                                        const T* __restrict__ wt, const T* __restrict__ bt, const T* __restrict__ state_in,
                                                        const int* __restrict__ lengths, Args a) {
     typedef typename AccOf<T>::type A;
-    constexpr int V = Width<T>::v, H = W - 1;
+    constexpr int V = Width<T>::v, H = W - 1, U = BACKWARD_ROWS;
     __shared__ A red[4][W + 1][32 * V + 1];
     rpb_pdl_trigger();
     rpb_pdl_wait();
@@ -321,7 +323,8 @@ __global__ void __launch_bounds__(128) backward_kernel(T* dx, T* dstate_in, type
 }
 
 /* Rows per thread.  A run costs W - 1 (backward: 2 (W - 1)) rows of extra reading, which the longest run makes
- * cheapest; it is halved while the runs do not fill the chip with `warps` warps.  At least 8, so that only the first run of
+ * cheapest; it is halved while the runs do not fill the chip with `warps` warps (16 per SM
+ * forward; 8 backward, whose runs cost twice as much: 52 us instead of 56 at 3 x 1999 x 1531).  At least 8, so that only the first run of
  * a sequence reaches back to the state. */
 int pick_run(long long batch, int len, long long n_vec, int longest, int warps) {
     int run = longest;
@@ -330,7 +333,7 @@ int pick_run(long long batch, int len, long long n_vec, int longest, int warps) 
 }
 
 template <typename T> int backward_run(const RpbCausalConv* c) {
-    return pick_run(c->batch, c->len, (c->channels + Width<T>::v - 1) / Width<T>::v, 64, SM_COUNT * 16);
+    return pick_run(c->batch, c->len, (c->channels + Width<T>::v - 1) / Width<T>::v, 64, SM_COUNT * 8);
 }
 template <typename T> long long backward_groups(const RpbCausalConv* c) {
     const int run = backward_run<T>(c);
@@ -362,7 +365,7 @@ template <typename T> Args make_args(const RpbCausalConv* c, int run) {
 template <typename T, int W, bool VEC>
 int forward_w(void* y, void* state_out, const void* x, const void* w, const void* bias, const void* state_in, const int* lengths,
               const RpbCausalConv* c, cudaStream_t s) {
-    const Args a = make_args<T>(c, pick_run(c->batch, c->len, (c->channels + Width<T>::v - 1) / Width<T>::v, 32, SM_COUNT * 16));
+    const Args a = make_args<T>(c, pick_run(c->batch, c->len, (c->channels + Width<T>::v - 1) / Width<T>::v, 64, SM_COUNT * 16));
     const long long warps = (long long)c->batch * a.runs * a.vec_blocks;
     const int per = warps < SM_COUNT * 4 ? 1 : 4;                  /* few warps: one per block, on more SMs */
     const long long blocks = ((long long)c->batch * a.runs + per - 1) / per * a.vec_blocks;
