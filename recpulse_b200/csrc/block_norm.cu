@@ -113,6 +113,16 @@ template <typename T, int NV, bool PACKS> struct Span {
             if (has(k, i)) p.v[i] = row[channel(k, i)];
         return p;
     }
+    /* The thread's channels of a weight: packs lie on boundaries of the row, which need not be boundaries of the weight. */
+    __device__ __forceinline__ Pack<T, V> load_weight(const T* w, int k) const {
+        if (PACKS && mask[k] == ALL && reinterpret_cast<uintptr_t>(w + channel(k, 0)) % 16 == 0)
+            return *reinterpret_cast<const Pack<T, V>*>(w + channel(k, 0));
+        Pack<T, V> p = zero_pack<T, V>();
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (has(k, i)) p.v[i] = w[channel(k, i)];
+        return p;
+    }
     __device__ __forceinline__ void store(T* row, int k, const Pack<T, V>& p) const {
         if (PACKS && mask[k] == ALL) { *reinterpret_cast<Pack<T, V>*>(row + channel(k, 0)) = p; return; }
         if (PACKS && mask[k] == 0) return;
@@ -187,7 +197,7 @@ forward_kernel(T* __restrict__ out, T* __restrict__ y, const T* __restrict__ u, 
         const Pack<T, V>* from = ring + slot * 3 * per;
         const T* rows[3] = {u + (long long)(int)row * a.u_row, z + (long long)(int)row * a.z_row, r + (long long)(int)row * a.r_row};
         auto take = [&](int n, int k) { return SLOTS ? span.take(from + n * per, k) : span.load_one(rows[n], k); };
-        auto weight = [&](int n, const T* w, int k) { return SLOTS ? ws[n * per + k * nt + tid] : w ? span.load_one(w, k) : zero_pack<T, V>(); };
+        auto weight = [&](int n, const T* w, int k) { return SLOTS ? ws[n * per + k * nt + tid] : w ? span.load_weight(w, k) : zero_pack<T, V>(); };
         A o[NV][V], sq[1] = {0};
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
@@ -289,7 +299,7 @@ backward_kernel(T* du, T* dz, T* dr, typename AccOf<T>::type* __restrict__ parts
         const Pack<T, V>* from = ring + slot * 5 * per;
         const T* rows[5] = {u + (long long)(int)row * a.u_row, z + (long long)(int)row * a.z_row, r + (long long)(int)row * a.r_row, dout + (long long)(int)row * a.out_row, dy + (long long)(int)row * a.y_row};
         auto take = [&](int n, int k) { return SLOTS ? span.take(from + n * per, k) : span.load_one(rows[n], k); };
-        auto weight = [&](int n, const T* w, int k) { return SLOTS ? ws[n * per + k * nt + tid] : w ? span.load_one(w, k) : zero_pack<T, V>(); };
+        auto weight = [&](int n, const T* w, int k) { return SLOTS ? ws[n * per + k * nt + tid] : w ? span.load_weight(w, k) : zero_pack<T, V>(); };
         A v[NV][V], total[NV][V], sq[2] = {0, 0};
 #pragma unroll
         for (int k = 0; k < NV; ++k) {

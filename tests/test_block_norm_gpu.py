@@ -246,3 +246,17 @@ def test_replayed_from_a_graph_on_another_stream(lib):
         ref = reference(s, dtype)
         for k, v in got.items():
             close(v, ref[k], ref[k + "_slack"], k)
+
+
+@pytest.mark.parametrize("dtype,rows,d", [("float32", 5, 4093), ("float32", 5, 8191), ("float64", 5, 2047), ("float64", 3, 8189), ("float16", 9, 8191),
+                                          ("bfloat16", 9, 8187), ("float32", 3, 8192), ("float64", 2, 8192), ("bfloat16", 3, 8192)])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_wide_rows_and_their_weights(lib, dtype, rows, d, shift):
+    """Packed operands with rows too wide for shared memory: rows that begin off a 16-byte boundary meet weights that lie on one,
+    and (shift) weights that begin off one meet rows that do not."""
+    s = {k: v.contiguous() for k, v in make(rows, d, dtype, rows + d).items()}
+    for k in ("w_after", "scale", "w_before"):
+        memory = torch.full((shift + d,), float("nan"), dtype=s[k].dtype, device="cuda")
+        memory[shift:] = s[k]
+        s[k] = memory[shift:]
+    check(lib, s, dtype, f"{dtype} {rows}x{d} weights {shift} off")
