@@ -254,14 +254,18 @@ void backward_selective_scan_fn(GradFn* self, Tensor* grad_output) {
 
 /* ------------------------------------------------------------------ norms around a block */
 
-/* rows of the last dimension at one distance from each other: that distance, or -1 */
+/* rows of the last dimension at one distance from each other: that distance, or -1.  Dimensions of size 1 have no say. */
 static long long row_stride(const Tensor* t) {
     const int n = t->ndim;
     if (t->shape[n - 1] > 1 && t->strides[n - 1] != 1) return -1;
-    if (n == 1) return t->shape[0];
-    for (int d = 0; d + 2 < n; d++)
-        if (t->shape[d] > 1 && (long long)t->strides[d] != (long long)t->strides[d + 1] * t->shape[d + 1]) return -1;
-    return t->strides[n - 2] < 0 ? -1 : t->strides[n - 2];
+    long long stride = t->shape[n - 1], rows = 1;       /* rows: of the dimensions behind d, which lie `stride` apart */
+    for (int d = n - 2; d >= 0; d--) {
+        if (t->shape[d] == 1) continue;
+        if (rows == 1) stride = t->strides[d];
+        else if (t->strides[d] != stride * rows) return -1;
+        rows *= t->shape[d];
+    }
+    return stride < 0 ? -1 : stride;
 }
 static bool like(const Tensor* t, const Tensor* x) {
     if (t->ndim != x->ndim || t->dtype != x->dtype || t->device_id != x->device_id || row_stride(t) < 0) return false;

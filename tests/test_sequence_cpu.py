@@ -153,3 +153,24 @@ def test_norm_refuses_bad_calls():
     assert grad(dz=free, z=None) == -1 and grad(dw_after=free, wa=None) == -1 and grad(dscale=free, sc=None) == -1
     assert grad(dw_before=free, dy=None) == -1 and grad(dw_before=free, ws=None) == -1
     assert grad(du=u) == -1 and grad(dr=at(13000)) == -1 and grad(du=free, dr=free) == -1
+
+
+def tensor(shape, strides, dtype=rpb.F32, data=None):
+    """A Tensor struct as RecPulse lays it out, on device 0, over memory that no test reaches."""
+    t = rpb._lib.CTensor()
+    t.dtype, t.ndim, t.device_id, t.refcount, t.size = dtype, len(shape), 0, 1, int(np.prod(shape))
+    t.shape, t.strides = (C.c_int * len(shape))(*shape), (C.c_int * len(strides))(*strides)
+    t.data = data if data is not None else BUF.ctypes.data
+    return t
+
+
+@pytest.mark.parametrize("shape,strides", [((4, 1, 5, 8), (80, 80, 8, 1)), ((4, 5, 1, 8), (80, 8, 8, 1)), ((4, 5, 8), (80, 8, 1)), ((3, 1, 4, 1, 8), (32, 0, 16, 8, 1)),
+                                           ((4, 5, 8), (8, 0, 1)), ((2, 8), (8, 2)), ((2, 8), (-8, 1))])
+def test_norm_nodes_refuse_rows_at_several_distances(shape, strides, capfd):
+    lib = rpb.load()
+    u, w = tensor(shape, strides), tensor((8,), (1,))
+    good = tensor(shape, tuple(int(np.prod(shape[d + 1:])) for d in range(len(shape))))
+    assert not lib.op_rms_norm(C.byref(u), C.byref(w), 1e-5)
+    assert not lib.op_gated_norm(C.byref(u), None, C.byref(w), None, None, 1e-5)
+    assert not lib.op_gated_norm(C.byref(good), None, C.byref(w), None, C.byref(u), 1e-5)
+    assert capfd.readouterr().err.count("rows at one distance") == 3

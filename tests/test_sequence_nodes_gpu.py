@@ -272,3 +272,29 @@ def test_a_block_replayed_from_a_graph(lib):
         assert rel(f64(o.to_numpy(), dtype), want.detach().numpy()) <= TOL[dtype], trial
         for got, l in zip(grads, ls):
             assert rel(f64(got.to_numpy(), dtype), l.grad.numpy()) <= TOL[dtype], trial
+
+
+@pytest.mark.parametrize("shape,strides", [((4, 1, 8), (40, 8, 1)), ((4, 1, 5, 8), (40, 3, 8, 1)), ((1, 5, 8), (7, 8, 1)), ((2, 3, 1, 8), (48, 16, 1, 1)),
+                                           ((1, 1, 8), (3, 5, 1)), ((4, 5, 8), (0, 0, 1))])
+def test_norm_nodes_take_rows_at_one_distance(lib, shape, strides):
+    """Dimensions of size 1 may have any stride; the upstream gradient likewise."""
+    rng = np.random.default_rng(11)
+    dtype, size = "float32", 1 + sum((n - 1) * s for n, s in zip(shape, strides))
+    base, w = rand_operand(rng, (size,), dtype), rand_operand(rng, (8,), dtype)
+    cut = lambda a: np.lib.stride_tricks.as_strided(a, shape, [4 * s for s in strides])       # noqa: E731
+    u, lu = T(base, dtype, True).as_strided(shape, strides), leaf(f64(cut(base), dtype).copy())
+    W, lw = T(w, dtype, True), leaf(f64(w, dtype))
+    node, value = u.op_rms_norm(W, EPS), norm64(lu, None, lw, None, None)
+    g = rand_operand(rng, (size,), dtype)
+    assert rel(f64(node.to_numpy(), dtype), value.detach().numpy()) <= TOL[dtype]
+    node.backward(T(g, dtype).as_strided(shape, strides))
+    value.backward(torch.tensor(f64(cut(g), dtype).copy()))
+    assert rel(f64(u.grad.to_numpy(), dtype), lu.grad.numpy()) <= TOL[dtype]
+    assert rel(f64(W.grad.to_numpy(), dtype), lw.grad.numpy()) <= TOL[dtype]
+
+
+def test_norm_nodes_refuse_rows_at_several_distances(lib):
+    rng = np.random.default_rng(12)
+    base, w = T(rand_operand(rng, (4, 1, 10, 8), "float32"), "float32"), T(rand_operand(rng, (8,), "float32"), "float32")
+    with pytest.raises(RuntimeError):
+        base.as_strided((4, 1, 5, 8), (80, 80, 8, 1)).op_rms_norm(w)
