@@ -30,6 +30,12 @@ static Tensor* refused(const char* op, const char* why) {
     return NULL;
 }
 
+static bool empty(const Tensor* t) {
+    for (int d = 0; t && d < t->ndim; d++)
+        if (t->shape[d] <= 0) return true;
+    return false;
+}
+
 /* [batch, len, cols] with unit stride within a row, on x's device and of its type */
 static bool sequence_ok(const Tensor* t, const Tensor* x, int cols) {
     return t && t->ndim == 3 && t->dtype == x->dtype && t->device_id == x->device_id && t->shape[0] == x->shape[0] && t->shape[1] == x->shape[1] &&
@@ -99,6 +105,7 @@ Tensor* op_causal_conv(Tensor* x, Tensor* w, Tensor* bias, int activation) {
     const char* op = "op_causal_conv";
     if (!x || !w || x->ndim != 3 || w->ndim != 2) return NULL;
     if (x->device_id < 0) return refused(op, "host tensors: this library has no CPU path");
+    if (empty(x) || empty(w)) return refused(op, "a dimension of size 0");
     if (!sequence_ok(x, x, x->shape[2]) || w->shape[0] != x->shape[2]) return refused(op, "x is [batch, len, channels], w [channels, width]");
     if (!vector_ok(w, x->dtype, x->device_id, (long long)w->shape[0] * w->shape[1])) return refused(op, "w must be packed, of x's type and device");
     if (bias && !vector_ok(bias, x->dtype, x->device_id, x->shape[2])) return refused(op, "bias must be packed, of x's type and device");
@@ -166,6 +173,7 @@ Tensor* op_selective_scan(Tensor* x, Tensor* dt, Tensor* A, Tensor* B, Tensor* C
     const char* op = "op_selective_scan";
     if (!x || !dt || !A || !B || !C || x->ndim != 3 || A->ndim != 2 || B->ndim != 3) return NULL;
     if (x->device_id < 0) return refused(op, "host tensors: this library has no CPU path");
+    if (empty(x) || empty(A) || empty(B)) return refused(op, "a dimension of size 0");
     const int channels = x->shape[2], states = A->shape[1], cols = B->shape[2];
     const DType acc = x->dtype == DTYPE_FLOAT64 ? DTYPE_FLOAT64 : DTYPE_FLOAT32;
     if (!sequence_ok(x, x, channels) || !sequence_ok(dt, x, channels) || (z && !sequence_ok(z, x, channels)))
@@ -287,6 +295,7 @@ static int norm_geometry(RpbBlockNorm* c, const Tensor* u, const Tensor* z, cons
 static Tensor* norm_node(const char* op, Tensor* u, Tensor* z, Tensor* w, Tensor* scale, Tensor* r, float eps, int before) {
     if (!u || u->ndim < 1) return NULL;
     if (u->device_id < 0) return refused(op, "host tensors: this library has no CPU path");
+    if (empty(u)) return refused(op, "a dimension of size 0");
     const int d = u->shape[u->ndim - 1];
     if (row_stride(u) < 0 || (z && !like(z, u)) || (r && !like(r, u))) return refused(op, "u, z and r have one shape and type, and rows at one distance");
     if ((w && !vector_ok(w, u->dtype, u->device_id, d)) || (scale && !vector_ok(scale, u->dtype, u->device_id, d)))

@@ -174,3 +174,20 @@ def test_norm_nodes_refuse_rows_at_several_distances(shape, strides, capfd):
     assert not lib.op_gated_norm(C.byref(u), None, C.byref(w), None, None, 1e-5)
     assert not lib.op_gated_norm(C.byref(good), None, C.byref(w), None, C.byref(u), 1e-5)
     assert capfd.readouterr().err.count("rows at one distance") == 3
+
+
+def test_nodes_refuse_empty_dimensions(capfd):
+    """A Tensor with no elements (RecPulse's own can be had) is refused, not divided by."""
+    lib = rpb.load()
+    x, empty = tensor((2, 5, 8), (40, 8, 1)), tensor((2, 5, 0), (0, 0, 1))
+    A, w = tensor((8, 4), (4, 1)), tensor((8,), (1,))
+    none = tensor((8, 0), (0, 1))
+    by = C.byref
+    assert not lib.op_selective_scan(by(x), by(x), by(none), by(x), by(x), None, None, None, 1)
+    assert not lib.op_selective_scan(by(x), by(x), by(A), by(empty), by(empty), None, None, None, 1)
+    assert not lib.op_selective_scan(by(empty), by(empty), by(none), by(x), by(x), None, None, None, 1)
+    for t in (empty, tensor((0, 8), (8, 1)), tensor((0,), (1,))):
+        assert not lib.op_rms_norm(by(t), by(w), 1e-5) and not lib.op_gated_norm(by(t), None, None, None, None, 1e-5)
+    assert not lib.op_causal_conv(by(empty), by(tensor((0, 4), (4, 1))), None, 1)
+    assert not lib.op_causal_conv(by(x), by(none), None, 1)
+    assert "cudaMalloc" not in capfd.readouterr().err
