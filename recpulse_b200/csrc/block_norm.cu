@@ -589,11 +589,8 @@ const char* bad_geometry(const RpbBlockNorm* c, DType dtype) {
 }
 bool readable_rows(const RpbBlockNorm* c, const void* p, long long row) { return !p || c->rows == 1 || row >= 0; }
 bool writable_rows(const RpbBlockNorm* c, const void* p, long long row) { return !p || c->rows == 1 || row >= c->channels; }
-/* whether rows of two operands meet */
-bool meet(const RpbBlockNorm* c, const void* p, long long p_row, const void* q, long long q_row, size_t es) {
-    if (!p || !q) return false;
-    const long long rows = c->rows < 0x7fffffffLL ? c->rows : 0x7fffffffLL;
-    return overlaps({p, 0, p_row, c->channels}, {q, 0, q_row, c->channels}, 1, (int)rows, es);
+Area row_area(const RpbBlockNorm* c, const char* name, const void* p, long long row, size_t es) {
+    return strided(name, {p, 0, row, c->channels}, 1, (int)c->rows, es);
 }
 
 }  // namespace rpb_norm
@@ -621,10 +618,11 @@ int rp_block_norm_ex(void* out, void* y, const void* u, const void* z, const voi
     if (!readable_rows(c, u, c->u_row) || !readable_rows(c, z, c->z_row) || !readable_rows(c, r, c->r_row)) return refuse(name, "strides of an operand");
     if (!writable_rows(c, out, c->out_row) || !writable_rows(c, y, c->y_row)) return refuse(name, "strides of out or y");
     const size_t es = rpb_dtype_size((int)dtype);
-    const Rows ins[3] = {{u, 0, c->u_row, 0}, {z, 0, c->z_row, 0}, {r, 0, c->r_row, 0}};
-    for (const Rows& i : ins)
-        if (meet(c, out, c->out_row, i.p, i.row, es) || meet(c, y, c->y_row, i.p, i.row, es)) return refuse(name, "out or y overlaps an operand");
-    if (meet(c, out, c->out_row, y, c->y_row, es)) return refuse(name, "out and y overlap");
+    const long long D = c->channels;
+    const Area outs[] = {row_area(c, "out", out, c->out_row, es), row_area(c, "y", y, c->y_row, es)};
+    const Area ins[] = {row_area(c, "u", u, c->u_row, es), row_area(c, "z", z, c->z_row, es), row_area(c, "r", r, c->r_row, es),
+                        packed("w_after", w_after, D, es), packed("scale", scale, D, es), packed("w_before", w_before, D, es)};
+    if (refuse_overlaps(name, outs, ins)) return -1;
     DeviceScope scope;
     if (scope.enter(device_id)) return refuse(name, "no such device");
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
@@ -657,18 +655,20 @@ int rp_block_norm_grad_ex(void* du, void* dz, void* dr, void* dw_after, void* ds
     if ((dz && !z) || (dw_after && !w_after) || (dscale && !scale) || (dw_before && !dy)) return refuse(name, "a gradient of an operand that is not given");
     if ((dw_after || dscale || dw_before) && !ws) return refuse(name, "the weights' gradients need a workspace");
     if (device_id < 0) return refuse(name, "needs a CUDA device (no CPU path in this library)");
-    const Rows ins[5] = {{u, 0, c->u_row, 0}, {z, 0, c->z_row, 0}, {r, 0, c->r_row, 0}, {dout, 0, c->out_row, 0}, {dy, 0, c->y_row, 0}};
-    const Rows outs[3] = {{du, 0, c->du_row, 0}, {dz, 0, c->dz_row, 0}, {dr, 0, c->dr_row, 0}};
+    if (!readable_rows(c, u, c->u_row) || !readable_rows(c, z, c->z_row) || !readable_rows(c, r, c->r_row) || !readable_rows(c, dout, c->out_row) ||
+        !readable_rows(c, dy, c->y_row))
+        return refuse(name, "strides of an operand");
+    if (!writable_rows(c, du, c->du_row) || !writable_rows(c, dz, c->dz_row) || !writable_rows(c, dr, c->dr_row)) return refuse(name, "strides of a gradient");
     const size_t es = rpb_dtype_size((int)dtype);
-    for (const Rows& i : ins)
-        if (!readable_rows(c, i.p, i.row)) return refuse(name, "strides of an operand");
-    for (int k = 0; k < 3; ++k) {
-        if (!writable_rows(c, outs[k].p, outs[k].row)) return refuse(name, "strides of a gradient");
-        for (const Rows& i : ins)
-            if (meet(c, outs[k].p, outs[k].row, i.p, i.row, es)) return refuse(name, "a gradient overlaps an operand");
-        for (int j = 0; j < k; ++j)
-            if (meet(c, outs[k].p, outs[k].row, outs[j].p, outs[j].row, es)) return refuse(name, "two gradients overlap");
-    }
+    const long long D = c->channels;
+    const bool weights = dw_after || dscale || dw_before;
+    const Area outs[] = {row_area(c, "du", du, c->du_row, es), row_area(c, "dz", dz, c->dz_row, es), row_area(c, "dr", dr, c->dr_row, es),
+                         packed("dw_after", dw_after, D, es), packed("dscale", dscale, D, es), packed("dw_before", dw_before, D, es),
+                         packed("ws", weights ? ws : nullptr, weights ? rp_block_norm_ws_bytes(c, dtype) : 0, 1)};
+    const Area ins[] = {row_area(c, "u", u, c->u_row, es), row_area(c, "z", z, c->z_row, es), row_area(c, "r", r, c->r_row, es),
+                        row_area(c, "dout", dout, c->out_row, es), row_area(c, "dy", dy, c->y_row, es),
+                        packed("w_after", w_after, D, es), packed("scale", scale, D, es), packed("w_before", w_before, D, es)};
+    if (refuse_overlaps(name, outs, ins)) return -1;
     DeviceScope scope;
     if (scope.enter(device_id)) return refuse(name, "no such device");
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

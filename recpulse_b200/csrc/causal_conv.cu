@@ -344,6 +344,8 @@ Rows x_rows(const RpbCausalConv* c, const void* x) { return {x, c->x_batch, c->x
 Rows y_rows(const RpbCausalConv* c, const void* y) { return {y, c->y_batch, c->y_row, c->channels}; }
 Rows dx_rows(const RpbCausalConv* c, const void* dx) { return {dx, c->dx_batch, c->dx_row, c->channels}; }
 
+long long state_elems(const RpbCausalConv* c) { return (long long)c->batch * (c->width - 1) * c->channels; }
+
 /* Whether every row of an operand (a packed state: p, 0 strides) can be moved in packs. */
 template <typename T> bool packs_ok(const RpbCausalConv* c, const Rows& r) {
     return !r.p || aligned_rows(r, c->batch, c->len, sizeof(T), sizeof(T) * Width<T>::v);
@@ -464,7 +466,12 @@ int rp_causal_conv_ex(void* y, void* state_out, const void* x, const void* w, co
     const Rows rx = x_rows(c, x), ry = y_rows(c, y);
     if (!readable(rx, c->batch, c->len)) return refuse(name, "strides of x");
     if (!writable(ry, c->batch, c->len)) return refuse(name, "strides of y");
-    if (overlaps(ry, rx, c->batch, c->len, rpb_dtype_size((int)dtype))) return refuse(name, "y overlaps x");
+    const size_t es = rpb_dtype_size((int)dtype);
+    const long long kept = state_elems(c);
+    const Area outs[] = {strided("y", ry, c->batch, c->len, es), packed("state_out", state_out, kept, es, state_in)};
+    const Area ins[] = {strided("x", rx, c->batch, c->len, es), packed("w", w, (long long)c->channels * c->width, es), packed("bias", bias, c->channels, es),
+                        packed("state_in", state_in, kept, es), packed("lengths", lengths, c->batch, sizeof(int))};
+    if (refuse_overlaps(name, outs, ins)) return -1;
     DeviceScope scope;
     if (scope.enter(device_id)) return refuse(name, "no such device");
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
@@ -501,8 +508,14 @@ int rp_causal_conv_grad_ex(void* dx, void* dw, void* dbias, void* dstate_in, int
     if (!readable(rx, c->batch, c->len)) return refuse(name, "strides of x");
     if (!readable(rg, c->batch, c->len)) return refuse(name, "strides of dy");
     if (dx && !writable(rd, c->batch, c->len)) return refuse(name, "strides of dx");
-    if (overlaps(rd, rx, c->batch, c->len, es) || overlaps(rd, rg, c->batch, c->len, es)) return refuse(name, "dx overlaps x or dy");
-    if (dstate_in && (dstate_in == dstate_out || dstate_in == state_in)) return refuse(name, "dstate_in overlaps dstate_out or state_in");
+    const long long kept = state_elems(c), taps = (long long)c->channels * c->width;
+    const bool filter = dw || dbias;
+    const Area outs[] = {strided("dx", rd, c->batch, c->len, es), packed("dw", dw, taps, es), packed("dbias", dbias, c->channels, es),
+                         packed("dstate_in", dstate_in, kept, es), packed("ws", filter ? ws : nullptr, filter ? rp_causal_conv_ws_bytes(c, dtype) : 0, 1)};
+    const Area ins[] = {strided("dy", rg, c->batch, c->len, es), strided("x", rx, c->batch, c->len, es), packed("w", w, taps, es),
+                        packed("bias", bias, c->channels, es), packed("state_in", state_in, kept, es), packed("dstate_out", dstate_out, kept, es),
+                        packed("lengths", lengths, c->batch, sizeof(int))};
+    if (refuse_overlaps(name, outs, ins)) return -1;
     DeviceScope scope;
     if (scope.enter(device_id)) return refuse(name, "no such device");
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

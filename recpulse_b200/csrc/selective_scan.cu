@@ -1315,11 +1315,6 @@ const char* bad_operands(const RpbScan* c, const Rowset& r, const Operands& o, b
     return nullptr;
 }
 
-bool meets_any(const RpbScan* c, const Rows& w, const Rowset& r, size_t es, bool with_y) {
-    return overlaps(w, r.x, c->batch, c->len, es) || overlaps(w, r.dt, c->batch, c->len, es) || overlaps(w, r.B, c->batch, c->len, es) ||
-           overlaps(w, r.C, c->batch, c->len, es) || overlaps(w, r.z, c->batch, c->len, es) || (with_y && overlaps(w, r.y, c->batch, c->len, es));
-}
-
 }  // namespace rpb_scan
 
 using namespace rpb_seq;
@@ -1362,9 +1357,16 @@ int rp_selective_scan_ex(void* y, void* h_out, void* saved, const void* x, const
     why = bad_operands(c, r, o, z != nullptr);
     if (why) return refuse(name, why);
     if (!writable(r.y, c->batch, c->len)) return refuse(name, "strides of y");
-    if (meets_any(c, r.y, r, rpb_dtype_size((int)dtype), false)) return refuse(name, "y overlaps an operand");
-    if (!ws && rp_selective_scan_ws_bytes(c, dtype, 0) > 0) return refuse(name, "this size needs a workspace");
-    if (saved && (saved == h_in || saved == h_out || saved == ws)) return refuse(name, "saved overlaps another buffer");
+    const long long ws_bytes = rp_selective_scan_ws_bytes(c, dtype, 0), d = c->channels, all = (long long)c->batch * d * c->states;
+    if (!ws && ws_bytes > 0) return refuse(name, "this size needs a workspace");
+    const size_t es = rpb_dtype_size((int)dtype), as = dtype == DTYPE_FLOAT64 ? 8 : 4;
+    auto area = [&](const char* n, const Rows& rows) { return strided(n, rows, c->batch, c->len, es); };
+    const Area outs[] = {area("y", r.y), packed("h_out", h_out, all, as, h_in), packed("saved", saved, rp_selective_scan_saved_elems(c, dtype), as),
+                         packed("ws", ws, ws_bytes, 1)};
+    const Area ins[] = {area("x", r.x), area("dt", r.dt), area("B", r.B), area("C", r.C), area("z", r.z), packed("A", A, d * c->states, as),
+                        packed("D", D, d, as), packed("dt_bias", dt_bias, d, as), packed("h_in", h_in, all, as),
+                        packed("lengths", lengths, c->batch, sizeof(int))};
+    if (refuse_overlaps(name, outs, ins)) return -1;
     DeviceScope scope;
     if (scope.enter(device_id)) return refuse(name, "no such device");
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
@@ -1393,14 +1395,18 @@ int rp_selective_scan_grad_ex(void* dx, void* ddt, void* dA, void* dB, void* dC,
     const Rows w[5] = {{dx, c->dx_batch, c->dx_row, c->channels}, {ddt, c->ddt_batch, c->ddt_row, c->channels}, {dz, c->dz_batch, c->dz_row, c->channels},
                        {dB, c->db_batch, c->db_row, gn}, {dC, c->dc_batch, c->dc_row, gn}};
     const size_t es = rpb_dtype_size((int)dtype);
-    for (int i = 0; i < 5; ++i) {
-        if (!w[i].p) continue;
-        if (!writable(w[i], c->batch, c->len)) return refuse(name, "strides of a gradient");
-        if (meets_any(c, w[i], r, es, true)) return refuse(name, "a gradient overlaps an operand");
-        for (int k = 0; k < i; ++k)
-            if (overlaps(w[i], w[k], c->batch, c->len, es)) return refuse(name, "two gradients overlap");
-    }
-    if (dh_in && dh_in == dh_out) return refuse(name, "dh_in overlaps dh_out");
+    for (const Rows& g : w)
+        if (g.p && !writable(g, c->batch, c->len)) return refuse(name, "strides of a gradient");
+    const size_t as = dtype == DTYPE_FLOAT64 ? 8 : 4;
+    const long long d = c->channels, all = (long long)c->batch * d * c->states;
+    auto area = [&](const char* n, const Rows& rows) { return strided(n, rows, c->batch, c->len, es); };
+    const Area outs[] = {area("dx", w[0]), area("ddt", w[1]), area("dz", w[2]), area("dB", w[3]), area("dC", w[4]), packed("dA", dA, d * c->states, as),
+                         packed("dD", dD, d, as), packed("ddt_bias", ddt_bias, d, as), packed("dh_in", dh_in, all, as),
+                         packed("ws", ws, rp_selective_scan_ws_bytes(c, dtype, 1), 1)};
+    const Area ins[] = {area("dy", r.y), area("x", r.x), area("dt", r.dt), area("B", r.B), area("C", r.C), area("z", r.z),
+                        packed("A", A, d * c->states, as), packed("D", D, d, as), packed("dt_bias", dt_bias, d, as), packed("dh_out", dh_out, all, as),
+                        packed("saved", saved, rp_selective_scan_saved_elems(c, dtype), as), packed("lengths", lengths, c->batch, sizeof(int))};
+    if (refuse_overlaps(name, outs, ins)) return -1;
     DeviceScope scope;
     if (scope.enter(device_id)) return refuse(name, "no such device");
     const Wanted want = {dx, ddt, dA, dB, dC, dD, ddt_bias, dz, dh_in, accumulate};

@@ -224,21 +224,53 @@ inline bool aligned_rows(const Rows& r, int batch, int len, size_t es, size_t by
     return (reinterpret_cast<uintptr_t>(r.p) % bytes) == 0 && (batch == 1 || r.batch * size % step == 0) && (len == 1 || r.row * size % step == 0);
 }
 
-/* Whether two such operands share an element.  Column blocks of one buffer (the halves of a projection's output) do not;
- * where that cannot be seen from the strides, operands whose extents meet count as sharing. */
-inline bool overlaps(const Rows& a, const Rows& b, int batch, int len, size_t es) {
-    if (!a.p || !b.p) return false;
-    const char *a0 = reinterpret_cast<const char*>(a.p), *b0 = reinterpret_cast<const char*>(b.p);
-    const long long size = (long long)es;
-    const char* a1 = a0 + ((batch - 1) * a.batch + (len - 1) * a.row + a.channels) * size;
-    const char* b1 = b0 + ((batch - 1) * b.batch + (len - 1) * b.row + b.channels) * size;
+/* What a call reads or writes, for the host's checks of overlaps: a strided operand, or a packed one as a single row. */
+struct Area {
+    const char* name;
+    Rows r;
+    int batch, len;
+    long long size;             /* bytes per element */
+    const void* in_place;       /* an operand that this output may be, or NULL */
+};
+inline Area strided(const char* name, const Rows& r, int batch, int len, size_t size) { return {name, r, batch, len, (long long)size, nullptr}; }
+inline Area packed(const char* name, const void* p, long long elems, size_t size, const void* in_place = nullptr) {
+    return {name, {elems > 0 ? p : nullptr, 0, 0, elems}, 1, 1, (long long)size, in_place};
+}
+
+/* Whether two of them share a byte.  Column blocks of one buffer (the halves of a projection's output) do not; where that cannot
+ * be seen from the strides, operands whose extents meet count as sharing. */
+inline bool overlaps(const Area& a, const Area& b) {
+    if (!a.r.p || !b.r.p) return false;
+    const char *a0 = reinterpret_cast<const char*>(a.r.p), *b0 = reinterpret_cast<const char*>(b.r.p);
+    const char* a1 = a0 + ((a.batch - 1) * a.r.batch + (a.len - 1) * a.r.row + a.r.channels) * a.size;
+    const char* b1 = b0 + ((b.batch - 1) * b.r.batch + (b.len - 1) * b.r.row + b.r.channels) * b.size;
     if (a1 <= b0 || b1 <= a0) return false;
-    const long long unit = len > 1 ? a.row : a.batch;       /* every row of both begins a multiple of `unit` from its base */
-    if (unit <= 0 || (len > 1 && a.row != b.row)) return true;
-    if (batch > 1 && (a.batch % unit != 0 || b.batch % unit != 0)) return true;
-    const long long apart = (b0 - a0) % (unit * size);
-    const long long shift = apart < 0 ? apart + unit * size : apart;
-    return !(shift >= a.channels * size && shift + b.channels * size <= unit * size);
+    const bool a_single = a.batch == 1 && a.len == 1, b_single = b.batch == 1 && b.len == 1;
+    if (a_single && b_single) return true;
+    if (a_single) return overlaps(b, a);
+    const long long unit = a.len > 1 ? a.r.row : a.r.batch;     /* every row of a (of both, if b has several) begins a multiple of it from its base */
+    if (unit <= 0 || (a.batch > 1 && a.r.batch % unit != 0)) return true;
+    if (!b_single && (a.size != b.size || (a.len > 1 && a.r.row != b.r.row) || (a.batch > 1 && b.r.batch % unit != 0))) return true;
+    const long long apart = (b0 - a0) % (unit * a.size);
+    const long long shift = apart < 0 ? apart + unit * a.size : apart;
+    return !(shift >= a.r.channels * a.size && shift + b.r.channels * b.size <= unit * a.size);
+}
+
+/* Refuses outputs that share memory with what the call reads, or with one another. */
+template <int N, int M> int refuse_overlaps(const char* what, const Area (&outs)[N], const Area (&ins)[M]) {
+    for (int i = 0; i < N; ++i) {
+        for (int k = 0; k < M; ++k)
+            if (!(outs[i].in_place && outs[i].r.p == outs[i].in_place && ins[k].r.p == outs[i].in_place) && overlaps(outs[i], ins[k])) {
+                fprintf(stderr, "recpulse_b200: %s: %s overlaps %s\n", what, outs[i].name, ins[k].name);
+                return -1;
+            }
+        for (int k = 0; k < i; ++k)
+            if (overlaps(outs[i], outs[k])) {
+                fprintf(stderr, "recpulse_b200: %s: %s overlaps %s\n", what, outs[i].name, outs[k].name);
+                return -1;
+            }
+    }
+    return 0;
 }
 
 constexpr int SM_COUNT = 148;       /* of the one chip this library is written for; sizes of splits follow it */

@@ -191,3 +191,85 @@ def test_nodes_refuse_empty_dimensions(capfd):
     assert not lib.op_causal_conv(by(empty), by(tensor((0, 4), (4, 1))), None, 1)
     assert not lib.op_causal_conv(by(x), by(none), None, 1)
     assert "cudaMalloc" not in capfd.readouterr().err
+
+
+def overlap_refused(capfd, call, *names):
+    """The call is refused, for an overlap of the two named buffers (in any order)."""
+    capfd.readouterr()
+    assert call() == -1
+    err = capfd.readouterr().err
+    assert "overlaps" in err and all(f" {n} " in err.replace("\n", " ") for n in names), (names, err)
+
+
+def test_convolution_refuses_outputs_over_packed_operands(capfd):
+    lib, c = rpb.load(), conv()                                    # x, y 320 bytes, w 128, bias 32, states 192
+    base = dict(y=at(0), so=None, x=at(8192), w=at(16384), b=at(17000), si=at(18000), n=at(19000))
+    call = lambda **k: lambda: lib.rp_causal_conv_ex(*{**base, **k}.values(), C.byref(c), 0, 0, None)          # noqa: E731
+    overlap_refused(capfd, call(y=at(16384 + 124)), "y", "w")
+    overlap_refused(capfd, call(y=at(17000 - 316)), "y", "bias")
+    overlap_refused(capfd, call(y=at(18000)), "y", "state_in")
+    overlap_refused(capfd, call(y=at(19004)), "y", "lengths")
+    overlap_refused(capfd, call(so=at(8192)), "state_out", "x")
+    overlap_refused(capfd, call(so=at(316)), "state_out", "y")
+    overlap_refused(capfd, call(so=at(18000 + 188)), "state_out", "state_in")      # in place it may be, shifted not
+    overlap_refused(capfd, call(so=at(18000 - 4)), "state_out", "state_in")
+    grads = dict(dx=at(0), dw=at(1000), db=at(2000), ds=at(3000), acc=0, dy=at(4000), dso=at(5000), x=at(8192), w=at(16384), b=at(17000), si=at(18000),
+                 n=None, ws=at(30000))
+    grad = lambda **k: lambda: lib.rp_causal_conv_grad_ex(*{**grads, **k}.values(), C.byref(c), 0, 0, None)    # noqa: E731
+    overlap_refused(capfd, grad(dx=at(16384)), "dx", "w")
+    overlap_refused(capfd, grad(dw=at(16384 + 4)), "dw", "w")
+    overlap_refused(capfd, grad(dw=at(4000)), "dw", "dy")
+    overlap_refused(capfd, grad(db=at(1124)), "dbias", "dw")
+    overlap_refused(capfd, grad(ds=at(18000 + 4)), "dstate_in", "state_in")
+    overlap_refused(capfd, grad(ds=at(5000)), "dstate_in", "dstate_out")
+    overlap_refused(capfd, grad(ws=at(8192)), "ws", "x")
+    overlap_refused(capfd, grad(ws=at(0)), "ws", "dx")
+
+
+def test_scan_refuses_outputs_over_packed_operands(capfd):
+    lib, c = rpb.load(), scan()                                    # rows 320 bytes each, A 128, D 32, states 256
+    a = [at(2048 * i) for i in range(16)]
+    base = dict(y=a[0], ho=None, saved=None, x=a[1], dt=a[2], A=a[3], B=a[4], C=a[5], D=a[6], bias=a[7], z=a[8], hi=a[9], n=a[10], ws=None)
+    call = lambda **k: lambda: lib.rp_selective_scan_ex(*{**base, **k}.values(), C.byref(c), 0, 0, None)       # noqa: E731
+    for name, i in (("A", 3), ("D", 6), ("dt_bias", 7), ("h_in", 9), ("lengths", 10)):
+        overlap_refused(capfd, call(y=a[i]), "y", name)
+    overlap_refused(capfd, call(ho=at(2048 * 9 + 4)), "h_out", "h_in")
+    overlap_refused(capfd, call(ho=a[1]), "h_out", "x")
+    overlap_refused(capfd, call(ho=at(316)), "h_out", "y")
+    overlap_refused(capfd, call(saved=at(2048 * 9 + 252)), "saved", "h_in")
+    overlap_refused(capfd, call(saved=a[11], ho=at(2048 * 11 + 4)), "saved", "h_out")
+    long = scan(batch=1, length=300, channels=4, states=1, groups=1)
+    split = lambda ws: lambda: lib.rp_selective_scan_ex(at(0), None, None, at(8192), at(16384), at(24000), at(26000), at(30000), None, None, None, None,     # noqa: E731
+                                                        None, ws, C.byref(long), 0, 0, None)
+    assert lib.rp_selective_scan_ws_bytes(C.byref(long), 0, 0) > 0
+    overlap_refused(capfd, split(at(8192)), "ws", "x")
+    names = ("dx", "ddt", "dA", "dB", "dC", "dD", "ddt_bias", "dz", "dh_in")
+    outs = {k: at(32768 + 1024 * i) for i, k in enumerate(names)}
+    rest = dict(acc=0, dy=a[0], dho=a[11], x=a[1], dt=a[2], A=a[3], B=a[4], C=a[5], D=a[6], bias=a[7], z=a[8], n=None, saved=a[12], ws=at(50000))
+    grad = lambda **k: lambda: lib.rp_selective_scan_grad_ex(*{**outs, **rest, **k}.values(), C.byref(c), 0, 0, None)      # noqa: E731
+    overlap_refused(capfd, grad(dA=a[3]), "dA", "A")
+    overlap_refused(capfd, grad(dD=outs["dA"]), "dD", "dA")
+    overlap_refused(capfd, grad(ddt_bias=a[1]), "ddt_bias", "x")
+    overlap_refused(capfd, grad(dh_in=at(2048 * 11 + 4)), "dh_in", "dh_out")
+    overlap_refused(capfd, grad(dx=a[12]), "dx", "saved")
+    overlap_refused(capfd, grad(ws=a[0]), "ws", "dy")
+    overlap_refused(capfd, grad(ws=outs["dx"]), "ws", "dx")
+
+
+def test_norm_refuses_outputs_over_weights(capfd):
+    lib, c = rpb.load(), norm()                                    # rows 128 bytes, weights 32
+    base = dict(out=at(0), y=at(1000), u=at(2000), z=at(3000), wa=at(4000), sc=at(4100), r=at(5000), wb=at(4200))
+    call = lambda **k: lambda: lib.rp_block_norm_ex(*{**base, **k}.values(), C.byref(c), 0, 0, None)           # noqa: E731
+    overlap_refused(capfd, call(out=at(4000)), "out", "w_after")
+    overlap_refused(capfd, call(y=at(4228)), "y", "w_before")
+    overlap_refused(capfd, call(out=at(4100 - 124), wa=at(6000)), "out", "scale")
+    overlap_refused(capfd, call(y=at(124)), "y", "out")
+    outs = dict(du=at(10000), dz=at(11000), dr=at(12000), dwa=at(13000), dsc=at(13100), dwb=at(13200), acc=0, dout=at(14000), dy=at(15000))
+    rest = {k: base[k] for k in ("u", "z", "wa", "sc", "r", "wb")}
+    grad = lambda **k: lambda: lib.rp_block_norm_grad_ex(*{**outs, **rest, "ws": at(20000), **k}.values(), C.byref(c), 0, 0, None)     # noqa: E731
+    overlap_refused(capfd, grad(dwa=at(4000)), "dw_after", "w_after")
+    overlap_refused(capfd, grad(dsc=at(13000)), "dscale", "dw_after")
+    overlap_refused(capfd, grad(du=at(4200)), "du", "w_before")
+    overlap_refused(capfd, grad(dwb=at(2000)), "dw_before", "u")
+    overlap_refused(capfd, grad(ws=at(3000)), "ws", "z")
+    overlap_refused(capfd, grad(ws=at(13000)), "ws", "dw_after")
