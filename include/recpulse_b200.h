@@ -207,8 +207,8 @@ int rp_conv2d_backward_ex(void* grad_input, int accumulate_input, void* grad_wei
  * the last width-1 rows of xp and may be state_in.  One token per call (len = 1) with the state in place is the form for
  * generation.  lengths: NULL, or `batch` ints in device memory; rows at and behind lengths[b] (clamped to 0 .. len) are not
  * part of sequence b: they are not read, their y (and dx) is 0, and the state is the one after the last row in front of them.
- * No output may overlap what the call reads or another output (refused; state_out = state_in apart).  Everything is of `dtype`;
- * sums are float32 (float64 for float64), one rounding.
+ * No output may overlap what the call reads or another output (refused; state_out = state_in apart), and every buffer is aligned
+ * to its elements (else refused).  Everything is of `dtype`; sums are float32 (float64 for float64), one rounding.
  * Asynchronous on `stream`; 0 / -1. */
 typedef struct {
     int batch, len, channels, width;
@@ -245,7 +245,8 @@ int rp_causal_conv_grad_ex(void* dx, void* dw, void* dbias, void* dstate_in, int
  * states h_in, h_out [batch, channels, states] (or NULL: zeros / not wanted; h_out may be h_in) are packed float32 (float64
  * when `dtype` is float64), and so are all sums.  One token per call (len = 1) with the state in place is the form for
  * generation.  lengths: as in rp_causal_conv_ex; h_out is the state behind the last row in front of lengths[b].
- * No output may overlap what the call reads or another output (refused; h_out = h_in apart).  Asynchronous on `stream`; 0 / -1. */
+ * No output may overlap what the call reads or another output (refused; h_out = h_in apart), and every buffer is aligned to its
+ * elements, the workspace to those of the sums (else refused).  Asynchronous on `stream`; 0 / -1. */
 typedef struct {
     int batch, len, channels, states, groups;
     int softplus;
@@ -288,7 +289,8 @@ int rp_selective_scan_grad_ex(void* dx, void* ddt, void* dA, void* dB, void* dC,
  *   y = out / sqrt(mean out^2 + eps_before) * w_before           the norm before the next block
  * out or y may be NULL (not wanted); w_before is needed for y.  y is computed from the sum before its rounding.  Everything is
  * of `dtype`; means and sums are float32 (float64), each output is rounded once.  Row strides in elements, channel stride 1;
- * weights packed.  No output may overlap what the call reads or another output (refused).  Asynchronous on `stream`; 0 / -1. */
+ * weights packed.  No output may overlap what the call reads or another output, and every buffer is
+ * aligned to its elements (else refused).  Asynchronous on `stream`; 0 / -1. */
 typedef struct {
     long long rows;
     int channels;

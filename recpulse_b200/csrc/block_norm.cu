@@ -622,7 +622,7 @@ int rp_block_norm_ex(void* out, void* y, const void* u, const void* z, const voi
     const Area outs[] = {row_area(c, "out", out, c->out_row, es), row_area(c, "y", y, c->y_row, es)};
     const Area ins[] = {row_area(c, "u", u, c->u_row, es), row_area(c, "z", z, c->z_row, es), row_area(c, "r", r, c->r_row, es),
                         packed("w_after", w_after, D, es), packed("scale", scale, D, es), packed("w_before", w_before, D, es)};
-    if (refuse_overlaps(name, outs, ins)) return -1;
+    if (refuse_buffers(name, outs, ins)) return -1;
     DeviceScope scope;
     if (scope.enter(device_id)) return refuse(name, "no such device");
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
@@ -659,16 +659,16 @@ int rp_block_norm_grad_ex(void* du, void* dz, void* dr, void* dw_after, void* ds
         !readable_rows(c, dy, c->y_row))
         return refuse(name, "strides of an operand");
     if (!writable_rows(c, du, c->du_row) || !writable_rows(c, dz, c->dz_row) || !writable_rows(c, dr, c->dr_row)) return refuse(name, "strides of a gradient");
-    const size_t es = rpb_dtype_size((int)dtype);
+    const size_t es = rpb_dtype_size((int)dtype), as = dtype == DTYPE_FLOAT64 ? 8 : 4;
     const long long D = c->channels;
     const bool weights = dw_after || dscale || dw_before;
     const Area outs[] = {row_area(c, "du", du, c->du_row, es), row_area(c, "dz", dz, c->dz_row, es), row_area(c, "dr", dr, c->dr_row, es),
                          packed("dw_after", dw_after, D, es), packed("dscale", dscale, D, es), packed("dw_before", dw_before, D, es),
-                         packed("ws", weights ? ws : nullptr, weights ? rp_block_norm_ws_bytes(c, dtype) : 0, 1)};
+                         packed("ws", weights ? ws : nullptr, weights ? rp_block_norm_ws_bytes(c, dtype) / (long long)as : 0, as)};
     const Area ins[] = {row_area(c, "u", u, c->u_row, es), row_area(c, "z", z, c->z_row, es), row_area(c, "r", r, c->r_row, es),
                         row_area(c, "dout", dout, c->out_row, es), row_area(c, "dy", dy, c->y_row, es),
                         packed("w_after", w_after, D, es), packed("scale", scale, D, es), packed("w_before", w_before, D, es)};
-    if (refuse_overlaps(name, outs, ins)) return -1;
+    if (refuse_buffers(name, outs, ins)) return -1;
     DeviceScope scope;
     if (scope.enter(device_id)) return refuse(name, "no such device");
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

@@ -471,7 +471,7 @@ int rp_causal_conv_ex(void* y, void* state_out, const void* x, const void* w, co
     const Area outs[] = {strided("y", ry, c->batch, c->len, es), packed("state_out", state_out, kept, es, state_in)};
     const Area ins[] = {strided("x", rx, c->batch, c->len, es), packed("w", w, (long long)c->channels * c->width, es), packed("bias", bias, c->channels, es),
                         packed("state_in", state_in, kept, es), packed("lengths", lengths, c->batch, sizeof(int))};
-    if (refuse_overlaps(name, outs, ins)) return -1;
+    if (refuse_buffers(name, outs, ins)) return -1;
     DeviceScope scope;
     if (scope.enter(device_id)) return refuse(name, "no such device");
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
@@ -504,18 +504,18 @@ int rp_causal_conv_grad_ex(void* dx, void* dw, void* dbias, void* dstate_in, int
     if ((dw || dbias) && !ws) return refuse(name, "the filter's gradients need a workspace");
     if (device_id < 0) return refuse(name, "needs a CUDA device (no CPU path in this library)");
     const Rows rx = x_rows(c, x), rg = y_rows(c, dy), rd = dx_rows(c, dx);
-    const size_t es = rpb_dtype_size((int)dtype);
+    const size_t es = rpb_dtype_size((int)dtype), as = dtype == DTYPE_FLOAT64 ? 8 : 4;
     if (!readable(rx, c->batch, c->len)) return refuse(name, "strides of x");
     if (!readable(rg, c->batch, c->len)) return refuse(name, "strides of dy");
     if (dx && !writable(rd, c->batch, c->len)) return refuse(name, "strides of dx");
     const long long kept = state_elems(c), taps = (long long)c->channels * c->width;
     const bool filter = dw || dbias;
     const Area outs[] = {strided("dx", rd, c->batch, c->len, es), packed("dw", dw, taps, es), packed("dbias", dbias, c->channels, es),
-                         packed("dstate_in", dstate_in, kept, es), packed("ws", filter ? ws : nullptr, filter ? rp_causal_conv_ws_bytes(c, dtype) : 0, 1)};
+                         packed("dstate_in", dstate_in, kept, es), packed("ws", filter ? ws : nullptr, filter ? rp_causal_conv_ws_bytes(c, dtype) / (long long)as : 0, as)};
     const Area ins[] = {strided("dy", rg, c->batch, c->len, es), strided("x", rx, c->batch, c->len, es), packed("w", w, taps, es),
                         packed("bias", bias, c->channels, es), packed("state_in", state_in, kept, es), packed("dstate_out", dstate_out, kept, es),
                         packed("lengths", lengths, c->batch, sizeof(int))};
-    if (refuse_overlaps(name, outs, ins)) return -1;
+    if (refuse_buffers(name, outs, ins)) return -1;
     DeviceScope scope;
     if (scope.enter(device_id)) return refuse(name, "no such device");
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

@@ -1362,11 +1362,11 @@ int rp_selective_scan_ex(void* y, void* h_out, void* saved, const void* x, const
     const size_t es = rpb_dtype_size((int)dtype), as = dtype == DTYPE_FLOAT64 ? 8 : 4;
     auto area = [&](const char* n, const Rows& rows) { return strided(n, rows, c->batch, c->len, es); };
     const Area outs[] = {area("y", r.y), packed("h_out", h_out, all, as, h_in), packed("saved", saved, rp_selective_scan_saved_elems(c, dtype), as),
-                         packed("ws", ws, ws_bytes, 1)};
+                         packed("ws", ws, ws_bytes / (long long)as, as)};
     const Area ins[] = {area("x", r.x), area("dt", r.dt), area("B", r.B), area("C", r.C), area("z", r.z), packed("A", A, d * c->states, as),
                         packed("D", D, d, as), packed("dt_bias", dt_bias, d, as), packed("h_in", h_in, all, as),
                         packed("lengths", lengths, c->batch, sizeof(int))};
-    if (refuse_overlaps(name, outs, ins)) return -1;
+    if (refuse_buffers(name, outs, ins)) return -1;
     DeviceScope scope;
     if (scope.enter(device_id)) return refuse(name, "no such device");
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
@@ -1402,11 +1402,11 @@ int rp_selective_scan_grad_ex(void* dx, void* ddt, void* dA, void* dB, void* dC,
     auto area = [&](const char* n, const Rows& rows) { return strided(n, rows, c->batch, c->len, es); };
     const Area outs[] = {area("dx", w[0]), area("ddt", w[1]), area("dz", w[2]), area("dB", w[3]), area("dC", w[4]), packed("dA", dA, d * c->states, as),
                          packed("dD", dD, d, as), packed("ddt_bias", ddt_bias, d, as), packed("dh_in", dh_in, all, as),
-                         packed("ws", ws, rp_selective_scan_ws_bytes(c, dtype, 1), 1)};
+                         packed("ws", ws, rp_selective_scan_ws_bytes(c, dtype, 1) / (long long)as, as)};
     const Area ins[] = {area("dy", r.y), area("x", r.x), area("dt", r.dt), area("B", r.B), area("C", r.C), area("z", r.z),
                         packed("A", A, d * c->states, as), packed("D", D, d, as), packed("dt_bias", dt_bias, d, as), packed("dh_out", dh_out, all, as),
                         packed("saved", saved, rp_selective_scan_saved_elems(c, dtype), as), packed("lengths", lengths, c->batch, sizeof(int))};
-    if (refuse_overlaps(name, outs, ins)) return -1;
+    if (refuse_buffers(name, outs, ins)) return -1;
     DeviceScope scope;
     if (scope.enter(device_id)) return refuse(name, "no such device");
     const Wanted want = {dx, ddt, dA, dB, dC, dD, ddt_bias, dz, dh_in, accumulate};

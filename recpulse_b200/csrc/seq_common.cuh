@@ -256,8 +256,17 @@ inline bool overlaps(const Area& a, const Area& b) {
     return !(shift >= a.r.channels * a.size && shift + b.r.channels * b.size <= unit * a.size);
 }
 
-/* Refuses outputs that share memory with what the call reads, or with one another. */
-template <int N, int M> int refuse_overlaps(const char* what, const Area (&outs)[N], const Area (&ins)[M]) {
+/* Whether the elements lie on boundaries of their size: the GPU faults on others. */
+inline bool on_boundaries(const Area& a) { return reinterpret_cast<uintptr_t>(a.r.p) % (uintptr_t)a.size == 0; }
+
+/* Refuses buffers off their elements' boundaries, and outputs that share memory with what the call reads or with one another. */
+template <int N, int M> int refuse_buffers(const char* what, const Area (&outs)[N], const Area (&ins)[M]) {
+    for (int i = 0; i < N + M; ++i) {
+        const Area& a = i < N ? outs[i] : ins[i - N];
+        if (on_boundaries(a)) continue;
+        fprintf(stderr, "recpulse_b200: %s: %s is not aligned to its elements\n", what, a.name);
+        return -1;
+    }
     for (int i = 0; i < N; ++i) {
         for (int k = 0; k < M; ++k)
             if (!(outs[i].in_place && outs[i].r.p == outs[i].in_place && ins[k].r.p == outs[i].in_place) && overlaps(outs[i], ins[k])) {

@@ -273,3 +273,43 @@ def test_norm_refuses_outputs_over_weights(capfd):
     overlap_refused(capfd, grad(dwb=at(2000)), "dw_before", "u")
     overlap_refused(capfd, grad(ws=at(3000)), "ws", "z")
     overlap_refused(capfd, grad(ws=at(13000)), "ws", "dw_after")
+
+
+@pytest.mark.parametrize("dtype,size", [(rpb.F32, 4), (rpb.F64, 8), (rpb.F16, 2), (rpb.BF16, 2)])
+def test_buffers_off_their_elements_are_refused(dtype, size, capfd):
+    """The GPU faults on them, so no call with one may reach it."""
+    lib = rpb.load()
+    wide = 8 if dtype == rpb.F64 else 4                            # of sums, states and workspaces
+    start = (-BUF.ctypes.data) % 16
+
+    def refused(fn, names, sizes, tail):
+        """Every buffer in turn one byte (half an element) off, the others where they belong."""
+        places = [None if s is None else at(start + 3072 * i) for i, s in enumerate(sizes)]
+        for i, (name, s) in enumerate(zip(names, sizes)):
+            if s is None or name is None:
+                continue
+            for shift in {1, s // 2}:
+                now = list(places)
+                now[i] = at(start + 3072 * i + shift)
+                capfd.readouterr()
+                assert fn(*now, *tail) == -1
+                assert f"{name} is not aligned" in capfd.readouterr().err, name
+
+    c = conv()
+    tail = (C.byref(c), dtype, 0, None)
+    refused(lib.rp_causal_conv_ex, ("y", "state_out", "x", "w", "bias", "state_in", "lengths"), (size,) * 6 + (4,), tail)
+    grad = lambda *p: lib.rp_causal_conv_grad_ex(*p[:4], 0, *p[4:])                                # noqa: E731
+    refused(grad, ("dx", "dw", "dbias", "dstate_in", "dy", "dstate_out", "x", "w", "bias", "state_in", "lengths", "ws"), (size,) * 10 + (4, wide), tail)
+    c2 = scan()
+    tail = (C.byref(c2), dtype, 0, None)
+    refused(lib.rp_selective_scan_ex, ("y", "h_out", "saved", "x", "dt", "A", "B", "C", "D", "dt_bias", "z", "h_in", "lengths", "ws"),
+            (size, wide, wide, size, size, wide, size, size, wide, wide, size, wide, 4, None), tail)
+    grad2 = lambda *p: lib.rp_selective_scan_grad_ex(*p[:9], 0, *p[9:])                            # noqa: E731
+    refused(grad2, ("dx", "ddt", "dA", "dB", "dC", "dD", "ddt_bias", "dz", "dh_in", "dy", "dh_out", "x", "dt", "A", "B", "C", "D", "dt_bias", "z", "lengths"),
+            (size, size, wide, size, size, wide, wide, size, wide, size, wide, size, size, wide, size, size, wide, wide, size, 4, wide, wide), tail)
+    c3 = norm()
+    tail = (C.byref(c3), dtype, 0, None)
+    refused(lib.rp_block_norm_ex, ("out", "y", "u", "z", "w_after", "scale", "r", "w_before"), (size,) * 8, tail)
+    grad3 = lambda *p: lib.rp_block_norm_grad_ex(*p[:6], 0, *p[6:])                                # noqa: E731
+    refused(grad3, ("du", "dz", "dr", "dw_after", "dscale", "dw_before", "dout", "dy", "u", "z", "w_after", "scale", "r", "w_before", "ws"),
+            (size,) * 14 + (wide,), tail)
