@@ -257,12 +257,11 @@ __global__ void __launch_bounds__(128) backward_kernel(T* dx, T* dstate_in, type
                         if (j >= skip) pre += w[j][i] * win[k + j][i];
                     const A d = s < stop && s < end ? up(g[k].v[i]) * act_slope(pre, a.silu) : A(0);
                     dp[H + k][i] = d;
-                    const A own = s < pl.t1 ? d : A(0);
-                    db[i] += own;
-                    if (s < end) {
+                    if (s < pl.t1 && s < end) {         /* the run's own rows: 0 times an infinity of the next run's is formed nowhere */
+                        db[i] += d;
 #pragma unroll
                         for (int j = 0; j < W; ++j)
-                            if (j >= skip) dw[j][i] += own * win[k + j][i];
+                            if (j >= skip) dw[j][i] += d * win[k + j][i];
                     }
                 }
                 const int r = s - H;                /* the row whose gradient is complete now */

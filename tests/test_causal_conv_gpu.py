@@ -240,3 +240,29 @@ def test_replayed_from_a_graph_on_another_stream(lib):
         ref = reference(x, w, bias, None, None, 1, dy, None, dtype)
         for name, got in (("y", y), ("dx", dx), ("dw", dw), ("dbias", db)):
             close(got, ref[name], ref[name + "_slack"], name)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("width", [1, 2, 3, 4, 6, 8])
+@pytest.mark.parametrize("d", [64, 61])
+def test_one_infinite_row_in_every_place(lib, dtype, width, d):
+    """Channel c holds one infinity, in row c: in the first rows of a thread's run as anywhere else it makes the gradients of the
+    taps that meet it infinite, with the definition's sign, and nothing else."""
+    batch, length = 1, 45
+    x, w, bias, _, dy = make(batch, length, d, width, dtype, 41, cols=1)
+    c, ends = geometry(x, width, 0), torch.tensor([40], dtype=torch.int32, device="cuda")
+    rows = torch.arange(d) % length
+    finite = reference(x, w, bias, None, [40], 0, dy, None, dtype)
+    x[0, rows, torch.arange(d)] = float("inf")
+    line = torch.cat([torch.zeros(width - 1, d, dtype=torch.float64), x[0, :40].double().cpu()])
+    want = torch.stack([(dy[0, :40].double().cpu() * line[j:j + 40]).sum(0) for j in range(width)], dim=1)
+    dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty_like(bias)
+    backward(lib, dy, x, w, bias, None, ends, c, dtype, dx, dw, db)
+    far = torch.isinf(want)
+    assert int(far.sum()) == sum(max(0, min(width, 40 - int(r))) for r in rows) and not want.isnan().any()
+    assert torch.equal(dw.cpu().double()[far], want[far])
+    hit = rows[:, None] < 40                    # the rest of a channel's taps lack the product with the infinite row's old value
+    close(dw.cpu()[~hit.expand_as(far)], finite["dw"][~hit.expand_as(far)], finite["dw_slack"][~hit.expand_as(far)], "dw")
+    assert torch.isfinite(dw.cpu()[~far]).all()
+    close(dx, finite["dx"], finite["dx_slack"], "dx")
+    close(db, finite["dbias"], finite["dbias_slack"], "dbias")
