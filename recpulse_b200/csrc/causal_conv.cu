@@ -273,11 +273,20 @@ __global__ void __launch_bounds__(128) backward_kernel(T* dx, T* dstate_in, type
                 const int from_end = r - (end - keep);              /* row of the final state that is this row of xp */
                 A v[V];
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    v[i] = 0;
+                for (int i = 0; i < V; ++i) v[i] = 0;
+                if (r >= 0 && s < end) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i)
+#pragma unroll
+                        for (int j = 0; j < W; ++j)
+                            if (j >= skip) v[i] += w[j][i] * dp[H + k - j][i];
+                } else {                            /* rows that are not of the sequence form no product */
 #pragma unroll
                     for (int j = 0; j < W; ++j)
-                        if (j >= skip) v[i] += w[j][i] * dp[H + k - j][i];
+                        if (j >= skip && s - j >= 0 && s - j < end) {
+#pragma unroll
+                            for (int i = 0; i < V; ++i) v[i] += w[j][i] * dp[H + k - j][i];
+                        }
                 }
                 if (more_from && from_end >= 0 && from_end < keep) {
                     const Pack<T, V> more = lane.load(more_from + (long long)from_end * a.channels, true);

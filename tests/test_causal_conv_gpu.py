@@ -266,3 +266,30 @@ def test_one_infinite_row_in_every_place(lib, dtype, width, d):
     assert torch.isfinite(dw.cpu()[~far]).all()
     close(dx, finite["dx"], finite["dx_slack"], "dx")
     close(db, finite["dbias"], finite["dbias_slack"], "dbias")
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("width", [1, 2, 3, 4, 6, 8])
+@pytest.mark.parametrize("d", [64, 61])
+def test_infinite_taps_at_the_ends_of_a_sequence(lib, dtype, width, d):
+    """Channel c has one infinite tap.  Rows whose product with it would need a row in front of or behind the sequence keep a finite
+    gradient, rows behind a sequence 0."""
+    batch, length, ends = 4, 45, [40, 3, 0, 45]
+    x, w, bias, state, dy = make(batch, length, d, width, dtype, 43, state=True, cols=1)
+    taps = torch.arange(d) % width
+    w[torch.arange(d), taps] = float("inf")
+    c, given = geometry(x, width, 0), torch.tensor(ends, dtype=torch.int32, device="cuda")
+    dx, ds = torch.empty_like(x), torch.empty_like(state)
+    backward(lib, dy, x, w, bias, state, given, c, dtype, dx, None, None, ds)
+    want, slack = torch.zeros(batch, width - 1 + length, d, dtype=torch.float64), torch.zeros(batch, width - 1 + length, d, dtype=torch.float64)
+    w64, w_finite = w.double().cpu(), torch.where(w.isinf(), 0.0, w.double()).cpu()
+    for b, end in enumerate(ends):
+        g = dy[b, :end].double().cpu()
+        for j in range(width):
+            want[b, j:j + end] += w64[:, j] * g
+            slack[b, j:j + end] += (width + 1) * unit(dtype) * (w_finite[:, j] * g).abs()
+    assert not want.isnan().any()
+    got = torch.cat([ds, dx], dim=1).cpu().double()
+    far = want.isinf()
+    assert torch.equal(got[far], want[far])
+    close(torch.cat([ds, dx], dim=1).cpu()[~far], want[~far], slack[~far], "dx, dstate")
