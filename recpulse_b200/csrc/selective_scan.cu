@@ -127,6 +127,16 @@ __device__ __forceinline__ A delta_of(T raw, A bias, int softplus) {
     return softplus ? softplus_of(v) : v;
 }
 
+/* h across a chunk whose deltas add up to `sum` and that ends with `part` from zero.  The chunk's decay in two halves: it may be
+ * beyond the type's range where its product with h is not, and a state of 0 stays 0 however fast states grow. */
+template <typename A> __device__ __forceinline__ void cross_chunk(A (&h)[S], const A (&part)[S], const A (&rate)[S], A sum) {
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+        const A half = decay(sum * A(0.5), rate[i]);
+        h[i] = h[i] == A(0) ? part[i] : h[i] * half * half + part[i];
+    }
+}
+
 /* Four states of one channel and their step: h = exp(delta A) h + dx b, and c . h.  In float the four are two register pairs
  * (mul / fma.f32x2: 13 instructions instead of 20 beside the four exponentials, which bound the scan). */
 template <typename A> struct Walk {
@@ -252,9 +262,7 @@ forward_kernel(T* __restrict__ y, typename AccOf<T>::type* h_out, typename AccOf
                 const long long at = (pl.b * (long long)a.chunks + c) * a.channels + d;
                 A part[S];
                 load_states(part, chunk_h + at * a.states, n0, a.states, a.vec_n);
-                const A s = chunk_s[at];
-#pragma unroll
-                for (int i = 0; i < S; ++i) h[i] = decay(s, rate[i]) * h[i] + part[i];
+                cross_chunk(h, part, rate, chunk_s[at]);
             }
         }
         Walk<A> w;
@@ -677,18 +685,17 @@ backward_kernel(Grads<T> out, typename AccOf<T>::type* __restrict__ chunk_g, typ
                 t1[i] = decay_rate(t0[i]);
                 z0[i] = 0;
             }
-            Av.set(t0); rate.set(t1); g.set(z0); dA.set(z0);
+            Av.set(t0); rate.set(t1); dA.set(z0);
             if (!AGG && on) {
-                if (dh_out) { load_states(t0, dh_out + (pl.b * D + d) * a.states, n0, a.states, a.vec_n); g.set(t0); }
+                if (dh_out) load_states(z0, dh_out + (pl.b * D + d) * a.states, n0, a.states, a.vec_n);
 #pragma unroll 4
                 for (int c = a.chunks - 1; c > pl.c; --c) {
                     const long long at = (pl.b * (long long)a.chunks + c) * D + d;
-                    V4<A> part;
                     load_states(t0, chunk_g + at * a.states, n0, a.states, a.vec_n);
-                    part.set(t0);
-                    g = mad(decays(chunk_s[at], rate), g, part);
+                    cross_chunk(z0, t0, t1, chunk_s[at]);
                 }
             }
+            g.set(z0);
             Av = swap_halves(Av, odd); rate = swap_halves(rate, odd); g = swap_halves(g, odd);
         }
         /* the states in front of the segments, the next one's on their way while one is worked on */

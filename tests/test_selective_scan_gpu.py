@@ -368,3 +368,28 @@ def test_replayed_from_a_graph_on_another_stream(lib):
         close(y, ref["y"], ref["y_slack"], "y"); close(h, ref["h"], ref["h_slack"], "h")
         for k in GRADS:
             close(got[k], ref[k], ref[k + "_slack"], k)
+
+
+@pytest.mark.parametrize("dtype,n,groups", [("float32", 4, 1), ("bfloat16", 16, 2), ("float64", 3, 1), ("float16", 33, 1)])
+def test_zero_states_cross_fast_growing_chunks(lib, dtype, n, groups):
+    """A split sequence part of which would let states grow beyond the type's range within a chunk: in front of the first x, and (for
+    the gradients) behind the last dy.  The states there are 0 and stay it, so nothing overflows in the recurrence."""
+    d, length = 12, 500
+    s = make(1, length, d, n, groups, dtype, 45, gate=False, bias=False)
+    s["A"][:] = 4.0 if dtype != "float64" else 32.0                 # a chunk is at least 64 rows: e^(64 * 0.5 * 4)
+    s["dt"][:] = 0.5
+    s["dt"][:, 400:] = 0.0003
+    s["x"][:, :400] = 0
+    c = geometry(s, n, groups, 0)
+    assert lib.rp_selective_scan_ws_bytes(C.byref(c), CODE[dtype], 0) > 0          # it is split
+    ref = reference(s, n, groups, 0, dtype=dtype)
+    assert all(torch.isfinite(ref[k]).all() for k in ("y", "y_slack", "h", "h_slack"))
+    y, h, _ = forward(lib, s, c, dtype)
+    close(y, ref["y"], ref["y_slack"], "y")
+    close(h, ref["h"], ref["h_slack"], "h")
+    s["dt"] = s["dt"].flip(1).contiguous()
+    s["x"][:] = 0
+    s["dy"][:, 100:] = 0
+    ref = reference(s, n, groups, 0, None, True, dtype)
+    assert all(torch.isfinite(ref[k]).all() for k in ref)
+    check(lib, s, n, groups, 0, dtype, "growing behind the gradients")
