@@ -8,6 +8,8 @@
  *   dA = sum of da delta,  ddelta = sum_n (da A + dh B x),  dx = delta sum_n dh B + D dy,
  *   dB = sum over channels of dh delta x,  dC = sum over channels of dy h,  dD = sum of dy x.
  */
+#include <cfloat>
+
 #include "seq_common.cuh"
 
 namespace rpb_scan {
@@ -46,9 +48,13 @@ template <typename A> struct Pair { A delta, dx; };
 constexpr float CENTRE = 2.5e-8f;
 __device__ __forceinline__ float decay(float delta, float a) { return ex2_fast(fmaf(delta, a, CENTRE)); }
 __device__ __forceinline__ double decay(double delta, double a) { return exp(delta * a); }
-/* A as the decay wants it: in float times log2(e), for the base-2 exponential */
-__device__ __forceinline__ float decay_rate(float a) { return a * 1.44269504088896341f; }
-__device__ __forceinline__ double decay_rate(double a) { return a; }
+/* A as the decay wants it: in float times log2(e), for the base-2 exponential; finite, so that a delta of 0 (a row that is not part of
+ * the sequence) changes nothing whatever A is */
+__device__ __forceinline__ float decay_rate(float a) {
+    const float r = a * 1.44269504088896341f;
+    return isinf(r) ? copysignf(FLT_MAX, r) : r;
+}
+__device__ __forceinline__ double decay_rate(double a) { return isinf(a) ? copysign(DBL_MAX, a) : a; }
 
 __device__ __forceinline__ int row_end(const int* lengths, int b, int len) {
     if (!lengths) return len;

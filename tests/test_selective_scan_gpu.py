@@ -393,3 +393,24 @@ def test_zero_states_cross_fast_growing_chunks(lib, dtype, n, groups):
     ref = reference(s, n, groups, 0, None, True, dtype)
     assert all(torch.isfinite(ref[k]).all() for k in ref)
     check(lib, s, n, groups, 0, dtype, "growing behind the gradients")
+
+
+@pytest.mark.parametrize("dtype,length,ends", [("float32", 37, [37, 5, 0]), ("bfloat16", 70, [70, 33, 1]), ("float64", 21, [21, 8, 3]), ("float16", 9, [9, 9, 9]),
+                                               ("float32", 300, [300, 100, 290])])
+@pytest.mark.parametrize("infinite", [False, True])
+def test_states_that_forget_at_once(lib, dtype, length, ends, infinite):
+    """A at the end of its type's range, or infinite: every row's state is its own feed, also behind rows of a tile that are not part
+    of the sequence, whose delta is 0."""
+    d, n, a = 12, 6, acc_type(dtype)
+    s = make(3, length, d, n, 1, dtype, 47, state=True)
+    s["A"][:, ::2] = -1e30                                         # the same decays: 0 for every delta of a row
+    ref = reference(s, n, 1, 1, ends, True, dtype)
+    s["A"][:, ::2] = -float("inf") if infinite else -torch.finfo(a).max
+    c, given = geometry(s, n, 1, 1), torch.tensor(ends, dtype=torch.int32, device="cuda")
+    y, h, saved = forward(lib, s, c, dtype, given, keep=True)
+    close(y, ref["y"], ref["y_slack"], "y")
+    close(h, ref["h"], ref["h_slack"], "h")
+    got = backward(lib, s, c, dtype, saved, given)
+    for k in GRADS:
+        if not (infinite and k in ("ddt", "ddt_bias")):             # 0 times A is part of these
+            close(got[k], ref[k], ref[k + "_slack"], k)
