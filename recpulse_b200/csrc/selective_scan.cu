@@ -730,7 +730,8 @@ backward_kernel(Grads<T> out, typename AccOf<T>::type* __restrict__ chunk_g, typ
             } else {
                 /* dA of one tile, then added to the total: sums of at most 16 and of as many as there are tiles, where one sum
                  * over all rows would have lost a digit */
-                V4<A> dA_tile = mul(dA, A(0));
+                V4<A> dA_tile;
+                { const A none[S] = {0, 0, 0, 0}; dA_tile.set(none); }
                 /* PARTIAL: rows from `live` on are not part of the sequence (or the chunk).  Their decay is 1 and nothing enters,
                  * so the state and its gradient pass through them, and their results are 0 whatever the state holds. */
                 auto segment = [&](int r0, int live, auto partial) {

@@ -414,3 +414,18 @@ def test_states_that_forget_at_once(lib, dtype, length, ends, infinite):
     for k in GRADS:
         if not (infinite and k in ("ddt", "ddt_bias")):             # 0 times A is part of these
             close(got[k], ref[k], ref[k + "_slack"], k)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n,d", [(4, 8), (16, 3)])
+def test_an_infinite_gradient_of_A_stays_one(lib, dtype, n, d):
+    """One infinite dy in the last tile of several: what the tiles in front of it add leaves dA the infinity that it is."""
+    s = make(1, 100, d, n, 1, dtype, 53, state=True, gate=False)
+    for k in ("B", "C", "h", "x", "D", "dy", "dh"):
+        s[k] = s[k].abs() + 0.01
+    s["A"][:] = -0.1
+    s["dy"][:, 95] = float("inf")
+    c = geometry(s, n, 1, 1)
+    _, _, saved = forward(lib, s, c, dtype, keep=True)
+    got = backward(lib, s, c, dtype, saved)
+    assert (got["dA"] == float("inf")).all() and (got["dh_in"] == float("inf")).all()
