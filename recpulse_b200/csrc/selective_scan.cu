@@ -151,6 +151,7 @@ template <typename A> struct Walk {
     __device__ __forceinline__ void set_rate(const A (&r)[S]) { for (int i = 0; i < S; ++i) rate[i] = r[i]; }
     __device__ __forceinline__ void set(const A (&v)[S]) { for (int i = 0; i < S; ++i) h[i] = v[i]; }
     __device__ __forceinline__ void get(A (&v)[S]) const { for (int i = 0; i < S; ++i) v[i] = h[i]; }
+    __device__ __forceinline__ void clear(const bool (&real)[S]) { for (int i = 0; i < S; ++i) h[i] = real[i] ? h[i] : A(0); }
     __device__ __forceinline__ void decays(Four& e, A delta) const {
 #pragma unroll
         for (int i = 0; i < S; ++i) e.v[i] = decay(delta, rate[i]);
@@ -172,6 +173,13 @@ template <> struct Walk<float> {
     __device__ __forceinline__ void set_rate(const float (&r)[S]) { r0 = pack2(r[0], r[1]); r1 = pack2(r[2], r[3]); }
     __device__ __forceinline__ void set(const float (&v)[S]) { h0 = pack2(v[0], v[1]); h1 = pack2(v[2], v[3]); }
     __device__ __forceinline__ void get(float (&v)[S]) const { unpack2(h0, v[0], v[1]); unpack2(h1, v[2], v[3]); }
+    __device__ __forceinline__ void clear(const bool (&real)[S]) {
+        float v[S];
+        get(v);
+#pragma unroll
+        for (int i = 0; i < S; ++i) v[i] = real[i] ? v[i] : 0.0f;
+        set(v);
+    }
     __device__ __forceinline__ void decays(Four& e, float delta) const {
         const f32x2 dl = pack2(delta, delta);
         float e0, e1, e2, e3;
@@ -210,7 +218,9 @@ template <typename T, int P> struct Forward : Tile<T, P, NT> {
  * finish tile i - 1 (skip, gate, rounding, whole packs to memory); one barrier per tile.
  * AGG: the first of two passes over a long sequence that is split into chunks.  It leaves, per chunk, the state that the
  * chunk would end with from zero and the sum of its deltas; exp(A sum) is the whole chunk's decay, so the state in front of
- * a chunk is folded from these, and the second pass (AGG = false) runs every chunk from its own. */
+ * a chunk is folded from these, and the second pass (AGG = false) runs every chunk from its own.
+ * PADS: some of the P lanes' states are behind the last one.  They are cleared after every row: their B and C are 0, but 0 times an
+ * infinite delta x would make them NaN, and y with them. */
 template <typename T> struct Resident { static constexpr int value = sizeof(T) <= 4 ? 2 : 1; };
 
 template <typename T, int P> struct Ring { static constexpr int DEPTH = P == 16 || sizeof(T) == 8 ? 1 : sizeof(T) == 4 ? 2 : 3, SLOTS = DEPTH + 2; };
@@ -225,7 +235,7 @@ template <typename T, int P, bool AGG> struct ForwardShared {
     alignas(16) A Bs[2][Sh::TT][Sh::NP], Cs[2][ONE][Sh::NP], ys[2][ONE][Sh::YROW];
 };
 
-template <typename T, int P, bool AGG>
+template <typename T, int P, bool AGG, bool PADS>
 __global__ void __launch_bounds__(NT + Forward<T, P>::NL, Resident<T>::value)
 forward_kernel(T* __restrict__ y, typename AccOf<T>::type* h_out, typename AccOf<T>::type* __restrict__ saved, typename AccOf<T>::type* __restrict__ chunk_h,
                typename AccOf<T>::type* __restrict__ chunk_s, const T* __restrict__ x, const T* __restrict__ dt, const typename AccOf<T>::type* __restrict__ Am,
@@ -272,6 +282,9 @@ forward_kernel(T* __restrict__ y, typename AccOf<T>::type* h_out, typename AccOf
             }
         }
         Walk<A> w;
+        bool real[S];
+#pragma unroll
+        for (int i = 0; i < S; ++i) real[i] = n0 + i < a.states;
         w.set(h);
         w.set_rate(rate);
         A* keep = nullptr;
@@ -309,6 +322,7 @@ forward_kernel(T* __restrict__ y, typename AccOf<T>::type* h_out, typename AccOf
                     if (k + 2 < BLK) pr[(k + 2) % 3] = pairs[(t + k + 2) * Sh::ROW];
                     if (k + 1 < BLK) bring(k + 1);
                     w.step(e[k & 1], pr[k % 3].dx, bv[k & 1]);
+                    if (PADS) w.clear(real);
                     if (AGG) sum += pr[k % 3].delta;
                     else v[k] = w.dot(cv[k & 1]);
                 }
@@ -536,7 +550,7 @@ __global__ void __launch_bounds__(256) token_kernel(T* __restrict__ y, typename 
 #pragma unroll
             for (int i = 0; i < S; ++i) {
                 h[r][i] = decay(delta, rate[i]) * h[r][i] + dx * bv[r][i];
-                o[0] += h[r][i] * cv[r][i];
+                if (n0 + i < a.states) o[0] += h[r][i] * cv[r][i];     /* not 0 times the NaN of an infinite dx times 0 */
             }
         }
         if (on && b < a.batch && h_out) store_states(h_out + (b * (long long)a.channels + d) * a.states, h[r], n0, a.states, a.vec_n);
@@ -560,6 +574,13 @@ template <> struct V4<float> {
     __device__ __forceinline__ void set(const float (&x)[S]) { a = pack2(x[0], x[1]); b = pack2(x[2], x[3]); }
     __device__ __forceinline__ void get(float (&x)[S]) const { unpack2(a, x[0], x[1]); unpack2(b, x[2], x[3]); }
 };
+template <typename A> __device__ __forceinline__ void clear(V4<A>& x, const bool (&real)[S]) {
+    A v[S];
+    x.get(v);
+#pragma unroll
+    for (int i = 0; i < S; ++i) v[i] = real[i] ? v[i] : A(0);
+    x.set(v);
+}
 __device__ __forceinline__ V4<float> mul(const V4<float>& x, const V4<float>& y) { return {mul2(x.a, y.a), mul2(x.b, y.b)}; }
 __device__ __forceinline__ V4<float> mul(const V4<float>& x, float y) { const f32x2 s = pack2(y, y); return {mul2(x.a, s), mul2(x.b, s)}; }
 __device__ __forceinline__ V4<float> mad(const V4<float>& x, const V4<float>& y, const V4<float>& z) { return {fma2(x.a, y.a, z.a), fma2(x.b, y.b, z.b)}; }
@@ -607,6 +628,7 @@ __device__ __forceinline__ void fold_halves(const V4<double>& x, int mask, doubl
  * channels of a warp (for dB, dC) are taken by exchanging halves between lanes, so that every lane ends with a sum of its own.
  * Lanes of odd channels hold their four states with the halves swapped (from copies of B and C in that order): the half to
  * give away is then in the same registers in every lane, and the first and largest exchange needs no selection.
+ * PADS: as in the forward call, for the states and their gradients.
  * AGG: as in the forward call, from the chunk's end: the gradient that leaves the chunk's first row when none enters at its
  * end, and the sum of the deltas.
  * About 28 instructions per row, channel and state, which bound it: 410 us at 2 x 2048 x 4096 x 16 (1100 us before loaders and
@@ -650,7 +672,7 @@ template <typename T> struct Grads {
 template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
-template <typename T, int P, bool AGG>
+template <typename T, int P, bool AGG, bool PADS>
 __global__ void __launch_bounds__(2 * NT, Backward<T, P>::RESIDENT)
 backward_kernel(Grads<T> out, typename AccOf<T>::type* __restrict__ chunk_g, typename AccOf<T>::type* __restrict__ chunk_s, const T* __restrict__ dy,
                 const typename AccOf<T>::type* __restrict__ dh_out, const T* __restrict__ x, const T* __restrict__ dt,
@@ -683,6 +705,9 @@ backward_kernel(Grads<T> out, typename AccOf<T>::type* __restrict__ chunk_g, typ
         const long long d = pl.d0 + ch;
         V4<A> rate, Av, g, dA;
         A sum = 0;
+        bool real[S];               /* PADS: the states in front of the last one, in this lane's order */
+#pragma unroll
+        for (int i = 0; i < S; ++i) real[i] = n0 + (odd ? i ^ 2 : i) < a.states;
         {
             A t0[S], t1[S], z0[S];
 #pragma unroll
@@ -748,6 +773,7 @@ backward_kernel(Grads<T> out, typename AccOf<T>::type* __restrict__ chunk_g, typ
                         const V4<A> cv = *reinterpret_cast<const V4<A>*>(cs + (r0 + k) * 2 * NP);
                         av[k] = decays(pr.delta, rate);
                         h[k] = mad(av[k], k ? h[k - 1] : h0, mul(bv, pr.dx));
+                        if (PADS) clear(h[k], real);
                         yv[k] = dot(h[k], cv);
                     }
                     /* M lanes of a warp hold the same states of M channels; MS rows give one sum (or two) per lane */
@@ -764,7 +790,8 @@ backward_kernel(Grads<T> out, typename AccOf<T>::type* __restrict__ chunk_g, typ
                         if (PARTIAL && k >= live) {
                             qv[k] = rv[k] = yv[k] = b2[0] = b2[1] = c2[0] = c2[1] = 0;
                         } else {
-                            const V4<A> dh = mad(cv, gy, g);
+                            V4<A> dh = mad(cv, gy, g);
+                            if (PADS) clear(dh, real);
                             g = mul(dh, av[k]);
                             const V4<A> da = mul(g, k ? h[k - 1] : h0);
                             qv[k] = dot(dh, bv);
@@ -1170,7 +1197,7 @@ struct Operands {
     const int* lengths;
 };
 
-template <typename T, int P>
+template <typename T, int P, bool PADS>
 int forward_p(void* y, void* h_out, void* saved, const Operands& o, const void* h_in, void* ws, const RpbScan* c, cudaStream_t s) {
     typedef typename AccOf<T>::type A;
     typedef Forward<T, P> Sh;
@@ -1205,14 +1232,14 @@ int forward_p(void* y, void* h_out, void* saved, const Operands& o, const void* 
     static unsigned char done[2][64];
     int device = 0;
     SEQ_CUDA(cudaGetDevice(&device));
-    if (allow_shared(forward_kernel<T, P, true>, sizeof(ForwardShared<T, P, true>), device, done[0]) ||
-        allow_shared(forward_kernel<T, P, false>, sizeof(ForwardShared<T, P, false>), device, done[1])) return -1;
+    if (allow_shared(forward_kernel<T, P, true, false>, sizeof(ForwardShared<T, P, true>), device, done[0]) ||
+        allow_shared(forward_kernel<T, P, false, PADS>, sizeof(ForwardShared<T, P, false>), device, done[1])) return -1;
     if (a.chunks > 1) {
-        SEQ_CUDA(rpb_launch(forward_kernel<T, P, true>, dim3((unsigned)blocks), dim3(NT + Forward<T, P>::NL), sizeof(ForwardShared<T, P, true>), s, 1, reinterpret_cast<T*>(y), ho, reinterpret_cast<A*>(saved),
+        SEQ_CUDA(rpb_launch(forward_kernel<T, P, true, false>, dim3((unsigned)blocks), dim3(NT + Forward<T, P>::NL), sizeof(ForwardShared<T, P, true>), s, 1, reinterpret_cast<T*>(y), ho, reinterpret_cast<A*>(saved),
                             chunk_h, chunk_s, x, dt, Am, B, C, Dv, bias, z, hi, o.lengths, a));
         rpb_count_launches(1);
     }
-    SEQ_CUDA(rpb_launch(forward_kernel<T, P, false>, dim3((unsigned)blocks), dim3(NT + Forward<T, P>::NL), sizeof(ForwardShared<T, P, false>), s, 1, reinterpret_cast<T*>(y), ho, reinterpret_cast<A*>(saved),
+    SEQ_CUDA(rpb_launch(forward_kernel<T, P, false, PADS>, dim3((unsigned)blocks), dim3(NT + Forward<T, P>::NL), sizeof(ForwardShared<T, P, false>), s, 1, reinterpret_cast<T*>(y), ho, reinterpret_cast<A*>(saved),
                         chunk_h, chunk_s, x, dt, Am, B, C, Dv, bias, z, hi, o.lengths, a));
     rpb_count_launches(1);
     return 0;
@@ -1223,7 +1250,7 @@ struct Wanted {
     int accumulate;
 };
 
-template <typename T, int P>
+template <typename T, int P, bool PADS>
 int backward_p(const Wanted& w, const void* dy, const void* dh_out, const Operands& o, const void* saved, void* ws, const RpbScan* c,
                cudaStream_t s) {
     typedef typename AccOf<T>::type A;
@@ -1260,12 +1287,12 @@ int backward_p(const Wanted& w, const void* dy, const void* dh_out, const Operan
     static unsigned char done[2][64];
     int device = 0;
     SEQ_CUDA(cudaGetDevice(&device));
-    if (allow_shared(backward_kernel<T, P, true>, agg, device, done[0]) || allow_shared(backward_kernel<T, P, false>, smem, device, done[1])) return -1;
+    if (allow_shared(backward_kernel<T, P, true, false>, agg, device, done[0]) || allow_shared(backward_kernel<T, P, false, PADS>, smem, device, done[1])) return -1;
     if (Sh::UNEVEN) {
         static int registers = 0;       /* the same on every device */
         if (registers == 0) {
             cudaFuncAttributes attr;
-            SEQ_CUDA(cudaFuncGetAttributes(&attr, backward_kernel<T, P, false>));
+            SEQ_CUDA(cudaFuncGetAttributes(&attr, backward_kernel<T, P, false, PADS>));
             registers = attr.numRegs;
         }
         if (registers != 128) return refuse("rp_selective_scan_grad_ex", "built with another number of registers than its kernel divides");
@@ -1273,11 +1300,11 @@ int backward_p(const Wanted& w, const void* dy, const void* dh_out, const Operan
     const A* dho = reinterpret_cast<const A*>(dh_out);
     const A* sv = reinterpret_cast<const A*>(saved);
     if (a.chunks > 1) {
-        SEQ_CUDA(rpb_launch(backward_kernel<T, P, true>, dim3((unsigned)blocks), dim3(2 * NT), agg, s, 1, out, chunk_g, chunk_s, g, dho, x, dt, Am, B, C, Dv, bias,
+        SEQ_CUDA(rpb_launch(backward_kernel<T, P, true, false>, dim3((unsigned)blocks), dim3(2 * NT), agg, s, 1, out, chunk_g, chunk_s, g, dho, x, dt, Am, B, C, Dv, bias,
                             z, o.lengths, sv, a));
         rpb_count_launches(1);
     }
-    SEQ_CUDA(rpb_launch(backward_kernel<T, P, false>, dim3((unsigned)blocks), dim3(2 * NT), smem, s, 1, out, chunk_g, chunk_s, g, dho, x, dt, Am, B, C, Dv, bias, z,
+    SEQ_CUDA(rpb_launch(backward_kernel<T, P, false, PADS>, dim3((unsigned)blocks), dim3(2 * NT), smem, s, 1, out, chunk_g, chunk_s, g, dho, x, dt, Am, B, C, Dv, bias, z,
                         o.lengths, sv, a));
     rpb_count_launches(1);
     if (w.dB || w.dC) {
@@ -1297,14 +1324,11 @@ int backward_p(const Wanted& w, const void* dy, const void* dh_out, const Operan
     return sum_parts<A>(d, parts, c->batch * a.chunks, D * (N + 2), s);
 }
 
+/* The lanes of a channel, and whether they have states behind the last one. */
 template <typename F> int by_lanes(int states, F f) {
-    switch (lanes_for(states)) {
-        case 1: return f(std::integral_constant<int, 1>());
-        case 2: return f(std::integral_constant<int, 2>());
-        case 4: return f(std::integral_constant<int, 4>());
-        case 8: return f(std::integral_constant<int, 8>());
-        case 16: return f(std::integral_constant<int, 16>());
-    }
+#define CASE(n) case n: return states == n * S ? f(std::integral_constant<int, n>(), std::false_type()) : f(std::integral_constant<int, n>(), std::true_type());
+    switch (lanes_for(states)) { CASE(1) CASE(2) CASE(4) CASE(8) CASE(16) }
+#undef CASE
     return -1;
 }
 
@@ -1385,7 +1409,7 @@ int rp_selective_scan_ex(void* y, void* h_out, void* saved, const void* x, const
     if (scope.enter(device_id)) return refuse(name, "no such device");
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     return by_type(dtype, [&](auto t) {
-        return by_lanes(c->states, [&](auto p) { return forward_p<decltype(t), decltype(p)::value>(y, h_out, saved, o, h_in, ws, c, s); });
+        return by_lanes(c->states, [&](auto p, auto pads) { return forward_p<decltype(t), decltype(p)::value, decltype(pads)::value>(y, h_out, saved, o, h_in, ws, c, s); });
     });
 }
 
@@ -1426,7 +1450,7 @@ int rp_selective_scan_grad_ex(void* dx, void* ddt, void* dA, void* dB, void* dC,
     const Wanted want = {dx, ddt, dA, dB, dC, dD, ddt_bias, dz, dh_in, accumulate};
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     return by_type(dtype, [&](auto t) {
-        return by_lanes(c->states, [&](auto p) { return backward_p<decltype(t), decltype(p)::value>(want, dy, dh_out, o, saved, ws, c, s); });
+        return by_lanes(c->states, [&](auto p, auto pads) { return backward_p<decltype(t), decltype(p)::value, decltype(pads)::value>(want, dy, dh_out, o, saved, ws, c, s); });
     });
 }
 

@@ -429,3 +429,55 @@ def test_an_infinite_gradient_of_A_stays_one(lib, dtype, n, d):
     _, _, saved = forward(lib, s, c, dtype, keep=True)
     got = backward(lib, s, c, dtype, saved)
     assert (got["dA"] == float("inf")).all() and (got["dh_in"] == float("inf")).all()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n", [1, 2, 3, 5, 6, 9, 17, 20, 33, 62])
+@pytest.mark.parametrize("length,d", [(1, 10), (45, 24), (400, 6)])
+def test_one_infinite_row_of_each_channel(lib, dtype, n, length, d):
+    """Channel c has one infinite x (then one infinite dy), with states, B and C of one sign: what follows it (backward: what is in front
+    of it) is infinite with the definition's sign, the rest as without it, however many states a thread has room for."""
+    s = make(1, length, d, n, 1, dtype, 51, state=True)
+    rows = (torch.arange(d) * 7) % length
+    at = (0, rows, torch.arange(d))
+    for k in ("B", "C", "h", "x", "D", "dy", "dh"):
+        s[k] = s[k].abs() + 0.01
+    s["A"][:] = -0.1
+    s["x"][at] = 0.5
+    s["dy"][at] = 0.5
+    s["z"] = s["z"].masked_fill(s["z"] == 0, 0.01)
+    c = geometry(s, n, 1, 1)
+    ref = reference(s, n, 1, 1, None, True, dtype)
+    t = torch.arange(length)[None, :, None]
+    behind = (t >= rows).expand(1, length, d)
+    s["x"][at] = float("inf")
+    y, h, saved = forward(lib, s, c, dtype, keep=True)
+    y2, h2, _ = forward(lib, s, c, dtype)                          # a single token has a kernel of its own
+    z = s["z"].double().cpu()
+    for got in (y, y2):
+        got = got.cpu()
+        assert torch.equal(got.double()[behind], (float("inf") * z.sign())[behind])
+        close(got[~behind], ref["y"][~behind], ref["y_slack"][~behind], "y")
+    assert (h == float("inf")).all() and (h2 == float("inf")).all()
+    dz = backward(lib, s, c, dtype, saved)["dz"].cpu()
+    slope = 1 + z * torch.sigmoid(-z)
+    assert torch.equal(dz.double()[behind], (float("inf") * slope.sign())[behind])
+    close(dz[~behind], ref["dz"][~behind], ref["dz_slack"][~behind], "dz")
+    # the gradients, without the gate
+    s["x"][at] = 0.5
+    s["z"] = None
+    c = geometry(s, n, 1, 1)
+    ref = reference(s, n, 1, 1, None, True, dtype)
+    _, _, saved = forward(lib, s, c, dtype, keep=True)
+    s["dy"][at] = float("inf")
+    got = {k: v.cpu() for k, v in backward(lib, s, c, dtype, saved).items() if v is not None}
+    front = (t <= rows).expand(1, length, d)
+    assert (got["dx"][front] == float("inf")).all()
+    close(got["dx"][~front], ref["dx"][~front], ref["dx_slack"][~front], "dx")
+    for k in ("dA", "dD", "dh_in"):
+        assert (got[k] == float("inf")).all(), k
+    hit = torch.zeros(length, dtype=torch.bool)
+    hit[rows] = True
+    for k, inf in (("dC", hit), ("dB", torch.arange(length) <= int(rows.max()))):
+        assert (got[k][:, inf] == float("inf")).all(), k
+        close(got[k][:, ~inf], ref[k][:, ~inf], ref[k + "_slack"][:, ~inf], k)
