@@ -51,8 +51,9 @@ __device__ __forceinline__ double decay(double delta, double a) { return exp(del
 /* A as the decay wants it: in float times log2(e), for the base-2 exponential; finite, so that a delta of 0 (a row that is not part of
  * the sequence) changes nothing whatever A is */
 __device__ __forceinline__ float decay_rate(float a) {
-    const float r = a * 1.44269504088896341f;
-    return isinf(r) ? copysignf(FLT_MAX, r) : r;
+    float r;        /* NaN stays NaN */
+    asm("{ .reg .f32 t; max.NaN.f32 t, %1, %2; min.NaN.f32 %0, t, %3; }" : "=f"(r) : "f"(a * 1.44269504088896341f), "f"(-FLT_MAX), "f"(FLT_MAX));
+    return r;
 }
 __device__ __forceinline__ double decay_rate(double a) { return isinf(a) ? copysign(DBL_MAX, a) : a; }
 
