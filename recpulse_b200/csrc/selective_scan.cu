@@ -584,6 +584,18 @@ template <typename A> __device__ __forceinline__ void clear(V4<A>& x, const bool
 }
 __device__ __forceinline__ V4<float> mul(const V4<float>& x, const V4<float>& y) { return {mul2(x.a, y.a), mul2(x.b, y.b)}; }
 __device__ __forceinline__ V4<float> mul(const V4<float>& x, float y) { const f32x2 s = pack2(y, y); return {mul2(x.a, s), mul2(x.b, s)}; }
+/* zeros formed from x: constants for them cost registers throughout the walk (594 us instead of 590 at 2 x 2048 x 4096 x 16); an
+ * infinite x times 0 is NaN, and the larger of NaN and 0 is 0 */
+__device__ __forceinline__ V4<float> zeros_like(const V4<float>& x) {
+    float v[S];
+    mul(x, 0.0f).get(v);
+#pragma unroll
+    for (int i = 0; i < S; ++i) v[i] = fmaxf(v[i], 0.0f);
+    V4<float> r;
+    r.set(v);
+    return r;
+}
+__device__ __forceinline__ V4<double> zeros_like(const V4<double>&) { return {{0, 0, 0, 0}}; }
 __device__ __forceinline__ V4<float> mad(const V4<float>& x, const V4<float>& y, const V4<float>& z) { return {fma2(x.a, y.a, z.a), fma2(x.b, y.b, z.b)}; }
 __device__ __forceinline__ V4<float> mad(const V4<float>& x, float y, const V4<float>& z) { const f32x2 s = pack2(y, y); return {fma2(x.a, s, z.a), fma2(x.b, s, z.b)}; }
 __device__ __forceinline__ float dot(const V4<float>& x, const V4<float>& y) {
@@ -756,8 +768,7 @@ backward_kernel(Grads<T> out, typename AccOf<T>::type* __restrict__ chunk_g, typ
             } else {
                 /* dA of one tile, then added to the total: sums of at most 16 and of as many as there are tiles, where one sum
                  * over all rows would have lost a digit */
-                V4<A> dA_tile;
-                { const A none[S] = {0, 0, 0, 0}; dA_tile.set(none); }
+                V4<A> dA_tile = zeros_like(dA);
                 /* PARTIAL: rows from `live` on are not part of the sequence (or the chunk).  Their decay is 1 and nothing enters,
                  * so the state and its gradient pass through them, and their results are 0 whatever the state holds. */
                 auto segment = [&](int r0, int live, auto partial) {
