@@ -481,3 +481,40 @@ def test_one_infinite_row_of_each_channel(lib, dtype, n, length, d):
     for k, inf in (("dC", hit), ("dB", torch.arange(length) <= int(rows.max()))):
         assert (got[k][:, inf] == float("inf")).all(), k
         close(got[k][:, ~inf], ref[k][:, ~inf], ref[k + "_slack"][:, ~inf], k)
+
+
+def unmasked(s, n, groups, softplus, dtype):
+    """Nothing overflows in the recurrence, so that no comparison with it is left out."""
+    ref = reference(s, n, groups, softplus, None, True, dtype)
+    assert all(torch.isfinite(v).all() for v in ref.values())
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n", [1, 4, 6, 16, 24, 33, 64])
+def test_step_sizes_given_as_they_are(lib, dtype, n):
+    """softplus = 0 with positive dt: the states stay finite, so every value and gradient is compared; whole and split sequences."""
+    for k, (batch, length, d, groups) in enumerate([(3, 17, 64, 2), (2, 33, 36, 3), (1, 300, 24, 1)]):
+        s = make(batch, length, d, n, groups, dtype, 61 * n + k, state=k != 0, gate=k != 1, bias=False)
+        s["dt"] = 0.3 * s["dt"].abs() + 0.01
+        unmasked(s, n, groups, 0, dtype)
+        check(lib, s, n, groups, 0, dtype, f"{dtype} n={n} {batch}x{length}x{d}/{groups}")
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n", [4, 8, 12, 16, 32, 64])
+@pytest.mark.parametrize("softplus", [0, 1])
+def test_split_sequences_in_whole_packs(lib, dtype, n, softplus):
+    """Split sequences whose every operand is aligned and whose blocks are full, two groups, two sequences: asynchronous copies in
+    both passes and both directions, with states entering and gradients leaving."""
+    lanes = 1
+    while 4 * lanes < n:
+        lanes *= 2
+    d, length = 2 * (128 // lanes), 300
+    s = make(2, length, d, n, 2, dtype, 67 + n, state=True, bias=softplus == 1)
+    s["B"], s["C"] = s["B"].contiguous(), s["C"].contiguous()
+    if not softplus:
+        s["dt"] = 0.3 * s["dt"].abs() + 0.01
+    assert all(s[k].data_ptr() % 16 == 0 and s[k].stride(1) * s[k].element_size() % 16 == 0 for k in ("x", "z", "dt", "B", "C", "dy"))
+    unmasked(s, n, 2, softplus, dtype)
+    c = check(lib, s, n, 2, softplus, dtype, f"{dtype} n={n} split")
+    assert lib.rp_selective_scan_ws_bytes(C.byref(c), CODE[dtype], 0) > 0          # it is split
