@@ -546,12 +546,15 @@ int backward_n(const Wanted& w, const void* dout, const void* dy, const Operands
     return sum_parts<T>(d, ws, (int)blocks, 3 * D, s);
 }
 
+/* The pack that rows between two boundaries need beyond the longest row is there only where rows are moved in packs. */
 template <typename T, typename F> int by_packs(int packs, bool whole, F f) {
 #define CASE(n) if (packs == n) return whole ? f(std::integral_constant<int, n>(), std::true_type()) : f(std::integral_constant<int, n>(), std::false_type());
+#define SPARE(n) if (packs == n && whole) return f(std::integral_constant<int, n>(), std::true_type());
     CASE(1) CASE(2)
-    if constexpr (sizeof(T) == 2) { CASE(3) }
-    if constexpr (sizeof(T) == 4) { CASE(4) CASE(5) }
-    if constexpr (sizeof(T) == 8) { CASE(4) CASE(8) CASE(9) }
+    if constexpr (sizeof(T) == 2) { SPARE(3) }
+    if constexpr (sizeof(T) == 4) { CASE(4) SPARE(5) }
+    if constexpr (sizeof(T) == 8) { CASE(4) CASE(8) SPARE(9) }
+#undef SPARE
 #undef CASE
     return -1;
 }

@@ -128,12 +128,6 @@ template <int CH> __device__ __forceinline__ Place place_of(const Args& a) {
     return p;
 }
 
-template <typename T, typename A>
-__device__ __forceinline__ A delta_of(T raw, A bias, int softplus) {
-    const A v = up(raw) + bias;
-    return softplus ? softplus_of(v) : v;
-}
-
 /* h across a chunk whose deltas add up to `sum` and that ends with `part` from zero.  The chunk's decay in two halves: it may be
  * beyond the type's range where its product with h is not, and a state of 0 stays 0 however fast states grow. */
 template <typename A> __device__ __forceinline__ void cross_chunk(A (&h)[S], const A (&part)[S], const A (&rate)[S], A sum) {
