@@ -103,8 +103,10 @@ __device__ __forceinline__ Pack<T, Width<T>::v> row_of(const T* x, const T* stat
     return lane.load(state + (long long)s * a.channels, state && s >= 0);
 }
 
-/* rows at a time, the next ones' values on their way meanwhile: 4 forward (2: 79 us instead of 71 at 4 x 4096 x 4096 bf16, 8: 103),
- * 2 backward (forward and backward of 3 x 1999 x 1531 f16: 56 us instead of 73, by its registers) */
+/* Rows at a time, the next ones' values on their way meanwhile: 4 forward (2: 79 us instead of 71 at 4 x 4096 x 4096 bf16, 8: 103),
+ * 2 backward.  Forward and backward kernels together, replayed from a graph, with 2 and with 4 rows backward: 47 and 64 us at
+ * 3 x 1999 x 1531 x 3 taps f16 (rows off the boundaries), 138 and 130 at 2 x 2048 x 4096 x 4 taps bf16, 73 and 72 at 2 x 2048 x
+ * 1024 x 8 taps float32. */
 constexpr int FORWARD_ROWS = 4, BACKWARD_ROWS = 2;
 
 /* The last W - 1 rows of x are kept in registers, so that x is read once but for W - 1 rows in front of each run. */
@@ -237,15 +239,10 @@ __global__ void __launch_bounds__(128) backward_kernel(T* dx, T* dstate_in, type
         for (int j = 0; j < H; ++j)
 #pragma unroll
             for (int i = 0; i < V; ++i) { win[j][i] = up(early[j].v[i]); dp[j][i] = 0; }
-        for (; t < stop; t += U) {
-            Pack<T, V> g[U];
-#pragma unroll
-            for (int k = 0; k < U; ++k) {
-                g[k] = gn[k];
-#pragma unroll
-                for (int i = 0; i < V; ++i) win[H + k][i] = up(xn[k].v[i]);
-            }
-            fetch(t + U);
+        /* U rows from t on.  INNER: all of them are the run's own, and every product of their gradients is with a row of the sequence;
+         * else each is looked at, since 0 times an infinity of x or of the filter is to be formed nowhere. */
+        auto rows = [&](auto inner, const Pack<T, V> (&g)[U]) {
+            constexpr bool INNER = decltype(inner)::value;
 #pragma unroll
             for (int k = 0; k < U; ++k) {
                 const int s = t + k;
@@ -255,9 +252,9 @@ __global__ void __launch_bounds__(128) backward_kernel(T* dx, T* dstate_in, type
 #pragma unroll
                     for (int j = 0; j < W; ++j)
                         if (j >= skip) pre += w[j][i] * win[k + j][i];
-                    const A d = s < stop && s < end ? up(g[k].v[i]) * act_slope(pre, a.silu) : A(0);
+                    const A d = INNER || (s < stop && s < end) ? up(g[k].v[i]) * act_slope(pre, a.silu) : A(0);
                     dp[H + k][i] = d;
-                    if (s < pl.t1 && s < end) {         /* the run's own rows: 0 times an infinity of the next run's is formed nowhere */
+                    if (INNER || (s < pl.t1 && s < end)) {
                         db[i] += d;
 #pragma unroll
                         for (int j = 0; j < W; ++j)
@@ -266,29 +263,21 @@ __global__ void __launch_bounds__(128) backward_kernel(T* dx, T* dstate_in, type
                 }
                 const int r = s - H;                /* the row whose gradient is complete now */
                 T* to = nullptr;
-                if (r >= pl.t1) break;
+                if (!INNER && r >= pl.t1) break;
                 if (r >= pl.t0) { if (ds) to = ds + r * a.dx_row; }
-                else if (pl.t0 == 0 && to_state && r >= -keep) to = to_state + (long long)(r + keep) * a.channels;
+                else if (!INNER && pl.t0 == 0 && to_state && r >= -keep) to = to_state + (long long)(r + keep) * a.channels;
                 if (!to) continue;
-                const int from_end = r - (end - keep);              /* row of the final state that is this row of xp */
                 A v[V];
 #pragma unroll
                 for (int i = 0; i < V; ++i) v[i] = 0;
-                if (r >= 0 && s < end) {
 #pragma unroll
-                    for (int i = 0; i < V; ++i)
+                for (int j = 0; j < W; ++j) {
+                    if (j < skip || !(INNER || (s - j >= 0 && s - j < end))) continue;
 #pragma unroll
-                        for (int j = 0; j < W; ++j)
-                            if (j >= skip) v[i] += w[j][i] * dp[H + k - j][i];
-                } else {                            /* rows that are not of the sequence form no product */
-#pragma unroll
-                    for (int j = 0; j < W; ++j)
-                        if (j >= skip && s - j >= 0 && s - j < end) {
-#pragma unroll
-                            for (int i = 0; i < V; ++i) v[i] += w[j][i] * dp[H + k - j][i];
-                        }
+                    for (int i = 0; i < V; ++i) v[i] += w[j][i] * dp[H + k - j][i];
                 }
-                if (more_from && from_end >= 0 && from_end < keep) {
+                const int from_end = r - (end - keep);              /* row of the final state that is this row of xp */
+                if (!INNER && more_from && from_end >= 0 && from_end < keep) {
                     const Pack<T, V> more = lane.load(more_from + (long long)from_end * a.channels, true);
 #pragma unroll
                     for (int i = 0; i < V; ++i) v[i] += up(more.v[i]);
@@ -300,6 +289,18 @@ __global__ void __launch_bounds__(128) backward_kernel(T* dx, T* dstate_in, type
                 }
                 lane.store(to, store_form<T, V>(v));
             }
+        };
+        for (; t < stop; t += U) {
+            Pack<T, V> g[U];
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                g[k] = gn[k];
+#pragma unroll
+                for (int i = 0; i < V; ++i) win[H + k][i] = up(xn[k].v[i]);
+            }
+            fetch(t + U);
+            if (t >= H && t + U <= pl.t1 && t + U <= end) rows(std::true_type(), g);
+            else rows(std::false_type(), g);
 #pragma unroll
             for (int j = 0; j < H; ++j)
 #pragma unroll
@@ -331,9 +332,9 @@ __global__ void __launch_bounds__(128) backward_kernel(T* dx, T* dstate_in, type
 }
 
 /* Rows per thread.  A run costs W - 1 (backward: 2 (W - 1)) rows of extra reading, which the longest run makes
- * cheapest; it is halved while the runs do not fill the chip with `warps` warps (16 per SM
- * forward; 8 backward, whose runs cost twice as much: 52 us instead of 56 at 3 x 1999 x 1531).  At least 8, so that only the first run of
- * a sequence reaches back to the state. */
+ * cheapest; it is halved while the runs do not fill the chip with `warps` warps: 16 per SM forward, 8 backward, whose runs cost
+ * twice as much (with 8 and with 16, at the three shapes above: 47 and 51, 138 and 124, 73 and 98 us).  At least 8, so that only
+ * the first run of a sequence reaches back to the state. */
 int pick_run(long long batch, int len, long long n_vec, int longest, int warps) {
     int run = longest;
     while (run > 8 && batch * ((len + run - 1) / run) * n_vec < (long long)warps * 32) run /= 2;
