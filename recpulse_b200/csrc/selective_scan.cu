@@ -635,7 +635,8 @@ __device__ __forceinline__ void fold_halves(const V4<double>& x, int mask, doubl
  * channels of a warp (for dB, dC) are taken by exchanging halves between lanes, so that every lane ends with a sum of its own.
  * Lanes of odd channels hold their four states with the halves swapped (from copies of B and C in that order): the half to
  * give away is then in the same registers in every lane, and the first and largest exchange needs no selection.
- * PADS: as in the forward call, for the states and their gradients.
+ * PADS: as in the forward call, for the states and their gradients; those of channels behind a group's last one too, whose zeros
+ * would be multiplied by an infinite B or C on the way into dB and dC.
  * AGG: as in the forward call, from the chunk's end: the gradient that leaves the chunk's first row when none enters at its
  * end, and the sum of the deltas.
  * About 28 instructions per row, channel and state, which bound it: 410 us at 2 x 2048 x 4096 x 16 (1100 us before loaders and
@@ -712,9 +713,9 @@ backward_kernel(Grads<T> out, typename AccOf<T>::type* __restrict__ chunk_g, typ
         const long long d = pl.d0 + ch;
         V4<A> rate, Av, g, dA;
         A sum = 0;
-        bool real[S];               /* PADS: the states in front of the last one, in this lane's order */
+        bool real[S];               /* PADS: the channel's states, in this lane's order */
 #pragma unroll
-        for (int i = 0; i < S; ++i) real[i] = n0 + (odd ? i ^ 2 : i) < a.states;
+        for (int i = 0; i < S; ++i) real[i] = on && n0 + (odd ? i ^ 2 : i) < a.states;
         {
             A t0[S], t1[S], z0[S];
 #pragma unroll
@@ -1330,9 +1331,13 @@ int backward_p(const Wanted& w, const void* dy, const void* dh_out, const Operan
     return sum_parts<A>(d, parts, c->batch * a.chunks, D * (N + 2), s);
 }
 
-/* The lanes of a channel, and whether they have states behind the last one. */
-template <typename F> int by_lanes(int states, F f) {
-#define CASE(n) case n: return states == n * S ? f(std::integral_constant<int, n>(), std::false_type()) : f(std::integral_constant<int, n>(), std::true_type());
+/* The lanes of a channel, and whether they have states behind the last one (or, where `per_group` is given, a group's last block
+ * channels behind the last one). */
+template <typename F> int by_lanes(int states, int per_group, F f) {
+#define CASE(n)                                                                                              \
+    case n:                                                                                                  \
+        return states == n * S && per_group % (NT / n) == 0 ? f(std::integral_constant<int, n>(), std::false_type()) \
+                                                            : f(std::integral_constant<int, n>(), std::true_type());
     switch (lanes_for(states)) { CASE(1) CASE(2) CASE(4) CASE(8) CASE(16) }
 #undef CASE
     return -1;
@@ -1415,7 +1420,7 @@ int rp_selective_scan_ex(void* y, void* h_out, void* saved, const void* x, const
     if (scope.enter(device_id)) return refuse(name, "no such device");
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     return by_type(dtype, [&](auto t) {
-        return by_lanes(c->states, [&](auto p, auto pads) { return forward_p<decltype(t), decltype(p)::value, decltype(pads)::value>(y, h_out, saved, o, h_in, ws, c, s); });
+        return by_lanes(c->states, 0, [&](auto p, auto pads) { return forward_p<decltype(t), decltype(p)::value, decltype(pads)::value>(y, h_out, saved, o, h_in, ws, c, s); });
     });
 }
 
@@ -1456,7 +1461,7 @@ int rp_selective_scan_grad_ex(void* dx, void* ddt, void* dA, void* dB, void* dC,
     const Wanted want = {dx, ddt, dA, dB, dC, dD, ddt_bias, dz, dh_in, accumulate};
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     return by_type(dtype, [&](auto t) {
-        return by_lanes(c->states, [&](auto p, auto pads) { return backward_p<decltype(t), decltype(p)::value, decltype(pads)::value>(want, dy, dh_out, o, saved, ws, c, s); });
+        return by_lanes(c->states, c->channels / c->groups, [&](auto p, auto pads) { return backward_p<decltype(t), decltype(p)::value, decltype(pads)::value>(want, dy, dh_out, o, saved, ws, c, s); });
     });
 }
 

@@ -518,3 +518,26 @@ def test_split_sequences_in_whole_packs(lib, dtype, n, softplus):
     unmasked(s, n, 2, softplus, dtype)
     c = check(lib, s, n, 2, softplus, dtype, f"{dtype} n={n} split")
     assert lib.rp_selective_scan_ws_bytes(C.byref(c), CODE[dtype], 0) > 0          # it is split
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n,d,groups", [(16, 24, 1), (4, 130, 1), (8, 40, 2), (64, 9, 1), (6, 64, 1)])
+def test_infinite_B_and_C_and_channels_that_leave_lanes_idle(lib, dtype, n, d, groups):
+    """One infinite row of B, then of C, everything of one sign: dC (dB) is the infinity of the definition from (up to) that row on, also
+    where a block has lanes for channels that are not there."""
+    length, r = 45, 20
+    s = make(1, length, d, n, groups, dtype, 71, state=True, gate=False)
+    for k in ("B", "C", "h", "x", "D", "dy", "dh"):
+        s[k] = s[k].abs() + 0.01
+    s["A"][:] = -0.1
+    c = geometry(s, n, groups, 1)
+    for name, key, rows, wide in (("B", "dC", slice(r, None), slice(None, r)), ("C", "dB", slice(None, r + 1), slice(r + 1, None))):
+        ref = reference(s, n, groups, 1, None, True, dtype)
+        keep = s[name]
+        s[name] = keep.clone()
+        s[name][:, r] = float("inf")
+        _, _, saved = forward(lib, s, c, dtype, keep=True)
+        got = {k: v.cpu() for k, v in backward(lib, s, c, dtype, saved).items() if v is not None}
+        assert (got[key][:, rows] == float("inf")).all(), key
+        close(got[key][:, wide], ref[key][:, wide], ref[key + "_slack"][:, wide], key)
+        s[name] = keep
