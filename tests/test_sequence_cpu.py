@@ -284,13 +284,13 @@ def test_buffers_off_their_elements_are_refused(dtype, size, capfd):
 
     def refused(fn, names, sizes, tail):
         """Every buffer in turn one byte (half an element) off, the others where they belong."""
-        places = [None if s is None else at(start + 3072 * i) for i, s in enumerate(sizes)]
+        places = [None if s is None else at(start + 2960 * i) for i, s in enumerate(sizes)]
         for i, (name, s) in enumerate(zip(names, sizes)):
             if s is None or name is None:
                 continue
             for shift in {1, s // 2}:
                 now = list(places)
-                now[i] = at(start + 3072 * i + shift)
+                now[i] = at(start + 2960 * i + shift)
                 capfd.readouterr()
                 assert fn(*now, *tail) == -1
                 assert f"{name} is not aligned" in capfd.readouterr().err, name
