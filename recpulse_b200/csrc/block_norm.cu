@@ -4,8 +4,10 @@
  *   y = out rsqrt(mean out^2 + eps_before) w_before.
  * Backward: with t = v i (i = rsqrt(mean v^2 + eps)) and m the gradient of t, dv = i (m - t mean(m t)); y's norm likewise.
  * A block of threads holds a whole row in registers, so each operand is read once and the row's sums are taken from there.
- * Memory bounds it (51 us for the forward call at 8192 x 4096 bf16); it takes 84 us there, for the instructions of two block sums
- * per row, and 100 us for the backward call at 4001 x 2999 f16.
+ * Its floor is memory (51 us for the forward call at 8192 x 4096 bf16); it takes 84 us there, for the latency of two block sums per row,
+ * and 100 us for the backward call at 4001 x 2999 f16, with three (there the forward call's issue slots are 68% busy, the backward
+ * call's 50%).  Rows of up to 256 16-bit channels have a block of one warp each, of which too few run at once: 37 us at 32768 x 128
+ * bf16 against 6, and 260 us forward and backward against 13.
  */
 #include "seq_common.cuh"
 
@@ -460,7 +462,8 @@ template <typename T> void shape_of(int channels, bool spare, int* packs, int* t
 /* Blocks of the backward call: each leaves one part of the weights' gradients behind.  A multiple of 8, so that the classes of
  * rows (8 at most) share them evenly. */
 long long backward_blocks(const RpbBlockNorm* c) {
-    const long long most = c->channels > 2048 ? SM_COUNT / 8 * 8 : SM_COUNT * 2;        /* as many as the registers hold at once */
+    /* what the registers hold at once of blocks of 256 threads and more; of narrower ones they would hold more */
+    const long long most = c->channels > 2048 ? SM_COUNT / 8 * 8 : SM_COUNT * 2;
     const long long rows = (c->rows + 7) / 8 * 8;
     return rows < most ? rows : most;
 }

@@ -1,9 +1,10 @@
 /*
  * Short causal convolution along a sequence, one filter per channel, with its SiLU and its gradients:
  *   pre[b,t,d] = bias[d] + sum over j < width of w[d,j] * xp[b,t+j,d],   y = pre or pre / (1 + exp(-pre))
- * where xp is x behind width-1 earlier rows (the state of the sequence, or zeros).  Memory bounds it: 41 us for reading and writing
- * 4 x 4096 x 4096 bf16 at the measured copy rate; the forward kernel takes 71 us there (16 bytes per thread and window moves took
- * 119 us).
+ * where xp is x behind width-1 earlier rows (the state of the sequence, or zeros).  Its floor is memory: 41 us for reading and writing
+ * 4 x 4096 x 4096 bf16 at the measured copy rate (about 30 with the lengths measured); the forward kernel takes 71 us there (16 bytes
+ * per thread and window moves took 119 us).  About 25 instructions per value are some 32 us of issue; five warps per scheduler at 95
+ * registers do not overlap them with the loads that they wait for (issue slots 48% busy).
  */
 #include "seq_common.cuh"
 

@@ -2,8 +2,9 @@
  * Selective state space scan: per sequence and channel a vector h of `states` values with
  *   delta = dt + dt_bias (behind a softplus when asked for),   h_t = exp(delta A) h_{t-1} + delta x_t B_t,
  *   y_t = C_t . h_t + D x_t,   out = y (or y z / (1 + exp(-z))).
- * B and C are shared by the channels of a group.  One exponential per row, channel and state bounds it (16 per clock and SM):
- * 119 us at 2 x 4096 x 4096 x 16, where the forward kernel takes 264 us with two walking warps per scheduler.  Backward, with dy the gradient of y:
+ * B and C are shared by the channels of a group.  One exponential per row, channel and state (16 per clock and SM) is the floor:
+ * 119 us at 2 x 4096 x 4096 x 16, where the forward kernel takes 264 us: it waits, with two walking warps per scheduler and the
+ * issue slots 48% busy, for shared memory, for arithmetic and at the barrier of each tile.  Backward, with dy the gradient of y:
  *   dh_t = C_t dy_t + a_{t+1} dh_{t+1},  a = exp(delta A);   da_t = dh_t h_{t-1} a_t (by the exponent)
  *   dA = sum of da delta,  ddelta = sum_n (da A + dh B x),  dx = delta sum_n dh B + D dy,
  *   dB = sum over channels of dh delta x,  dC = sum over channels of dy h,  dD = sum of dy x.
@@ -44,7 +45,8 @@ template <typename A> struct Pair { A delta, dx; };
 /* The hardware's base-2 exponential is low on average: by 0.5e-8 to 2.5e-8 of its value for arguments from -1e-4 to -0.3
  * (2^20 each), and a state that decays slowly collects that over its whole memory: dA over 2 x 2048 rows was 9e-7 low on
  * average.  This much more in the exponent, in the multiply-add that forms it, leaves 9e-8 (3.6e-8 overshoots to +2.8e-7);
- * 2^CENTRE itself still is 1, so a delta of 0 changes nothing. */
+ * 2^CENTRE itself still is 1, so a delta of 0 changes nothing.  It is added to every exponent; those beyond -0.3, behind which little
+ * of a state is left, were not measured one by one. */
 constexpr float CENTRE = 2.5e-8f;
 __device__ __forceinline__ float decay(float delta, float a) { return ex2_fast(fmaf(delta, a, CENTRE)); }
 __device__ __forceinline__ double decay(double delta, double a) { return exp(delta * a); }
@@ -639,8 +641,9 @@ __device__ __forceinline__ void fold_halves(const V4<double>& x, int mask, doubl
  * would be multiplied by an infinite B or C on the way into dB and dC.
  * AGG: as in the forward call, from the chunk's end: the gradient that leaves the chunk's first row when none enters at its
  * end, and the sum of the deltas.
- * About 28 instructions per row, channel and state, which bound it: 410 us at 2 x 2048 x 4096 x 16 (1100 us before loaders and
- * walkers were apart and the exchanges without selections). */
+ * About 28 instructions per row, channel and state are 209 us of issue at 2 x 2048 x 4096 x 16, where it takes 410 us (1100 us before
+ * loaders and walkers were apart and the exchanges without selections): the issue slots are 57% busy, and what the two walking
+ * warps per scheduler wait for is arithmetic, shared memory and the barrier of each tile, in that order. */
 template <typename T, int P> struct Backward {
     static constexpr int CH = NT / P, TT = P == 1 || sizeof(T) == 8 ? 8 : 16, NP = S * P, NL = NT;
     static constexpr int V = CH * TT >= NL ? CH * TT / NL : 1, K = CH / V;      /* loaders behind the TT-th row have nothing to do */

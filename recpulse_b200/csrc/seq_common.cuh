@@ -131,8 +131,9 @@ __device__ __forceinline__ float logistic(float v) { return reciprocal(1.0f + ex
 __device__ __forceinline__ double logistic(double v) { return 1.0 / (1.0 + exp(-v)); }
 
 /* log(1 + exp(v)) = max(v, 0) + log(1 + e) with e = exp(-|v|) in (0, 1]; log(1 + e) / e as a polynomial of degree 9
- * (Chebyshev interpolation on [0, 1]), within 2.2 half-steps of float32 as computed here: a third of log1pf's instructions,
- * and no cancellation for small e */
+ * (Chebyshev interpolation on [0, 1]), within 2.2 half-steps of float32 for the e that it is given: a third of log1pf's instructions,
+ * and no cancellation for small e.  e carries exp_of's error, which for v far below 0, where the result is e, is the result's: within
+ * (2 + |v|) steps more */
 __device__ __forceinline__ float softplus_of(float v) {
     const float e = exp_of(-fabsf(v));
     float p = -0.0031760570127516985f;
